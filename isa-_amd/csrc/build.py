@@ -1,7 +1,8 @@
-"""Build libisa_ekv_hip.so (gfx950) in-tree with hipcc.
+"""Build the HIP libraries (gfx950) in-tree with hipcc.
 
 Usage: ``python isa-_amd/csrc/build.py`` (also called by ``__graft_entry__.build()``).
-The library lands next to its ctypes loader in ``isa/kernels/transformer_ffn/``.
+Each library lands next to its ctypes loader: ``libisa_ekv_hip.so`` in
+``isa/kernels/transformer_ffn/``, ``libisa_block_hip.so`` in ``isa/kernels/transformer_block/``.
 """
 
 from __future__ import annotations
@@ -10,6 +11,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 CSRC = Path(__file__).resolve().parent
@@ -18,6 +21,8 @@ REPO = PKG_ROOT.parent
 SOURCES = [CSRC / "ekv_lut.hip"]
 INCLUDE = REPO / "include"
 OUT = PKG_ROOT / "isa" / "kernels" / "transformer_ffn" / "libisa_ekv_hip.so"
+BLOCK_SOURCES = [CSRC / f"block_{name}.hip" for name in ("api", "norm", "attention", "loss")]
+BLOCK_OUT = PKG_ROOT / "isa" / "kernels" / "transformer_block" / "libisa_block_hip.so"
 ARCH = os.environ.get("ISA_EKV_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [
@@ -39,19 +44,43 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found: set HIPCC or install ROCm")
 
 
-def build(verbose: bool = False) -> Path:
-    tmp = OUT.with_suffix(".so.tmp")
-    cmd = [hipcc(), *HIPCC_FLAGS, f"-I{INCLUDE}", "-o", str(tmp), *map(str, SOURCES)]
+def _run(cmd: list, verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
+
+
+def _ekv(verbose: bool) -> None:
+    tmp = OUT.with_suffix(".so.tmp")
+    _run([hipcc(), *HIPCC_FLAGS, f"-I{INCLUDE}", "-o", str(tmp), *map(str, SOURCES)], verbose)
     os.replace(tmp, OUT)
+
+
+def _block(verbose: bool, pool: ThreadPoolExecutor) -> None:
+    compile_flags = [f for f in HIPCC_FLAGS if f != "-shared"]
+    tmp = BLOCK_OUT.with_suffix(".so.tmp")
+    with tempfile.TemporaryDirectory() as work:
+        objects = [str(Path(work) / f"{src.stem}.o") for src in BLOCK_SOURCES]
+        jobs = [pool.submit(_run, [hipcc(), *compile_flags, f"-I{INCLUDE}", "-c", "-o", obj, str(src)], verbose)
+                for src, obj in zip(BLOCK_SOURCES, objects)]
+        for job in jobs:
+            job.result()
+        _run([hipcc(), *HIPCC_FLAGS, "-o", str(tmp), *objects], verbose)
+    os.replace(tmp, BLOCK_OUT)
+
+
+def build(verbose: bool = False) -> Path:
+    """Compile both libraries, the block's sources and the projection's side by side; returns the latter's path."""
+    with ThreadPoolExecutor(max_workers=1 + len(BLOCK_SOURCES)) as pool:
+        ekv = pool.submit(_ekv, verbose)
+        _block(verbose, pool)
+        ekv.result()
     return OUT
 
 
 if __name__ == "__main__":
     path = build(verbose=True)
-    print(f"built {path}")
+    print(f"built {path}\nbuilt {BLOCK_OUT}")
     sys.exit(0)
