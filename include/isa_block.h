@@ -84,7 +84,8 @@ typedef struct isa_block_attention {
     const int32_t* key_lengths; /* [batch], or null */
     /* [batch][queries][heads][head_dim] and [batch][keys][kv_heads][head_dim] with the strides of
      * batch, token and head; a head's elements are adjacent. Pointers are 16-byte aligned and
-     * strides multiples of 8 elements; so is head_dim, at most ISA_BLOCK_ATTENTION_MAX_DIM. */
+     * strides multiples of 8 elements, those of tokens at least head_dim elements and under
+     * 16 MiB; head_dim is a multiple of 8, at most ISA_BLOCK_ATTENTION_MAX_DIM. */
     const void *q, *k, *v;
     int64_t q_strides[3], k_strides[3], v_strides[3];
 } isa_block_attention;
@@ -92,9 +93,10 @@ typedef struct isa_block_attention {
 
 size_t isa_block_attention_forward_workspace(const isa_block_attention* att);
 
-/* out [batch][queries][heads][head_dim]. For a backward call: lse [batch][heads][queries] fp32 (the
- * base-2 logarithm of the sum of a row's exponentials, -inf for a row that sees nothing), and with
- * 16-bit types rest, shaped and typed as out: what out's rounding left. Both may be null. */
+/* out [batch][queries][heads][head_dim]. For a backward call: lse [batch][heads][queries][2] fp32 (two
+ * numbers whose sum is the base-2 logarithm of the sum of a row's exponentials, the first -inf for
+ * a row that sees nothing), and with 16-bit types rest, shaped and typed as out: what out's rounding
+ * left. Both may be null. */
 int isa_block_attention_forward(const isa_block_attention* att, void* out, void* rest, float* lse, void* workspace,
                                 size_t workspace_bytes, void* stream);
 

@@ -1,0 +1,348 @@
+// What the attention's forward and backward share: operands of the matrix cores, tiles in LDS, spans
+// of keys. block_attention.hip describes the whole.
+#pragma once
+
+#include <algorithm>
+#include <climits>
+
+#include "block_common.hpp"
+
+namespace isa_block {
+
+constexpr int kTile = 32;  // of the matrix instruction, both ways
+constexpr float kLog2E = 1.44269504088896340736f;
+constexpr int kMaxLength = 1 << 30;
+
+using acc16 = vec<float, 16>;
+
+struct AttnArgs {
+    const void *q, *k, *v, *out, *dout;
+    void *result, *rest, *dk, *dv;  // result: out, or dq
+    float *lse, *delta, *partial;
+    const int32_t* lengths;
+    int64_t qs[3], ks[3], vs[3], gs[3];
+    int batch, queries, keys, heads, kv_heads, group, dim, window, sinks;
+    int splits;         // forward: blocks that share a tile of rows
+    int near, far;      // dk, dv: blocks that share a tile of keys, and one that holds sinks
+    int far_tiles;      // tiles of keys that hold sinks
+    float c, c_rest, scale;  // scale log2 e as two floats
+};
+
+// ---- fragments: 16 bytes a lane: of an operand's row lane % 32, one of the two chunks of a step -----
+
+template <typename T>
+struct Frag {
+    static constexpr int N = 16 / sizeof(T);  // elements
+    using V = vec<T, N>;
+};
+
+__device__ __forceinline__ void mma(acc16& acc, vec<bf16, 8> a, vec<bf16, 8> b) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(acc16& acc, vec<f16, 8> a, vec<f16, 8> b) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, acc, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(acc16& acc, vec<float, 4> a, vec<float, 4> b) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], acc, 0, 0, 0);
+}
+
+// Values u N .. u N + N - 1 of a lane's column of a product, as an operand of the next one.
+template <typename T>
+__device__ __forceinline__ typename Frag<T>::V operand(const acc16& x, int u) {
+    typename Frag<T>::V f;
+#pragma unroll
+    for (int e = 0; e < Frag<T>::N; ++e) f[e] = static_cast<T>(x[u * Frag<T>::N + e]);
+    return f;
+}
+
+// sum plus an operand's values as they were rounded: a row's weights, whose sum is what they are
+// divided by, then add up to 1 as the product sees them.
+__device__ __forceinline__ float add_all(vec<bf16, 8> x, float sum) {
+    const vec<bf16, 2> one = {static_cast<bf16>(1.0f), static_cast<bf16>(1.0f)};
+#pragma unroll
+    for (int e = 0; e < 8; e += 2)
+        sum = __builtin_amdgcn_fdot2_f32_bf16(vec<bf16, 2>{x[e], x[e + 1]}, one, sum, false);
+    return sum;
+}
+__device__ __forceinline__ float add_all(vec<f16, 8> x, float sum) {
+    const vec<f16, 2> one = {static_cast<f16>(1.0f), static_cast<f16>(1.0f)};
+#pragma unroll
+    for (int e = 0; e < 8; e += 2)
+        sum = __builtin_amdgcn_fdot2(vec<f16, 2>{x[e], x[e + 1]}, one, sum, false);
+    return sum;
+}
+__device__ __forceinline__ float add_all(vec<float, 4> x, float sum) { return sum + ((x[0] + x[1]) + (x[2] + x[3])); }
+
+// The row of a 32-row product that register i of a lane in `half` holds.
+__device__ __forceinline__ constexpr int product_row(int i, int half) { return 8 * (i / 4) + 4 * half + i % 4; }
+
+// exp2(s c - base). In fp32 c is two floats: its rounding alone, times a score, would be an error of
+// the size of all others together.
+template <typename T>
+__device__ __forceinline__ float weight(float s, float c, float c_rest, float base) {
+    float x = fmaf(s, c, -base);
+    if constexpr (sizeof(T) == 4) x = s == -INFINITY ? x : fmaf(s, c_rest, x);  // (masked)
+    return __builtin_amdgcn_exp2f(x);
+}
+
+// ---- tiles in LDS -----------------------------------------------------------------------------
+// A row's 16-byte chunks lie in a power of two of slots, chunk c in slot c ^ key(row), so that both
+// kinds of reads use all banks: 16 rows' of one chunk, and 4 rows' of 4 adjacent chunks (the
+// transposing read: with keys that leave those 4 chunks in their 64 bytes it takes twice the time).
+// Tiles are loaded straight to LDS, 64 slots an
+// instruction; a buffer descriptor that ends with the last row makes what is behind it zeros.
+
+constexpr int slots_for(int chunks) { return chunks <= 4 ? 4 : chunks <= 8 ? 8 : chunks <= 16 ? 16 : 32; }
+
+template <typename T, int D>
+struct Tile {
+    static constexpr int N = Frag<T>::N;
+    static constexpr int kChunks = D / N;
+    static constexpr int kSlots = slots_for(kChunks);
+    static constexpr int kPitch = kSlots * N;              // elements
+    static constexpr int kSteps = kChunks / 2;             // of a product over D
+    static constexpr int kUses = kTile / (2 * N);          // operand()s of 32 rows
+    using V = typename Frag<T>::V;
+
+    // 256 bytes of banks: 4, 2, 1 or half a row
+    static __device__ __forceinline__ constexpr int key(int row) {
+        const int by_four = row / 4 % 4;
+        return kSlots == 4 ? by_four : kSlots == 8 ? row / 2 % 2 * 4 + by_four : row % 4 * 4 + by_four;
+    }
+
+    // of row (r0 + lane % 32), the dims of step t
+    static __device__ __forceinline__ V row(const T* tile, int r0, int t, int lane) {
+        const int r = lane % 32;
+        return *reinterpret_cast<const V*>(tile + r0 * kPitch + r * kPitch + ((2 * t + lane / 32) ^ key(r)) * N);
+    }
+
+    // of column (32 db + lane % 32), the rows r0 .. r0 + 31 that operand(x, u) holds in this half
+    static __device__ __forceinline__ V column(const T* tile, int r0, int u, int db, int lane) {
+        if constexpr (sizeof(T) == 4) {
+            V f;
+            const int at = 8 * db + lane % 32 / 4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = 8 * u + 4 * (lane / 32) + e;
+                f[e] = tile[r0 * kPitch + r * kPitch + (at ^ key(r)) * N + lane % 4];
+            }
+            return f;
+        } else {
+            // the transposing read: 16 lanes give the addresses of 4 rows x 16 columns, 4 columns each,
+            // and get a column's 4 rows each
+            using s4 = vec<short, 4>;
+            using lds = __attribute__((address_space(3))) s4;
+            union {
+                s4 part[2];
+                V f;
+            } x;
+            const int at = 4 * db + lane / 16 % 2 * 2 + lane % 4 / 2;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int r = 8 * j + 4 * (lane / 32) + lane % 16 / 4;  // 16 u further on the key is the same
+                const T* p = tile + (r0 + 16 * u) * kPitch + r * kPitch + (at ^ key(r)) * N + lane % 2 * 4;
+                x.part[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)const_cast<T*>(p));
+            }
+            return x.f;
+        }
+    }
+};
+
+using LdsPtr = __attribute__((address_space(3))) void*;
+constexpr int kBufferFlags = 0x00027000;  // raw buffer of 32-bit data
+constexpr unsigned kOutside = 0x7fffffffu;
+
+// COUNT times BYTES a lane, `step` bytes of LDS apart, from the buffer of `size` bytes at `base` (uniform); what lies outside is zeros.
+// (The buffer's type exists for the device alone: the host's pass over the kernels does without.)
+template <int BYTES, int COUNT>
+__device__ __forceinline__ void load_to_lds(void* to, const void* base, int size, const unsigned (&at)[COUNT],
+                                            int step) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, size, kBufferFlags);
+#pragma unroll
+    for (int n = 0; n < COUNT; ++n)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (LdsPtr)(static_cast<char*>(to) + n * step), BYTES, at[n], 0, 0,
+                                                 0);
+#endif
+}
+
+// One block's (or wave's) copies of ROWS rows at a time from memory to a tile.
+template <typename T, int D, int ROWS, int THREADS>
+struct Loader {
+    using L = Tile<T, D>;
+    static constexpr int kEach = ROWS * L::kSlots / THREADS;
+    static_assert(ROWS * L::kSlots % THREADS == 0);
+    unsigned at[kEach];  // a lane's byte offsets from the tile's first row
+    const char* base;    // of row 0 (uniform)
+    int stride;          // bytes between rows, under 2^24
+
+    // `thread`: of THREADS
+    __device__ __forceinline__ Loader(const T* base_, int64_t row_stride, int dim, int thread)
+        : base(reinterpret_cast<const char*>(base_)), stride(static_cast<int>(row_stride * sizeof(T))) {
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) {
+            const int slot = thread + n * THREADS, row = slot / L::kSlots;
+            const int chunk = slot % L::kSlots ^ L::key(row);
+            at[n] = chunk * L::N < dim ? static_cast<unsigned>(row * stride) + chunk * 16 : kOutside;
+        }
+    }
+
+    // rows first .. first + ROWS - 1; those from `end` on become zeros
+    __device__ __forceinline__ void load(T* tile, int first, int end, int wave) const {
+        load_from(tile, base + static_cast<int64_t>(first) * stride, end - first, wave);
+    }
+    __device__ __forceinline__ void load_from(T* tile, const char* from, int left, int wave) const {
+        load_to_lds<16, kEach>(tile + wave * kWave * L::N, from, min(max(left, 0), ROWS) * stride, at, THREADS * 16);
+    }
+};
+
+// 64 floats to LDS by one wave; from `end` on zeros.
+__device__ __forceinline__ void load_floats(float* to, const float* base, int64_t first, int count, int lane) {
+    const unsigned at[1] = {static_cast<unsigned>(lane) * 4};
+    load_to_lds<4, 1>(to, base + first, max(count, 0) * 4, at, 0);
+}
+
+// All of this wave's loads to LDS have arrived.
+__device__ __forceinline__ void loads_arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Dispatch gives block i to XCD i % 8; this gives each XCD a run of adjacent work, whose keys its
+// L2 then holds once.
+__device__ __forceinline__ int xcd_order(int id, int n) {
+    const int per = n / 8, rest = n % 8, x = id % 8;
+    return x * per + min(x, rest) + id / 8;
+}
+
+// x, of which the compiler knows nothing: what follows from it is computed again in each turn of a loop
+// instead of being held in registers.
+__device__ __forceinline__ int opaque(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// ---- which keys a block of rows sees --------------------------------------------------------
+
+__device__ __forceinline__ int length_of(const AttnArgs& a, int b) {
+    return a.lengths ? min(max(a.lengths[b], 0), a.keys) : a.keys;
+}
+
+__device__ __forceinline__ bool sees(const AttnArgs& a, int p, int j) {
+    return (j <= p) & ((j < a.sinks) | (j > p - a.window));  // without branches
+}
+
+// The tiles of BN keys that some query at pmin .. pmax sees: those of the sinks 0 .. sink - 1 that
+// lie before the window's, then those of lo .. hi - 1, starting at lo.
+template <int BN>
+struct Span {
+    int lo, hi, sink, sink_tiles, count;
+
+    __device__ __forceinline__ Span(const AttnArgs& a, int pmin, int pmax) {
+        hi = pmax + 1;
+        lo = max(0, pmin - a.window + 1);
+        if (a.sinks >= lo) lo = 0;
+        sink = min(a.sinks, lo);
+        sink_tiles = (sink + BN - 1) / BN;
+        count = hi <= 0 ? 0 : sink_tiles + (hi - lo + BN - 1) / BN;
+    }
+    __device__ __forceinline__ int first(int it) const {
+        return it < sink_tiles ? it * BN : lo + (it - sink_tiles) * BN;
+    }
+    __device__ __forceinline__ int end(int it) const { return it < sink_tiles ? sink : hi; }
+};
+
+// Rows of a wave against BN keys from j0 on: whether all see all of them, or none any.
+template <int BN>
+struct Sight {
+    bool all, none;
+    int limit;  // keys from here on are another tile's
+    __device__ __forceinline__ Sight(const AttnArgs& a, const Span<BN>& s, int it, int j0, int pmin, int pmax) {
+        if (it < s.sink_tiles) {
+            all = j0 + BN <= s.sink;
+            none = false;
+            limit = s.sink;
+        } else {
+            all = j0 + BN - 1 <= pmin && (j0 > pmax - a.window || j0 + BN <= a.sinks);
+            none = j0 > pmax || (j0 + BN - 1 <= pmin - a.window && j0 >= a.sinks);
+            limit = INT_MAX;
+        }
+    }
+};
+
+// A row of a block: its query's place in the sequence and its pointers' offsets.
+struct RowAt {
+    int query, head;
+    __device__ __forceinline__ RowAt(const AttnArgs& a, int row, int kv_head)
+        : query(row / a.group), head(kv_head * a.group + row % a.group) {}
+    __device__ __forceinline__ int64_t in(const int64_t (&s)[3], int b) const {
+        return b * s[0] + query * s[1] + head * s[2];
+    }
+    __device__ __forceinline__ int64_t stat(const AttnArgs& a, int b) const {
+        return (static_cast<int64_t>(b) * a.heads + head) * a.queries + query;
+    }
+    __device__ __forceinline__ int64_t packed(const AttnArgs& a, int b) const {
+        return ((static_cast<int64_t>(b) * a.queries + query) * a.heads + head) * a.dim;
+    }
+};
+
+// A row's elements as the fragments of a product over them, or zeros.
+template <typename T, int D>
+struct RowFrags {
+    using V = typename Frag<T>::V;
+    V v[Tile<T, D>::kSteps];
+    __device__ __forceinline__ const V& operator[](int t) const { return v[t]; }
+    __device__ __forceinline__ void load(const T* row, int dim, int lane) {
+#pragma unroll
+        for (int t = 0; t < Tile<T, D>::kSteps; ++t) {
+            const int at = (2 * t + lane / 32) * Frag<T>::N;
+            v[t] = V{};
+            if (row && at < dim) v[t] = *reinterpret_cast<const V*>(row + at);
+        }
+    }
+};
+
+// A row of a transposed product (lane: a row, registers: its dims) times `factor`; what its
+// rounding leaves goes to `rest` if that is set.
+template <typename T, int DB>
+__device__ __forceinline__ void store_row(T* row, const acc16 (&x)[DB], float factor, int dim, int lane,
+                                          T* rest = nullptr) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int at = 32 * db + product_row(i, lane / 32);
+            Pack<T, 4> p;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p.v[e] = static_cast<T>(x[db][i + e] * factor);
+            if (at < dim) *reinterpret_cast<Pack<T, 4>*>(row + at) = p;
+            if (!rest) continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p.v[e] = static_cast<T>(x[db][i + e] * factor - static_cast<float>(p.v[e]));
+            if (at < dim) *reinterpret_cast<Pack<T, 4>*>(rest + at) = p;
+        }
+}
+
+template <typename T>
+constexpr int kKeyTile = sizeof(T) == 4 ? 32 : 64;
+
+int check_attention(const isa_block_attention* t);
+AttnArgs attention_args(const isa_block_attention* t);
+bool strided(const void* p, const int64_t (&s)[3], int64_t tokens, int64_t dim, size_t bytes);
+
+// f(type, D) for the element type and the dims of a tile.
+template <typename F>
+void for_type(int type, int dim, F f) {
+    auto dims = [&](auto t) {
+        using T = decltype(t);
+        if (dim <= 32) return f(T{}, std::integral_constant<int, 32>{});
+        if (dim <= 64) return f(T{}, std::integral_constant<int, 64>{});
+        if (dim <= 96) return f(T{}, std::integral_constant<int, 96>{});
+        return f(T{}, std::integral_constant<int, 128>{});
+    };
+    if (type == ISA_BLOCK_F32) return dims(float{});
+    if (type == ISA_BLOCK_BF16) return dims(bf16{});
+    return dims(f16{});
+}
+
+}  // namespace isa_block

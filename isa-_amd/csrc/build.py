@@ -21,7 +21,10 @@ REPO = PKG_ROOT.parent
 SOURCES = [CSRC / "ekv_lut.hip"]
 INCLUDE = REPO / "include"
 OUT = PKG_ROOT / "isa" / "kernels" / "transformer_ffn" / "libisa_ekv_hip.so"
-BLOCK_SOURCES = [CSRC / f"block_{name}.hip" for name in ("api", "norm", "attention", "loss")]
+BLOCK_SOURCES = [CSRC / f"block_{name}.hip" for name in ("api", "norm", "attention", "attention_backward", "loss")]
+# products keep their sums in ordinary registers, which the softmax between two products works on: with
+# accumulation registers every one of them is moved there and back
+BLOCK_FLAGS = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 BLOCK_OUT = PKG_ROOT / "isa" / "kernels" / "transformer_block" / "libisa_block_hip.so"
 ARCH = os.environ.get("ISA_EKV_OFFLOAD_ARCH", "gfx950")
 
@@ -63,7 +66,7 @@ def _block(verbose: bool, pool: ThreadPoolExecutor) -> None:
     tmp = BLOCK_OUT.with_suffix(".so.tmp")
     with tempfile.TemporaryDirectory() as work:
         objects = [str(Path(work) / f"{src.stem}.o") for src in BLOCK_SOURCES]
-        jobs = [pool.submit(_run, [hipcc(), *compile_flags, f"-I{INCLUDE}", "-c", "-o", obj, str(src)], verbose)
+        jobs = [pool.submit(_run, [hipcc(), *compile_flags, *BLOCK_FLAGS, f"-I{INCLUDE}", "-c", "-o", obj, str(src)], verbose)
                 for src, obj in zip(BLOCK_SOURCES, objects)]
         for job in jobs:
             job.result()

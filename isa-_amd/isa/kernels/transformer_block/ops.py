@@ -132,10 +132,13 @@ def _strides(t: torch.Tensor):
 
 
 def attention_operand(t: torch.Tensor) -> torch.Tensor:
-    """t, or a copy where its heads' elements are apart or 16-byte loads would not be aligned."""
+    """t, or a copy where its heads' elements are apart, 16-byte loads would not be aligned or tokens
+    overlap (as broadcast ones do) or lie too far apart."""
     if t.numel() == 0:
         return t
-    if t.stride(3) == 1 and not t.data_ptr() & 15 and not any(s & 7 for s in _strides(t)):
+    s = _strides(t)
+    if t.stride(3) == 1 and not t.data_ptr() & 15 and not any(x & 7 for x in s) and (
+            t.shape[1] < 2 or t.shape[3] <= s[1] < _FAR // t.element_size()):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -185,6 +188,7 @@ def _attention(q, k, v, window, sinks, scale, key_lengths) -> "_hip.Attention":
 
 
 _LONGEST = 1 << 30
+_FAR = 1 << 24  # bytes between tokens
 
 
 def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: Optional[int], sinks: int,
@@ -194,7 +198,7 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window:
     lib, dev = _hip.load(), q.device
     a = _attention(q, k, v, window, sinks, scale, key_lengths)
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=dev) if for_backward else None
+    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1], 2), dtype=torch.float32, device=dev) if for_backward else None
     rest = torch.empty_like(out) if for_backward and q.dtype != torch.float32 else None
     ws = _workspace(lib.isa_block_attention_forward_workspace(ctypes.byref(a)), dev)
     with _hip.on_device(dev):
