@@ -2,7 +2,8 @@
 
 Usage: ``python isa-_amd/csrc/build.py`` (also called by ``__graft_entry__.build()``).
 Each library lands next to its ctypes loader: ``libisa_ekv_hip.so`` in
-``isa/kernels/transformer_ffn/``, ``libisa_block_hip.so`` in ``isa/kernels/transformer_block/``.
+``isa/kernels/transformer_ffn/``, ``libisa_block_hip.so`` in ``isa/kernels/transformer_block/``
+with ``_binding.so``, torch's binding to it.
 """
 
 from __future__ import annotations
@@ -11,6 +12,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
@@ -26,6 +28,8 @@ BLOCK_SOURCES = [CSRC / f"block_{name}.hip" for name in ("api", "norm", "attenti
 # accumulation registers every one of them is moved there and back
 BLOCK_FLAGS = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 BLOCK_OUT = PKG_ROOT / "isa" / "kernels" / "transformer_block" / "libisa_block_hip.so"
+BINDING_SOURCE = CSRC / "block_torch.cpp"
+BINDING_OUT = BLOCK_OUT.with_name("_binding.so")
 ARCH = os.environ.get("ISA_EKV_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [
@@ -52,7 +56,7 @@ def _run(cmd: list, verbose: bool) -> None:
         print(" ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
+        raise RuntimeError(f"{Path(cmd[0]).name} failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
 
 
 def _ekv(verbose: bool) -> None:
@@ -74,16 +78,41 @@ def _block(verbose: bool, pool: ThreadPoolExecutor) -> None:
     os.replace(tmp, BLOCK_OUT)
 
 
+def _binding_object(obj: Path, verbose: bool) -> None:
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    # the HIP headers' own switch, and torch's: which GPU runtime its headers stand for
+    flags = ["-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1"]
+    rocm = Path(hipcc()).resolve().parents[1] / "include"
+    includes = [f"-I{INCLUDE}", *(f"-isystem{p}" for p in (*include_paths(), sysconfig.get_paths()["include"], rocm))]
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          *flags, *includes, "-c", "-o", str(obj), str(BINDING_SOURCE)], verbose)
+
+
+def _link_binding(obj: Path, verbose: bool) -> None:
+    import torch
+
+    lib = Path(torch.__file__).resolve().parent / "lib"
+    tmp = BINDING_OUT.with_suffix(".so.tmp")
+    _run(["g++", "-shared", "-o", str(tmp), str(obj), f"-L{BLOCK_OUT.parent}", "-lisa_block_hip", f"-L{lib}", "-lc10",
+          "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"], verbose)
+    os.replace(tmp, BINDING_OUT)
+
+
 def build(verbose: bool = False) -> Path:
-    """Compile both libraries, the block's sources and the projection's side by side; returns the latter's path."""
-    with ThreadPoolExecutor(max_workers=1 + len(BLOCK_SOURCES)) as pool:
-        ekv = pool.submit(_ekv, verbose)
+    """Compile the libraries and the binding, side by side; returns the projection's library."""
+    with tempfile.TemporaryDirectory() as work, ThreadPoolExecutor(max_workers=2 + len(BLOCK_SOURCES)) as pool:
+        obj = Path(work) / "binding.o"
+        others = [pool.submit(_ekv, verbose), pool.submit(_binding_object, obj, verbose)]
         _block(verbose, pool)
-        ekv.result()
+        for job in others:
+            job.result()
+        _link_binding(obj, verbose)
     return OUT
 
 
 if __name__ == "__main__":
     path = build(verbose=True)
-    print(f"built {path}\nbuilt {BLOCK_OUT}")
+    print(f"built {path}\nbuilt {BLOCK_OUT}\nbuilt {BINDING_OUT}")
     sys.exit(0)
