@@ -128,8 +128,8 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(AttnArgs a)
                                            threadIdx.x);
     auto fetch = [&](int it, T* kt, T* vt) {
         const int j0 = span.first(it), je = span.end(it);
-        kload.load(kt, j0, je, wave);
-        vload.load(vt, j0, je, wave);
+        kload.load(kt, 0, j0, je, wave);
+        vload.load(vt, 0, j0, je, wave);
     };
     auto compute = [&](int it, const T* kt, const T* vt) {
         const int j0 = span.first(it);
@@ -168,7 +168,126 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(AttnArgs a)
     if (row <= last) finish<T, D>(r, a, at, b, split, lane);
 }
 
-// Rows from the partial sums of `splits` blocks: a wave each.
+// ---- few rows: tokens over a cache ---------------------------------------------------------------
+// One tile holds all rows of a key head, so the work is the keys': each wave walks its own part of
+// them through tiles of its own in LDS, without barriers, the next tile's copy in flight; the waves'
+// sums are joined at the end, and those of several blocks by the kernel below. Bound by HBM: with
+// 32 keys of 16-bit 128-wide heads a wave computes 512 cycles for 16 KB.
+
+template <typename T, int D>
+struct TokenShape {
+    static constexpr int kTileBytes = kTile * Tile<T, D>::kPitch * static_cast<int>(sizeof(T));
+    // two tiles each of K and V a wave, in 128 KB
+    static constexpr int kWaveCount = std::min(8, (128 << 10) / (4 * kTileBytes));
+    static constexpr int kThreadCount = kWaveCount * kWave;
+};
+
+template <int DB>
+__device__ __forceinline__ void put(float* to, const Running<DB>& r, int lane) {
+    using F = vec<float, 4>;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+            reinterpret_cast<F*>(to)[(db * 4 + i / 4) * kWave + lane] =
+                F{r.o[db][i], r.o[db][i + 1], r.o[db][i + 2], r.o[db][i + 3]};
+    to[DB * 16 * kWave + lane] = r.bound == -INFINITY ? -INFINITY : r.base;
+    to[DB * 16 * kWave + kWave + lane] = r.sum;
+}
+
+// Joins the sums that another wave put.
+template <int DB>
+__device__ __forceinline__ void join(Running<DB>& r, const float* from, int lane) {
+    using F = vec<float, 4>;
+    const float other = from[DB * 16 * kWave + lane], mine = r.bound == -INFINITY ? -INFINITY : r.base;
+    const float top = fmaxf(mine, other);
+    const float keep = mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - top);
+    const float take = other == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(other - top);
+    if (top == -INFINITY) return;
+    r.base = r.bound = top;
+    r.sum = r.sum * keep + from[DB * 16 * kWave + kWave + lane] * take;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const F x = reinterpret_cast<const F*>(from)[(db * 4 + i / 4) * kWave + lane];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r.o[db][i + e] = r.o[db][i + e] * keep + x[e] * take;
+        }
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__((TokenShape<T, D>::kThreadCount)) void attention_token_kernel(AttnArgs a) {
+    using L = Tile<T, D>;
+    using S = TokenShape<T, D>;
+    constexpr int DB = D / 32, kElements = kTile * L::kPitch, W = S::kWaveCount;
+    __shared__ __attribute__((aligned(1024))) T k0[W * kElements], v0[W * kElements], k1[W * kElements], v1[W * kElements];
+    const int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), half = lane / 32;
+    const int task = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+    const int kv_head = task % a.kv_heads, b = task / a.kv_heads;
+    const int shift = length_of(a, b) - a.queries, last = a.queries * a.group - 1;
+    const int pmin = shift, pmax = shift + a.queries - 1;
+    const Span<kTile> span(a, pmin, pmax);
+    const int part = split * W + wave, parts = a.splits * W;
+    const int begin = static_cast<int>(static_cast<int64_t>(span.count) * part / parts);
+    const int end = static_cast<int>(static_cast<int64_t>(span.count) * (part + 1) / parts);
+
+    const int row = lane % 32;
+    const RowAt at(a, min(row, last), kv_head);
+    const int p = shift + at.query;
+    RowFrags<T, D> q;
+    q.load(row <= last ? static_cast<const T*>(a.q) + at.in(a.qs, b) : nullptr, a.dim, lane);
+
+    Running<DB> r;
+    const Loader<T, D, kTile, kWave> kload(static_cast<const T*>(a.k) + b * a.ks[0] + kv_head * a.ks[2], a.ks[1], a.dim,
+                                           lane);
+    const Loader<T, D, kTile, kWave> vload(static_cast<const T*>(a.v) + b * a.vs[0] + kv_head * a.vs[2], a.vs[1], a.dim,
+                                           lane);
+    auto fetch = [&](int it, T* kt, T* vt) {
+        const int j0 = span.first(it), je = span.end(it);
+        kload.load(kt, wave * S::kTileBytes, j0, je, 0);
+        vload.load(vt, wave * S::kTileBytes, j0, je, 0);
+    };
+    auto compute = [&](int it, const T* kt, const T* vt) {
+        const int j0 = span.first(it);
+        const Sight<kTile> sight(a, span, it, j0, pmin, pmax);
+        acc16 s[1] = {};
+#pragma unroll
+        for (int t = 0; t < L::kSteps; ++t) mma(s[0], L::row(kt + wave * kElements, 0, t, lane), q[t]);
+        if (!sight.all) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int j = j0 + product_row(i, half);
+                s[0][i] = ((j < sight.limit) & sees(a, p, j)) ? s[0][i] : -INFINITY;
+            }
+        }
+        attend<T, D, 1>(r, s, vt + wave * kElements, a, lane);
+    };
+    if (begin < end) fetch(begin, k0, v0);
+    for (int it = begin; it < end; it += 2) {
+        loads_arrived();
+        if (it + 1 < end) fetch(it + 1, k1, v1);
+        compute(it, k0, v0);
+        if (it + 1 >= end) break;
+        loads_arrived();
+        if (it + 2 < end) fetch(it + 2, k0, v0);
+        compute(it + 1, k1, v1);
+    }
+    // joined by halves through the tiles' memory, a wave's sums in each of the four
+    static_assert((DB * 16 + 2) * kWave * sizeof(float) <= sizeof(k0) && W <= 8);
+    auto place = [&](int n) { return reinterpret_cast<float*>(n == 0 ? k0 : n == 1 ? v0 : n == 2 ? k1 : v1); };
+    __syncthreads();
+#pragma unroll
+    for (int n = W / 2; n >= 1; n /= 2) {
+        if (wave >= n && wave < 2 * n) put<DB>(place(wave - n), r, lane);
+        __syncthreads();
+        if (wave < n) join<DB>(r, place(wave), lane);
+        __syncthreads();
+    }
+    if (wave == 0 && row <= last) finish<T, D>(r, a, at, b, split, lane);
+}
+
+// Rows from the partial sums of `splits` blocks (at most 64): a wave each, a lane for a block's sum.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void attention_combine_kernel(AttnArgs a) {
     const int lane = threadIdx.x % kWave;
@@ -177,19 +296,20 @@ __global__ __launch_bounds__(kThreads) void attention_combine_kernel(AttnArgs a)
     if (row >= rows) return;
     const float* p = a.partial + row * (D + 4);
     const int64_t step = rows * (D + 4);
-    float top = -INFINITY, sum = 0.0f;
+    const bool have = lane < a.splits;
+    const float base = have ? p[lane * step + D] : -INFINITY, part = have ? p[lane * step + D + 1] : 0.0f;
+    const float top = wave_max(base);
+    const float mine = base == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(base - top);
+    const float sum = wave_sum(part * mine);
     constexpr int E = (D + 63) / 64;
     float o[E] = {};
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, p[s * step + D]);
-    if (top > -INFINITY)
-        for (int s = 0; s < a.splits; ++s) {
-            const float* x = p + s * step;
-            const float f = __builtin_amdgcn_exp2f(x[D] - top);
-            sum = fmaf(x[D + 1], f, sum);
+#pragma unroll 8
+    for (int s = 0; s < a.splits; ++s) {
+        const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine), s));
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (e * 64 + lane < a.dim) o[e] = fmaf(x[e * 64 + lane], f, o[e]);
-        }
+        for (int e = 0; e < E; ++e)
+            if (e * 64 + lane < a.dim) o[e] = fmaf(p[s * step + e * 64 + lane], f, o[e]);
+    }
     const float factor = sum > 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e)
@@ -211,16 +331,28 @@ __global__ __launch_bounds__(kThreads) void attention_combine_kernel(AttnArgs a)
 
 constexpr int kComputeUnits = 256;
 
+// One tile holds all rows of a key head.
+bool few_rows(const isa_block_attention* t) { return t->queries * (t->heads / t->kv_heads) <= kTile; }
+
 // Blocks that share a tile of rows: where the tiles alone leave compute units idle, as many as fill
-// them twice, each with two tiles of keys or more.
+// them (twice, of the kernel of which two share a unit), each wave or block with a tile of keys or two.
 int splits_of(const isa_block_attention* t) {
-    const int64_t group = t->heads / t->kv_heads;
-    const int64_t tasks = ceil_div(t->queries * group, kWaves * kTile) * t->batch * t->kv_heads;
+    const bool few = few_rows(t);
+    const int64_t group = t->heads / t->kv_heads, tile_rows = few ? kTile : kWaves * kTile;
+    const int64_t tasks = ceil_div(t->queries * group, tile_rows) * t->batch * t->kv_heads;
     if (tasks == 0 || tasks >= kComputeUnits) return 1;
-    const int64_t rows = std::min<int64_t>(t->queries, ceil_div(kWaves * kTile, group) + 1);
+    const int64_t rows = std::min<int64_t>(t->queries, ceil_div(tile_rows, group) + 1);
     const int64_t seen = t->window ? std::min(t->keys, t->window + rows + t->sinks) : t->keys;
-    const int64_t key_tiles = ceil_div(seen, t->type == ISA_BLOCK_F32 ? 32 : 64);
-    return static_cast<int>(std::max<int64_t>(1, std::min(2 * kComputeUnits / tasks, key_tiles / 2)));
+    int64_t least = 2 * (t->type == ISA_BLOCK_F32 ? 32 : 64), want = 2 * kComputeUnits / tasks;
+    if (few) {
+        int waves = 0;
+        for_type(t->type, static_cast<int>(t->head_dim), [&](auto type, auto dim) {
+            waves = TokenShape<decltype(type), decltype(dim)::value>::kWaveCount;
+        });
+        least = kTile * waves;
+        want = ceil_div(kComputeUnits, tasks);
+    }
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, seen / least, 64})));
 }
 
 int padded_dim(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }
@@ -321,9 +453,12 @@ extern "C" int isa_block_attention_forward(const isa_block_attention* t, void* o
     for_type(t->type, a.dim, [&](auto type, auto dim) {
         using T = decltype(type);
         constexpr int D = decltype(dim)::value;
-        const int64_t tiles = ceil_div(static_cast<int64_t>(a.queries) * a.group, kWaves * kTile);
-        const int64_t blocks = tiles * a.batch * a.kv_heads * a.splits;
-        attention_forward_kernel<T, D><<<dim3(static_cast<unsigned>(blocks)), kThreads, 0, s>>>(a);
+        const int64_t tiles = few_rows(t) ? 1 : ceil_div(static_cast<int64_t>(a.queries) * a.group, kWaves * kTile);
+        const dim3 blocks(static_cast<unsigned>(tiles * a.batch * a.kv_heads * a.splits));
+        if (few_rows(t))
+            attention_token_kernel<T, D><<<blocks, TokenShape<T, D>::kThreadCount, 0, s>>>(a);
+        else
+            attention_forward_kernel<T, D><<<blocks, kThreads, 0, s>>>(a);
         if (a.splits > 1) {
             const int64_t rows = static_cast<int64_t>(a.batch) * a.queries * a.heads;
             attention_combine_kernel<T, D><<<dim3(static_cast<unsigned>(ceil_div(rows, kWaves))), kThreads, 0, s>>>(a);

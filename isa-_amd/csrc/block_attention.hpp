@@ -149,20 +149,30 @@ struct Tile {
     }
 };
 
+// x, of which the compiler knows nothing: what follows from it is computed again in each turn of a loop
+// instead of being held in registers.
+__device__ __forceinline__ int opaque(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 using LdsPtr = __attribute__((address_space(3))) void*;
+using LdsBytes = __attribute__((address_space(3))) char*;
 constexpr int kBufferFlags = 0x00027000;  // raw buffer of 32-bit data
 constexpr unsigned kOutside = 0x7fffffffu;
 
-// COUNT times BYTES a lane, `step` bytes of LDS apart, from the buffer of `size` bytes at `base` (uniform); what lies outside is zeros.
+// COUNT times BYTES a lane to `lds` (an array: its address is known) + first, `step` bytes apart, from the buffer of `size` bytes at `base` (uniform); what lies outside is zeros.
 // (The buffer's type exists for the device alone: the host's pass over the kernels does without.)
 template <int BYTES, int COUNT>
-__device__ __forceinline__ void load_to_lds(void* to, const void* base, int size, const unsigned (&at)[COUNT],
-                                            int step) {
+__device__ __forceinline__ void load_to_lds(void* lds, int first, int step, const void* base, int size,
+                                            const unsigned (&at)[COUNT]) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, size, kBufferFlags);
+    const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, uniform(size), kBufferFlags);
 #pragma unroll
     for (int n = 0; n < COUNT; ++n)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (LdsPtr)(static_cast<char*>(to) + n * step), BYTES, at[n], 0, 0,
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (LdsPtr)((LdsBytes)lds + first + n * step), BYTES, at[n], 0, 0,
                                                  0);
 #endif
 }
@@ -189,22 +199,23 @@ struct Loader {
     }
 
     // rows first .. first + ROWS - 1; those from `end` on become zeros
-    __device__ __forceinline__ void load(T* tile, int first, int end, int wave) const {
-        load_from(tile, base + static_cast<int64_t>(first) * stride, end - first, wave);
+    // `place`: of the tile in `lds`, in bytes
+    __device__ __forceinline__ void load(T* lds, int place, int first, int end, int wave) const {
+        load_from(lds, place, base + static_cast<int64_t>(first) * stride, end - first, wave);
     }
-    __device__ __forceinline__ void load_from(T* tile, const char* from, int left, int wave) const {
-        load_to_lds<16, kEach>(tile + wave * kWave * L::N, from, min(max(left, 0), ROWS) * stride, at, THREADS * 16);
+    __device__ __forceinline__ void load_from(T* lds, int place, const char* from, int left, int wave) const {
+        load_to_lds<16, kEach>(lds, place + wave * kWave * 16, THREADS * 16, from, min(max(left, 0), ROWS) * stride, at);
     }
 };
 
-// 64 floats to LDS by one wave; from `end` on zeros.
-__device__ __forceinline__ void load_floats(float* to, const float* base, int64_t first, int count, int lane) {
+// 64 floats to lds + place by one wave, zeros from `count` on.
+__device__ __forceinline__ void load_floats(float* lds, int place, const float* base, int64_t first, int count, int lane) {
     const unsigned at[1] = {static_cast<unsigned>(lane) * 4};
-    load_to_lds<4, 1>(to, base + first, max(count, 0) * 4, at, 0);
+    load_to_lds<4, 1>(lds, place * 4, 0, base + first, max(count, 0) * 4, at);
 }
 
 // All of this wave's loads to LDS have arrived.
-__device__ __forceinline__ void loads_arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void loads_arrived() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
 
 // Dispatch gives block i to XCD i % 8; this gives each XCD a run of adjacent work, whose keys its
 // L2 then holds once.
@@ -212,15 +223,6 @@ __device__ __forceinline__ int xcd_order(int id, int n) {
     const int per = n / 8, rest = n % 8, x = id % 8;
     return x * per + min(x, rest) + id / 8;
 }
-
-// x, of which the compiler knows nothing: what follows from it is computed again in each turn of a loop
-// instead of being held in registers.
-__device__ __forceinline__ int opaque(int x) {
-    asm volatile("" : "+v"(x));
-    return x;
-}
-
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // ---- which keys a block of rows sees --------------------------------------------------------
 

@@ -133,8 +133,8 @@ __global__ __launch_bounds__(kThreads, (kDqWaves<T, D>)) void attention_dq_kerne
                                            threadIdx.x);
     auto fetch = [&](int it, T* kt, T* vt) {
         const int j0 = span.first(it), je = span.end(it);
-        kload.load(kt, j0, je, wave);
-        vload.load(vt, j0, je, wave);
+        kload.load(kt, 0, j0, je, wave);
+        vload.load(vt, 0, j0, je, wave);
     };
     auto compute = [&](int it, const T* kt, const T* vt) {
         const int j0 = span.first(it);
@@ -231,7 +231,7 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
     if constexpr (!S::kHoldV) {
         const Loader<T, D, S::kKeys, S::kThreadCount> vload(
             static_cast<const T*>(a.v) + b * a.vs[0] + kv_head * a.vs[2], a.vs[1], a.dim, threadIdx.x);
-        vload.load(held, j0, length, wave);
+        vload.load(held, 0, j0, length, wave);
     }
     RowFrags<T, D> k[KB], v[KB];
 #pragma unroll
@@ -261,10 +261,10 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
         const int head = it / turns, i0 = seen.first + (it - head * turns) * BR;
         const int64_t qat = (head * a.qs[2] + i0 * a.qs[1]) * static_cast<int64_t>(sizeof(T));
         const int64_t gat = (head * a.gs[2] + i0 * a.gs[1]) * static_cast<int64_t>(sizeof(T));
-        qload.load_from(qt, qload.base + qat, seen.end - i0, wave);
-        gload.load_from(gt, gload.base + gat, seen.end - i0, wave);
+        qload.load_from(qt, 0, qload.base + qat, seen.end - i0, wave);
+        gload.load_from(gt, 0, gload.base + gat, seen.end - i0, wave);
         const int64_t at = static_cast<int64_t>(head) * a.queries + i0;
-        if (wave < (sizeof(T) == 4 ? 3 : 2)) load_floats(stat + 64 * wave, stats + wave * plane, at, seen.end - i0, lane);
+        if (wave < (sizeof(T) == 4 ? 3 : 2)) load_floats(stat, 64 * wave, stats + wave * plane, at, seen.end - i0, lane);
     };
     auto compute = [&](int it, const T* qt, const T* gt, const float* stat) {
         const int lane = opaque(outer), half = lane / 32;
