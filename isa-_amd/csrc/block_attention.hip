@@ -22,8 +22,7 @@
 namespace isa_block {
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * kWave;
+constexpr int kCombineWaves = 4;
 
 // A row's running softmax: base = c times a maximum, the weights' sum, and the product.
 template <int DB>
@@ -100,9 +99,9 @@ __device__ __forceinline__ void finish(Running<D / 32>& r, const AttnArgs& a, co
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void attention_forward_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kThreads<T>) void attention_forward_kernel(AttnArgs a) {
     using L = Tile<T, D>;
-    constexpr int BN = kKeyTile<T>, NK = BN / 32, kRows = kWaves * kTile;
+    constexpr int BN = kKeyTile<T>, NK = BN / 32, kRows = isa_block::kRows<T>;
     __shared__ __attribute__((aligned(1024))) T k0[BN * L::kPitch], v0[BN * L::kPitch], k1[BN * L::kPitch],
         v1[BN * L::kPitch];
     const int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), half = lane / 32;
@@ -122,9 +121,9 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(AttnArgs a)
     q.load(row <= last ? static_cast<const T*>(a.q) + at.in(a.qs, b) : nullptr, a.dim, lane);
 
     Running<D / 32> r;
-    const Loader<T, D, BN, kThreads> kload(static_cast<const T*>(a.k) + b * a.ks[0] + kv_head * a.ks[2], a.ks[1], a.dim,
+    const Loader<T, D, BN, kThreads<T>> kload(static_cast<const T*>(a.k) + b * a.ks[0] + kv_head * a.ks[2], a.ks[1], a.dim,
                                            threadIdx.x);
-    const Loader<T, D, BN, kThreads> vload(static_cast<const T*>(a.v) + b * a.vs[0] + kv_head * a.vs[2], a.vs[1], a.dim,
+    const Loader<T, D, BN, kThreads<T>> vload(static_cast<const T*>(a.v) + b * a.vs[0] + kv_head * a.vs[2], a.vs[1], a.dim,
                                            threadIdx.x);
     auto fetch = [&](int it, T* kt, T* vt) {
         const int j0 = span.first(it), je = span.end(it);
@@ -143,13 +142,12 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(AttnArgs a)
             for (int t = 0; t < L::kSteps; ++t) mma(s[n], L::row(kt, 32 * n, t, lane), q[t]);
         }
         if (!sight.all) {
+            const Range seen(a, span.of_sinks(it), span.sink, p, j0, half);
 #pragma unroll
             for (int n = 0; n < NK; ++n)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int j = j0 + 32 * n + product_row(i, half);
-                    s[n][i] = ((j < sight.limit) & sees(a, p, j)) ? s[n][i] : -INFINITY;
-                }
+                for (int i = 0; i < 16; ++i)
+                    s[n][i] = seen.has(32 * n + product_row(i, 0)) ? s[n][i] : -INFINITY;
         }
         attend<T, D, NK>(r, s, vt, a, lane);
     };
@@ -255,11 +253,9 @@ __global__ __launch_bounds__((TokenShape<T, D>::kThreadCount)) void attention_to
 #pragma unroll
         for (int t = 0; t < L::kSteps; ++t) mma(s[0], L::row(kt + wave * kElements, 0, t, lane), q[t]);
         if (!sight.all) {
+            const Range seen(a, span.of_sinks(it), span.sink, p, j0, half);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int j = j0 + product_row(i, half);
-                s[0][i] = ((j < sight.limit) & sees(a, p, j)) ? s[0][i] : -INFINITY;
-            }
+            for (int i = 0; i < 16; ++i) s[0][i] = seen.has(product_row(i, 0)) ? s[0][i] : -INFINITY;
         }
         attend<T, D, 1>(r, s, vt + wave * kElements, a, lane);
     };
@@ -289,10 +285,10 @@ __global__ __launch_bounds__((TokenShape<T, D>::kThreadCount)) void attention_to
 
 // Rows from the partial sums of `splits` blocks (at most 64): a wave each, a lane for a block's sum.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void attention_combine_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kCombineWaves * kWave) void attention_combine_kernel(AttnArgs a) {
     const int lane = threadIdx.x % kWave;
     const int64_t rows = static_cast<int64_t>(a.batch) * a.queries * a.heads;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / kWave;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kCombineWaves + threadIdx.x / kWave;
     if (row >= rows) return;
     const float* p = a.partial + row * (D + 4);
     const int64_t step = rows * (D + 4);
@@ -338,7 +334,7 @@ bool few_rows(const isa_block_attention* t) { return t->queries * (t->heads / t-
 // them (twice, of the kernel of which two share a unit), each wave or block with a tile of keys or two.
 int splits_of(const isa_block_attention* t) {
     const bool few = few_rows(t);
-    const int64_t group = t->heads / t->kv_heads, tile_rows = few ? kTile : kWaves * kTile;
+    const int64_t group = t->heads / t->kv_heads, tile_rows = few ? kTile : t->type == ISA_BLOCK_F32 ? kRows<float> : kRows<bf16>;
     const int64_t tasks = ceil_div(t->queries * group, tile_rows) * t->batch * t->kv_heads;
     if (tasks == 0 || tasks >= kComputeUnits) return 1;
     const int64_t rows = std::min<int64_t>(t->queries, ceil_div(tile_rows, group) + 1);
@@ -411,7 +407,7 @@ AttnArgs attention_args(const isa_block_attention* t) {
     a.group = a.heads / a.kv_heads;
     a.dim = static_cast<int>(t->head_dim);
     a.window = t->window ? static_cast<int>(t->window) : kMaxLength;
-    a.sinks = static_cast<int>(t->sinks);
+    a.sinks = t->window ? static_cast<int>(t->sinks) : 0;  // all keys are in the window
     a.scale = t->scale;
     const double c = static_cast<double>(t->scale) * 1.44269504088896340736;
     a.c = static_cast<float>(c);
@@ -453,15 +449,16 @@ extern "C" int isa_block_attention_forward(const isa_block_attention* t, void* o
     for_type(t->type, a.dim, [&](auto type, auto dim) {
         using T = decltype(type);
         constexpr int D = decltype(dim)::value;
-        const int64_t tiles = few_rows(t) ? 1 : ceil_div(static_cast<int64_t>(a.queries) * a.group, kWaves * kTile);
+        const int64_t tiles = few_rows(t) ? 1 : ceil_div(static_cast<int64_t>(a.queries) * a.group, kRows<T>);
         const dim3 blocks(static_cast<unsigned>(tiles * a.batch * a.kv_heads * a.splits));
         if (few_rows(t))
             attention_token_kernel<T, D><<<blocks, TokenShape<T, D>::kThreadCount, 0, s>>>(a);
         else
-            attention_forward_kernel<T, D><<<blocks, kThreads, 0, s>>>(a);
+            attention_forward_kernel<T, D><<<blocks, kThreads<T>, 0, s>>>(a);
         if (a.splits > 1) {
             const int64_t rows = static_cast<int64_t>(a.batch) * a.queries * a.heads;
-            attention_combine_kernel<T, D><<<dim3(static_cast<unsigned>(ceil_div(rows, kWaves))), kThreads, 0, s>>>(a);
+            attention_combine_kernel<T, D>
+                <<<dim3(static_cast<unsigned>(ceil_div(rows, kCombineWaves))), kCombineWaves * kWave, 0, s>>>(a);
         }
     });
     return launched("the attention's forward");

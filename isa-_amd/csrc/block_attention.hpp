@@ -230,46 +230,49 @@ __device__ __forceinline__ int length_of(const AttnArgs& a, int b) {
     return a.lengths ? min(max(a.lengths[b], 0), a.keys) : a.keys;
 }
 
-__device__ __forceinline__ bool sees(const AttnArgs& a, int p, int j) {
-    return (j <= p) & ((j < a.sinks) | (j > p - a.window));  // without branches
-}
 
-// The tiles of BN keys that some query at pmin .. pmax sees: those of the sinks 0 .. sink - 1 that
-// lie before the window's, then those of lo .. hi - 1, starting at lo.
+// The tiles of BN keys that some query at pmin .. pmax sees: those of the sinks 0 .. sink - 1, then
+// those of the window lo .. hi - 1 behind them.
 template <int BN>
 struct Span {
     int lo, hi, sink, sink_tiles, count;
 
     __device__ __forceinline__ Span(const AttnArgs& a, int pmin, int pmax) {
-        hi = pmax + 1;
-        lo = max(0, pmin - a.window + 1);
-        if (a.sinks >= lo) lo = 0;
-        sink = min(a.sinks, lo);
+        hi = max(pmax + 1, 0);
+        sink = min(a.sinks, hi);
+        lo = max(sink, pmin - a.window + 1);
         sink_tiles = (sink + BN - 1) / BN;
-        count = hi <= 0 ? 0 : sink_tiles + (hi - lo + BN - 1) / BN;
+        count = sink_tiles + (max(hi - lo, 0) + BN - 1) / BN;
     }
+    __device__ __forceinline__ bool of_sinks(int it) const { return it < sink_tiles; }
     __device__ __forceinline__ int first(int it) const {
         return it < sink_tiles ? it * BN : lo + (it - sink_tiles) * BN;
     }
     __device__ __forceinline__ int end(int it) const { return it < sink_tiles ? sink : hi; }
 };
 
-// Rows of a wave against BN keys from j0 on: whether all see all of them, or none any.
+// Rows of a wave against a tile's keys j0 .. j0 + BN - 1: whether all see all of them, or none any.
 template <int BN>
 struct Sight {
     bool all, none;
-    int limit;  // keys from here on are another tile's
     __device__ __forceinline__ Sight(const AttnArgs& a, const Span<BN>& s, int it, int j0, int pmin, int pmax) {
-        if (it < s.sink_tiles) {
-            all = j0 + BN <= s.sink;
-            none = false;
-            limit = s.sink;
-        } else {
-            all = j0 + BN - 1 <= pmin && (j0 > pmax - a.window || j0 + BN <= a.sinks);
-            none = j0 > pmax || (j0 + BN - 1 <= pmin - a.window && j0 >= a.sinks);
-            limit = INT_MAX;
-        }
+        const bool sinks = s.of_sinks(it);
+        all = j0 + BN - 1 <= pmin && (sinks ? j0 + BN <= s.sink : j0 > pmax - a.window);
+        none = j0 > pmax || (!sinks && j0 + BN - 1 <= pmin - a.window);
     }
+};
+
+// What the query at p sees of a tile from j0 on, told for the registers of a product whose rows are
+// the tile's keys: one range of them, so that a subtraction and a comparison decide.
+struct Range {
+    int from;
+    unsigned count;
+    __device__ __forceinline__ Range(const AttnArgs& a, bool of_sinks, int sink, int p, int j0, int half) {
+        const int lo = of_sinks ? 0 : p - a.window + 1, hi = of_sinks ? min(p, sink - 1) : p;
+        from = lo - j0 - 4 * half;
+        count = max(hi - lo + 1, 0);
+    }
+    __device__ __forceinline__ bool has(int row) const { return static_cast<unsigned>(row - from) < count; }  // of half 0
 };
 
 // A row of a block: its query's place in the sequence and its pointers' offsets.
@@ -327,6 +330,18 @@ __device__ __forceinline__ void store_row(T* row, const acc16 (&x)[DB], float fa
 
 template <typename T>
 constexpr int kKeyTile = sizeof(T) == 4 ? 32 : 64;
+
+// Waves, of 32 rows each, that share a block's tiles. At the edges of a window they wait for each other
+// with nothing to compute; products in fp32 take 16 times as long as their operands' reads allow, so
+// there fewer share (GPT-L's step in fp32, window 256: forward and dq 114 + 164 us by fours, 107 + 148 by
+// twos, 121 + 169 alone; dk and dv 241, 205 and 188). 16-bit products need the sharing (2 x 4096 tokens of
+// 128-wide heads, window 1024: 97 + 127 + 172 us by fours, 122 + 172 + 269 by twos).
+template <typename T>
+constexpr int kWaves = sizeof(T) == 4 ? 2 : 4;
+template <typename T>
+constexpr int kThreads = kWaves<T> * kWave;
+template <typename T>
+constexpr int kRows = kWaves<T> * kTile;
 
 int check_attention(const isa_block_attention* t);
 AttnArgs attention_args(const isa_block_attention* t);

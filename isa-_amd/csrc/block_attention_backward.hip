@@ -13,8 +13,7 @@
 namespace isa_block {
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * kWave;
+constexpr int kRowThreads = 256;
 
 // What both walks read of a row beside q and do, in planes of the workspace: delta, and lse as one
 // float (16-bit types) or as two (fp32, where its rounding alone would be an error of the size of
@@ -37,8 +36,8 @@ __device__ __forceinline__ void put_planes(const AttnArgs& a, int64_t at, float 
 // Where one weight is close to 1, its key's dp is close to delta and ds is their difference: out's own
 // rounding would be most of it, so a 16-bit out comes with what that left.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttnArgs a) {
-    const int64_t r = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / 16;
+__global__ __launch_bounds__(kRowThreads) void attention_rows_kernel(AttnArgs a) {
+    const int64_t r = (static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x) / 16;
     const int64_t rows = static_cast<int64_t>(a.batch) * a.queries * a.heads;
     const int c = threadIdx.x % 16 * 8;
     float s = 0.0f;
@@ -90,9 +89,9 @@ template <typename T, int D>
 constexpr int kDkvWaves = sizeof(T) == 2 || D <= 64 ? 2 : 1;
 
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, (kDqWaves<T, D>)) void attention_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kThreads<T>, (kDqWaves<T, D>)) void attention_dq_kernel(AttnArgs a) {
     using L = Tile<T, D>;
-    constexpr int BN = kKeyTile<T>, DB = D / 32, kRows = kWaves * kTile;
+    constexpr int BN = kKeyTile<T>, DB = D / 32, kRows = isa_block::kRows<T>;
     __shared__ __attribute__((aligned(1024))) T k0[BN * L::kPitch], v0[BN * L::kPitch], k1[BN * L::kPitch],
         v1[BN * L::kPitch];
     const int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), half = lane / 32;
@@ -127,9 +126,9 @@ __global__ __launch_bounds__(kThreads, (kDqWaves<T, D>)) void attention_dq_kerne
     if (row <= last && lane < 32) put_planes<T>(a, stat, delta, base, log_sum);
 
     acc16 dq[DB] = {};
-    const Loader<T, D, BN, kThreads> kload(static_cast<const T*>(a.k) + b * a.ks[0] + kv_head * a.ks[2], a.ks[1], a.dim,
+    const Loader<T, D, BN, kThreads<T>> kload(static_cast<const T*>(a.k) + b * a.ks[0] + kv_head * a.ks[2], a.ks[1], a.dim,
                                            threadIdx.x);
-    const Loader<T, D, BN, kThreads> vload(static_cast<const T*>(a.v) + b * a.vs[0] + kv_head * a.vs[2], a.vs[1], a.dim,
+    const Loader<T, D, BN, kThreads<T>> vload(static_cast<const T*>(a.v) + b * a.vs[0] + kv_head * a.vs[2], a.vs[1], a.dim,
                                            threadIdx.x);
     auto fetch = [&](int it, T* kt, T* vt) {
         const int j0 = span.first(it), je = span.end(it);
@@ -151,11 +150,9 @@ __global__ __launch_bounds__(kThreads, (kDqWaves<T, D>)) void attention_dq_kerne
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = probability<T>(s[i], a, lse, lse_rest) * (d[i] - delta);
             if (!sight.all) {
+                const Range seen(a, span.of_sinks(it), span.sink, p, j0, half);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int j = j0 + 32 * n + product_row(i, half);
-                    s[i] = ((j < sight.limit) & sees(a, p, j)) ? s[i] : 0.0f;
-                }
+                for (int i = 0; i < 16; ++i) s[i] = seen.has(32 * n + product_row(i, 0)) ? s[i] : 0.0f;
             }
 #pragma unroll
             for (int u = 0; u < L::kUses; ++u) {
@@ -187,7 +184,7 @@ __global__ __launch_bounds__(kThreads, (kDqWaves<T, D>)) void attention_dq_kerne
 
 template <typename T, int D>
 struct DkvShape {
-    static constexpr int kWaveCount = 4, KB = 1;
+    static constexpr int kWaveCount = sizeof(T) == 4 ? 1 : 4, KB = 1;
     static constexpr int kKeys = kWaveCount * 32 * KB, kThreadCount = kWaveCount * kWave;
     // 16-bit rows of 128: V waits in LDS instead of in registers, and tiles of 32 queries leave room for
     // it, so that two blocks still share a compute unit
@@ -264,7 +261,9 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
         qload.load_from(qt, 0, qload.base + qat, seen.end - i0, wave);
         gload.load_from(gt, 0, gload.base + gat, seen.end - i0, wave);
         const int64_t at = static_cast<int64_t>(head) * a.queries + i0;
-        if (wave < (sizeof(T) == 4 ? 3 : 2)) load_floats(stat, 64 * wave, stats + wave * plane, at, seen.end - i0, lane);
+#pragma unroll
+        for (int n = 0; n < (sizeof(T) == 4 ? 3 : 2); ++n)
+            if (n % S::kWaveCount == wave) load_floats(stat, 64 * n, stats + n * plane, at, seen.end - i0, lane);
     };
     auto compute = [&](int it, const T* qt, const T* gt, const float* stat) {
         const int lane = opaque(outer), half = lane / 32;
@@ -300,9 +299,12 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
                     }
                 }
                 if (!all) {
+                    // queries at key .. key + window - 1 see it, of a sink all from it on
+                    const int from = key - pmin - 32 * r - 4 * half;
+                    const unsigned count = key < a.sinks ? INT_MAX : a.window;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const bool seen = sees(a, pmin + 32 * r + product_row(i, half), key);
+                        const bool seen = static_cast<unsigned>(product_row(i, 0) - from) < count;
                         s[i] = seen ? s[i] : 0.0f;
                         d[i] = seen ? d[i] : 0.0f;
                     }
@@ -428,11 +430,11 @@ void launch(AttnArgs a, const isa_block_attention* t, hipStream_t s) {
     using S = DkvShape<T, D>;
     const int64_t rows = static_cast<int64_t>(a.batch) * a.queries * a.heads;
     if (rows) {
-        const int64_t tiles = ceil_div(static_cast<int64_t>(a.queries) * a.group, kWaves * kTile);
+        const int64_t tiles = ceil_div(static_cast<int64_t>(a.queries) * a.group, kRows<T>);
         if (a.result)
-            attention_dq_kernel<T, D><<<dim3(static_cast<unsigned>(tiles * a.batch * a.kv_heads)), kThreads, 0, s>>>(a);
+            attention_dq_kernel<T, D><<<dim3(static_cast<unsigned>(tiles * a.batch * a.kv_heads)), kThreads<T>, 0, s>>>(a);
         else
-            attention_rows_kernel<T><<<dim3(static_cast<unsigned>(ceil_div(rows * 16, kThreads))), kThreads, 0, s>>>(a);
+            attention_rows_kernel<T><<<dim3(static_cast<unsigned>(ceil_div(rows * 16, kRowThreads))), kRowThreads, 0, s>>>(a);
     }
     if (!a.dk || !a.keys) return;
     const Cuts cuts(t, S::kKeys);
