@@ -13,8 +13,7 @@
 namespace isa_block {
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / kWave;
+constexpr int kMostThreads = 1024;
 constexpr float kLog2E = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
@@ -32,23 +31,25 @@ struct LossArgs {
     float scale;
 };
 
+template <int THREADS>
 __device__ __forceinline__ float block_max(float x, float* slots) {
     x = wave_max(x);
     if (threadIdx.x % kWave == 0) slots[threadIdx.x / kWave] = x;
     __syncthreads();
     x = slots[0];
 #pragma unroll
-    for (int k = 1; k < kWaves; ++k) x = fmaxf(x, slots[k]);
+    for (int k = 1; k < THREADS / kWave; ++k) x = fmaxf(x, slots[k]);
     return x;
 }
 
+template <int THREADS>
 __device__ __forceinline__ float block_sum(float x, float* slots) {
     x = wave_sum(x);
     if (threadIdx.x % kWave == 0) slots[threadIdx.x / kWave] = x;
     __syncthreads();
     x = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kWaves; ++k) x += slots[k];
+    for (int k = 0; k < THREADS / kWave; ++k) x += slots[k];
     return x;
 }
 
@@ -65,13 +66,17 @@ struct Row {
         skip = static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T));
     }
     __device__ int chunks() const { return (vocab + skip + N - 1) / N; }
-    __device__ Chunk load(int c, T fill) const {
+    __device__ __forceinline__ void load(Chunk& r, int c, T fill) const {
         const int at = c * N - skip;
-        Chunk r;
-        if (at >= 0 && at + N <= vocab) return *reinterpret_cast<const Chunk*>(p + at);
+        if (at >= 0 && at + N <= vocab) {
+            using V = vec<T, N>;
+            const V x = *reinterpret_cast<const V*>(p + at);
 #pragma unroll
-        for (int e = 0; e < N; ++e) r.v[e] = at + e >= 0 && at + e < vocab ? p[at + e] : fill;
-        return r;
+            for (int e = 0; e < N; ++e) r.v[e] = x[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) r.v[e] = at + e >= 0 && at + e < vocab ? p[at + e] : fill;
+        }
     }
     __device__ void store(T* out, int c, const Chunk& r) const {
         const int at = c * N - skip;
@@ -108,11 +113,11 @@ __device__ __forceinline__ float share_of(const LossArgs& a, int64_t r) {
 
 // C > 0: a thread holds C chunks of the row. C == 0: the row is read once for the statistics,
 // with a running maximum, and once more for the gradient.
-template <typename T, int C>
-__global__ __launch_bounds__(kThreads) void loss_kernel(LossArgs a) {
+template <typename T, int C, int THREADS>
+__global__ __launch_bounds__(THREADS) void loss_kernel(LossArgs a) {
     using R = Row<T>;
     constexpr int N = R::N;
-    __shared__ float slots[2][kWaves];
+    __shared__ float slots[2][THREADS / kWave];
     const int64_t r = blockIdx.x;
     const R row(static_cast<const T*>(a.logits) + r * a.stride, a.vocab);
     const int chunks = row.chunks();
@@ -124,7 +129,7 @@ __global__ __launch_bounds__(kThreads) void loss_kernel(LossArgs a) {
             if (a.stats) a.stats[2 * r] = a.stats[2 * r + 1] = 0.0f;
         }
         if (grad)
-            for (int c = threadIdx.x; c < chunks; c += kThreads) row.store(grad, c, typename R::Chunk{});
+            for (int c = threadIdx.x; c < chunks; c += THREADS) row.store(grad, c, typename R::Chunk{});
         return;
     }
     const T low = static_cast<T>(-INFINITY);
@@ -133,8 +138,8 @@ __global__ __launch_bounds__(kThreads) void loss_kernel(LossArgs a) {
     if constexpr (C > 0) {
 #pragma unroll
         for (int i = 0; i < C; ++i) {
-            const int c = threadIdx.x + i * kThreads;
-            if (c < chunks) held[i] = row.load(c, low);
+            const int c = threadIdx.x + i * THREADS;
+            if (c < chunks) row.load(held[i], c, low);
             else
 #pragma unroll
                 for (int e = 0; e < N; ++e) held[i].v[e] = low;
@@ -143,15 +148,16 @@ __global__ __launch_bounds__(kThreads) void loss_kernel(LossArgs a) {
         for (int i = 0; i < C; ++i)
 #pragma unroll
             for (int e = 0; e < N; ++e) top = fmaxf(top, static_cast<float>(held[i].v[e]));
-        top = block_max(top, slots[0]);
+        top = block_max<THREADS>(top, slots[0]);
 #pragma unroll
         for (int i = 0; i < C; ++i)
 #pragma unroll
             for (int e = 0; e < N; ++e)
                 sum += __builtin_amdgcn_exp2f((static_cast<float>(held[i].v[e]) - top) * kLog2E);
     } else {
-        for (int c = threadIdx.x; c < chunks; c += kThreads) {
-            const typename R::Chunk x = row.load(c, low);
+        for (int c = threadIdx.x; c < chunks; c += THREADS) {
+            typename R::Chunk x;
+            row.load(x, c, low);
             float t = top;
 #pragma unroll
             for (int e = 0; e < N; ++e) t = fmaxf(t, static_cast<float>(x.v[e]));
@@ -163,11 +169,11 @@ __global__ __launch_bounds__(kThreads) void loss_kernel(LossArgs a) {
             top = t;
         }
         const float mine = top;
-        top = block_max(top, slots[0]);
+        top = block_max<THREADS>(top, slots[0]);
         const float base = top == -INFINITY ? 0.0f : top;
         sum *= __builtin_amdgcn_exp2f((mine - base) * kLog2E);
     }
-    sum = block_sum(sum, slots[1]);
+    sum = block_sum<THREADS>(sum, slots[1]);
     const bool inside = target >= 0 && target < a.vocab;
     if (threadIdx.x == 0) {
         const float log_sum = logf(sum);
@@ -183,17 +189,20 @@ __global__ __launch_bounds__(kThreads) void loss_kernel(LossArgs a) {
     if constexpr (C > 0) {
 #pragma unroll
         for (int i = 0; i < C; ++i) {
-            const int c = threadIdx.x + i * kThreads;
+            const int c = threadIdx.x + i * THREADS;
             if (c < chunks) row.store(grad, c, gradient<T, N>(held[i], c * N - row.skip, hot, top, factor, share));
         }
     } else {
-        for (int c = threadIdx.x; c < chunks; c += kThreads)
-            row.store(grad, c, gradient<T, N>(row.load(c, low), c * N - row.skip, hot, top, factor, share));
+        for (int c = threadIdx.x; c < chunks; c += THREADS) {
+            typename R::Chunk x;
+            row.load(x, c, low);
+            row.store(grad, c, gradient<T, N>(x, c * N - row.skip, hot, top, factor, share));
+        }
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void loss_backward_kernel(LossArgs a) {
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void loss_backward_kernel(LossArgs a) {
     using R = Row<T>;
     constexpr int N = R::N;
     const int64_t r = blockIdx.x;
@@ -202,55 +211,76 @@ __global__ __launch_bounds__(kThreads) void loss_backward_kernel(LossArgs a) {
     const int64_t target = a.targets[r];
     T* grad = static_cast<T*>(a.grad) + r * a.grad_stride;
     if (target == a.ignore) {
-        for (int c = threadIdx.x; c < chunks; c += kThreads) row.store(grad, c, typename R::Chunk{});
+        for (int c = threadIdx.x; c < chunks; c += THREADS) row.store(grad, c, typename R::Chunk{});
         return;
     }
     const bool inside = target >= 0 && target < a.vocab;
     const float top = a.stats[2 * r], share = inside ? share_of(a, r) : NAN;
     const float factor = share * __builtin_amdgcn_exp2f(-a.stats[2 * r + 1] * kLog2E);
     const int hot = inside ? static_cast<int>(target) : -1;
-    for (int c = threadIdx.x; c < chunks; c += kThreads)
-        row.store(grad, c, gradient<T, N>(row.load(c, static_cast<T>(-INFINITY)), c * N - row.skip, hot, top, factor,
-                                          share));
+    for (int c = threadIdx.x; c < chunks; c += THREADS) {
+        typename R::Chunk x;
+        row.load(x, c, static_cast<T>(-INFINITY));
+        row.store(grad, c, gradient<T, N>(x, c * N - row.skip, hot, top, factor, share));
+    }
 }
 
 // The rows that count, as a float (exact to 2^24 rows; the rows' number is held to that).
-__global__ __launch_bounds__(kThreads) void loss_count_kernel(const int64_t* targets, int64_t rows, int64_t ignore,
+__global__ __launch_bounds__(kMostThreads) void loss_count_kernel(const int64_t* targets, int64_t rows, int64_t ignore,
                                                               float* count) {
-    __shared__ float slots[kWaves];
+    __shared__ float slots[kMostThreads / kWave];
     float n = 0.0f;
-    for (int64_t r = threadIdx.x; r < rows; r += kThreads) n += targets[r] != ignore ? 1.0f : 0.0f;
-    n = block_sum(n, slots);
+    for (int64_t r = threadIdx.x; r < rows; r += kMostThreads) n += targets[r] != ignore ? 1.0f : 0.0f;
+    n = block_sum<kMostThreads>(n, slots);
     if (threadIdx.x == 0) count[0] = n;
 }
 
-__global__ __launch_bounds__(kThreads) void loss_sum_kernel(const float* row_loss, int64_t rows, const float* count,
+__global__ __launch_bounds__(kMostThreads) void loss_sum_kernel(const float* row_loss, int64_t rows, const float* count,
                                                             float* out) {
-    __shared__ float slots[kWaves];
+    __shared__ float slots[kMostThreads / kWave];
     float s = 0.0f;
-    for (int64_t r = threadIdx.x; r < rows; r += kThreads) s += row_loss[r];
-    s = block_sum(s, slots);
+    for (int64_t r = threadIdx.x; r < rows; r += kMostThreads) s += row_loss[r];
+    s = block_sum<kMostThreads>(s, slots);
     if (threadIdx.x == 0) out[0] = count ? s / count[0] : s;
 }
 
-template <typename T, int C>
+template <typename T, int C, int THREADS>
 void launch(const LossArgs& a, hipStream_t s) {
-    loss_kernel<T, C><<<dim3(static_cast<unsigned>(a.rows)), dim3(kThreads), 0, s>>>(a);
+    loss_kernel<T, C, THREADS><<<dim3(static_cast<unsigned>(a.rows)), dim3(THREADS), 0, s>>>(a);
+}
+
+// Chunks of the longest row, one more where rows start inside a chunk.
+template <typename T>
+int64_t chunks_of(const LossArgs& a) {
+    return ceil_div(a.vocab, 16 / sizeof(T)) + 1;
+}
+
+// Blocks of 256 threads where those hold a row in four chunks each, so that several rows share a
+// compute unit (1023 rows of 5003 in bf16: SMALL us, in blocks of 1024 11.3); larger rows take 1024.
+template <typename T>
+void launch_rows(const LossArgs& a, hipStream_t s) {
+    const int64_t chunks = chunks_of<T>(a), few = ceil_div(chunks, 256), each = ceil_div(chunks, 1024);
+    if (!a.grad) return few <= 4 ? launch<T, 0, 256>(a, s) : launch<T, 0, 1024>(a, s);  // nothing is read twice
+    if (few <= 1) return launch<T, 1, 256>(a, s);
+    if (few <= 2) return launch<T, 2, 256>(a, s);
+    if (few <= 3) return launch<T, 3, 256>(a, s);
+    if (few <= 4) return launch<T, 4, 256>(a, s);
+    if (each <= 2) return launch<T, 2, 1024>(a, s);
+    if (each <= 4) return launch<T, 4, 1024>(a, s);
+    if (each <= 7) return launch<T, 7, 1024>(a, s);
+    if (each <= 10) return launch<T, 10, 1024>(a, s);
+    if (each <= 13) return launch<T, 13, 1024>(a, s);
+    if (each <= 16) return launch<T, 16, 1024>(a, s);
+    launch<T, 0, 1024>(a, s);
 }
 
 template <typename T>
-void launch_rows(const LossArgs& a, hipStream_t s) {
-    // chunks of the longest row, one more where rows start inside a chunk
-    const int64_t each = ceil_div(ceil_div(a.vocab, 16 / sizeof(T)) + 1, kThreads);
-    if (!a.grad) return launch<T, 0>(a, s);  // nothing is read twice
-    if (each <= 1) return launch<T, 1>(a, s);
-    if (each <= 2) return launch<T, 2>(a, s);
-    if (each <= 4) return launch<T, 4>(a, s);
-    if (each <= 7) return launch<T, 7>(a, s);
-    if (each <= 10) return launch<T, 10>(a, s);
-    if (each <= 13) return launch<T, 13>(a, s);
-    if (each <= 16) return launch<T, 16>(a, s);
-    launch<T, 0>(a, s);
+void launch_backward(const LossArgs& a, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>(a.rows));
+    if (chunks_of<T>(a) <= 1024)
+        loss_backward_kernel<T, 256><<<grid, 256, 0, s>>>(a);
+    else
+        loss_backward_kernel<T, 1024><<<grid, 1024, 0, s>>>(a);
 }
 
 void run_rows(int type, const LossArgs& a, hipStream_t s) {
@@ -313,7 +343,7 @@ extern "C" int isa_block_loss_forward(const isa_block_loss* l, int reduction, fl
     float* ws = static_cast<float*>(workspace);
     if (!count) count = ws;
     if (reduction == ISA_BLOCK_MEAN) {
-        loss_count_kernel<<<1, kThreads, 0, s>>>(l->targets, l->rows, l->ignore_index, count);
+        loss_count_kernel<<<1, kMostThreads, 0, s>>>(l->targets, l->rows, l->ignore_index, count);
         if (int rc = launched("loss_count_kernel")) return rc;
     }
     LossArgs a = args_of(l);
@@ -322,7 +352,7 @@ extern "C" int isa_block_loss_forward(const isa_block_loss* l, int reduction, fl
     if (l->rows) run_rows(l->type, a, s);
     if (int rc = launched("loss_kernel")) return rc;
     if (reduction == ISA_BLOCK_NONE) return 0;
-    loss_sum_kernel<<<1, kThreads, 0, s>>>(ws + 64, l->rows, reduction == ISA_BLOCK_MEAN ? count : nullptr, out);
+    loss_sum_kernel<<<1, kMostThreads, 0, s>>>(ws + 64, l->rows, reduction == ISA_BLOCK_MEAN ? count : nullptr, out);
     return launched("loss_sum_kernel");
 }
 
@@ -341,11 +371,10 @@ extern "C" int isa_block_loss_backward(const isa_block_loss* l, int reduction, c
     a.scale_step = reduction == ISA_BLOCK_NONE;
     a.grad = grad;
     a.grad_stride = grad_stride;
-    const dim3 grid(static_cast<unsigned>(l->rows));
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (l->type == ISA_BLOCK_F32) loss_backward_kernel<float><<<grid, kThreads, 0, s>>>(a);
-    else if (l->type == ISA_BLOCK_BF16) loss_backward_kernel<bf16><<<grid, kThreads, 0, s>>>(a);
-    else loss_backward_kernel<f16><<<grid, kThreads, 0, s>>>(a);
+    if (l->type == ISA_BLOCK_F32) launch_backward<float>(a, s);
+    else if (l->type == ISA_BLOCK_BF16) launch_backward<bf16>(a, s);
+    else launch_backward<f16>(a, s);
     return launched("loss_backward_kernel");
 }
 
@@ -357,7 +386,7 @@ extern "C" int isa_block_loss_with_grad(const isa_block_loss* l, float grad_scal
     if (int rc = check_workspace(l, workspace, workspace_bytes)) return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     float* ws = static_cast<float*>(workspace);
-    loss_count_kernel<<<1, kThreads, 0, s>>>(l->targets, l->rows, l->ignore_index, ws);
+    loss_count_kernel<<<1, kMostThreads, 0, s>>>(l->targets, l->rows, l->ignore_index, ws);
     if (int rc = launched("loss_count_kernel")) return rc;
     LossArgs a = args_of(l);
     a.row_loss = ws + 64;
@@ -367,6 +396,6 @@ extern "C" int isa_block_loss_with_grad(const isa_block_loss* l, float grad_scal
     a.grad_stride = grad_stride;
     if (l->rows) run_rows(l->type, a, s);
     if (int rc = launched("loss_kernel")) return rc;
-    loss_sum_kernel<<<1, kThreads, 0, s>>>(ws + 64, l->rows, ws, out);
+    loss_sum_kernel<<<1, kMostThreads, 0, s>>>(ws + 64, l->rows, ws, out);
     return launched("loss_sum_kernel");
 }
