@@ -33,11 +33,27 @@ struct Running {
 
 constexpr float kSlack = 8.0f;
 
+// Weights of 32 NK keys join the running sums of their rows.
+template <typename T, int D, int NK>
+__device__ __forceinline__ void add_weighted(Running<D / 32>& r, const acc16 (&p)[NK], const T* vtile, int lane) {
+    using L = Tile<T, D>;
+#pragma unroll
+    for (int n = 0; n < NK; ++n)
+#pragma unroll
+        for (int u = 0; u < L::kUses; ++u) {
+            const typename Frag<T>::V f = operand<T>(p[n], u);
+            r.sum = add_all(f, r.sum);
+#pragma unroll
+            for (int db = 0; db < D / 32; ++db) mma(r.o[db], L::column(vtile, 32 * n, u, db, lane), f);
+        }
+    constexpr int kProducts = NK * L::kUses * (D / 32);
+    reads_ahead<kProducts * L::kColumnReads, kProducts * L::kMmas, 4 * L::kColumnReads>();
+}
+
 // Scores of 32 NK keys (lane: a query) join the running sums of their rows.
 template <typename T, int D, int NK>
-__device__ __forceinline__ void attend(Running<D / 32>& r, acc16 (&s)[NK], const T* vtile, const AttnArgs& a,
+__device__ __forceinline__ void attend(Running<D / 32>& r, acc16 (&s)[NK], const T* vtile, const AttnArgs& a, bool sinks,
                                        int lane) {
-    using L = Tile<T, D>;
     float t = s[0][0];
 #pragma unroll
     for (int n = 0; n < NK; ++n)
@@ -59,16 +75,14 @@ __device__ __forceinline__ void attend(Running<D / 32>& r, acc16 (&s)[NK], const
             for (int i = 0; i < 16; ++i) r.o[db][i] *= decay;
     }
 #pragma unroll
-    for (int n = 0; n < NK; ++n) {
+    for (int n = 0; n < NK; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[n][i] = weight<T>(s[n][i], a.c, a.c_rest, r.base);
+    add_weighted<T, D, NK>(r, s, vtile, lane);
+    if (sizeof(T) == 2 && sinks) {
 #pragma unroll
-        for (int u = 0; u < L::kUses; ++u) {
-            const typename Frag<T>::V f = operand<T>(s[n], u);
-            r.sum = add_all(f, r.sum);
-#pragma unroll
-            for (int db = 0; db < D / 32; ++db) mma(r.o[db], L::column(vtile, 32 * n, u, db, lane), f);
-        }
+        for (int n = 0; n < NK; ++n) s[n] = remainder<T>(s[n]);
+        add_weighted<T, D, NK>(r, s, vtile, lane);
     }
 }
 
@@ -141,6 +155,7 @@ __global__ __launch_bounds__(kThreads<T>) void attention_forward_kernel(AttnArgs
 #pragma unroll
             for (int t = 0; t < L::kSteps; ++t) mma(s[n], L::row(kt, 32 * n, t, lane), q[t]);
         }
+        reads_ahead<NK * L::kSteps, NK * L::kSteps * L::kMmas, 4>();
         if (!sight.all) {
             const Range seen(a, span.of_sinks(it), span.sink, p, j0, half);
 #pragma unroll
@@ -149,7 +164,7 @@ __global__ __launch_bounds__(kThreads<T>) void attention_forward_kernel(AttnArgs
                 for (int i = 0; i < 16; ++i)
                     s[n][i] = seen.has(32 * n + product_row(i, 0)) ? s[n][i] : -INFINITY;
         }
-        attend<T, D, NK>(r, s, vt, a, lane);
+        attend<T, D, NK>(r, s, vt, a, span.of_sinks(it), lane);
     };
     if (begin < end) fetch(begin, k0, v0);
     for (int it = begin; it < end; it += 2) {
@@ -257,7 +272,7 @@ __global__ __launch_bounds__((TokenShape<T, D>::kThreadCount)) void attention_to
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[0][i] = seen.has(product_row(i, 0)) ? s[0][i] : -INFINITY;
         }
-        attend<T, D, 1>(r, s, vt + wave * kElements, a, lane);
+        attend<T, D, 1>(r, s, vt + wave * kElements, a, span.of_sinks(it), lane);
     };
     if (begin < end) fetch(begin, k0, v0);
     for (int it = begin; it < end; it += 2) {

@@ -56,6 +56,17 @@ __device__ __forceinline__ typename Frag<T>::V operand(const acc16& x, int u) {
     return f;
 }
 
+// What rounding the values of a column to T leaves. A product is taken with it too where the keys are sinks:
+// they draw most of many rows' weight, so their roundings would be most of out's and dq's error (dq of
+// bf16 rows that give sinks 0.8 of their weight: 2.8e-3 off without, 2.0e-3 with, of which the result's
+// own rounding is 1.7e-3).
+template <typename T>
+__device__ __forceinline__ acc16 remainder(acc16 x) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] -= static_cast<float>(static_cast<T>(x[i]));
+    return x;
+}
+
 // sum plus an operand's values as they were rounded: a row's weights, whose sum is what they are
 // divided by, then add up to 1 as the product sees them.
 __device__ __forceinline__ float add_all(vec<bf16, 8> x, float sum) {
@@ -103,6 +114,8 @@ struct Tile {
     static constexpr int kPitch = kSlots * N;              // elements
     static constexpr int kSteps = kChunks / 2;             // of a product over D
     static constexpr int kUses = kTile / (2 * N);          // operand()s of 32 rows
+    static constexpr int kMmas = sizeof(T) == 4 ? 4 : 1;   // matrix instructions of a mma()
+    static constexpr int kColumnReads = sizeof(T) == 4 ? 4 : 2;
     using V = typename Frag<T>::V;
 
     // 256 bytes of banks: 4, 2, 1 or half a row
@@ -307,25 +320,82 @@ struct RowFrags {
     }
 };
 
+// 8 dims k 16 + 8 half .. of a 32-dim block of a row, rounded. Each half of the wave holds 4 of every 8
+// dims of its lanes' rows; 16-bit types exchange them, so that a lane stores 16 bytes (stores of 8
+// take a fifth of the forward's time at 2 x 4096 tokens of 128-wide heads).
+template <typename T>
+__device__ __forceinline__ Pack<T, 8> eight(const float (&x)[16], int k) {
+    union {
+        Pack<T, 4> v[2];
+        unsigned u[2][2];
+    } a, b;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        a.v[0].v[e] = static_cast<T>(x[8 * k + e]);
+        a.v[1].v[e] = static_cast<T>(x[8 * k + 4 + e]);
+    }
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const auto r = __builtin_amdgcn_permlane32_swap(a.u[0][n], a.u[1][n], false, false);
+        b.u[0][n] = r[0];
+        b.u[1][n] = r[1];
+    }
+    Pack<T, 8> y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y.v[e] = b.v[e / 4].v[e % 4];
+    return y;
+}
+
 // A row of a transposed product (lane: a row, registers: its dims) times `factor`; what its
-// rounding leaves goes to `rest` if that is set.
+// rounding leaves goes to `rest` if that is set. Both lanes of a row come here.
 template <typename T, int DB>
 __device__ __forceinline__ void store_row(T* row, const acc16 (&x)[DB], float factor, int dim, int lane,
                                           T* rest = nullptr) {
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+    for (int db = 0; db < DB; ++db) {
+        float y[16];
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const int at = 32 * db + product_row(i, lane / 32);
-            Pack<T, 4> p;
+        for (int i = 0; i < 16; ++i) y[i] = x[db][i] * factor;
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) p.v[e] = static_cast<T>(x[db][i + e] * factor);
-            if (at < dim) *reinterpret_cast<Pack<T, 4>*>(row + at) = p;
+            for (int i = 0; i < 16; i += 4) {
+                const int at = 32 * db + product_row(i, lane / 32);
+                if (at < dim) *reinterpret_cast<vec<float, 4>*>(row + at) = vec<float, 4>{y[i], y[i + 1], y[i + 2], y[i + 3]};
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int at = 32 * db + 16 * k + lane / 32 * 8;
+                const Pack<T, 8> z = eight<T>(y, k);
+                if (at < dim) *reinterpret_cast<Pack<T, 8>*>(row + at) = z;
+            }
             if (!rest) continue;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) p.v[e] = static_cast<T>(x[db][i + e] * factor - static_cast<float>(p.v[e]));
-            if (at < dim) *reinterpret_cast<Pack<T, 4>*>(rest + at) = p;
+            for (int i = 0; i < 16; ++i) y[i] -= static_cast<float>(static_cast<T>(y[i]));
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int at = 32 * db + 16 * k + lane / 32 * 8;
+                const Pack<T, 8> z = eight<T>(y, k);
+                if (at < dim) *reinterpret_cast<Pack<T, 8>*>(rest + at) = z;
+            }
         }
+    }
+}
+
+// Asks the scheduler for this block of code's READS reads of LDS to run AHEAD of the MMAS products that
+// take them: left to itself it reads each operand right before its product, and the wave waits for
+// LDS once a product.
+template <int READS, int MMAS, int AHEAD>
+__device__ __forceinline__ void reads_ahead() {
+    constexpr int kFirst = AHEAD < READS ? AHEAD : READS, kEach = MMAS / READS > 0 ? MMAS / READS : 1;
+    constexpr int kReads = MMAS / READS > 0 ? 1 : READS / MMAS;
+    __builtin_amdgcn_sched_group_barrier(0x100, kFirst, 0);
+#pragma unroll
+    for (int i = kFirst; i < READS; i += kReads) {
+        __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, MMAS, 0);
 }
 
 template <typename T>

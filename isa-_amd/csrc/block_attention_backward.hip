@@ -147,6 +147,7 @@ __global__ __launch_bounds__(kThreads<T>, (kDqWaves<T, D>)) void attention_dq_ke
                 mma(s, L::row(kt, 32 * n, t, lane), q[t]);
                 mma(d, L::row(vt, 32 * n, t, lane), g[t]);
             }
+            reads_ahead<2 * L::kSteps, 2 * L::kSteps * L::kMmas, 4>();
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = probability<T>(s[i], a, lse, lse_rest) * (d[i] - delta);
             if (!sight.all) {
@@ -159,6 +160,16 @@ __global__ __launch_bounds__(kThreads<T>, (kDqWaves<T, D>)) void attention_dq_ke
                 const typename Frag<T>::V f = operand<T>(s, u);
 #pragma unroll
                 for (int db = 0; db < DB; ++db) mma(dq[db], L::column(kt, 32 * n, u, db, lane), f);
+            }
+            reads_ahead<L::kUses * DB * L::kColumnReads, L::kUses * DB * L::kMmas, 4 * L::kColumnReads>();
+            if (sizeof(T) == 2 && span.of_sinks(it)) {
+                s = remainder<T>(s);
+#pragma unroll
+                for (int u = 0; u < L::kUses; ++u) {
+                    const typename Frag<T>::V f = operand<T>(s, u);
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) mma(dq[db], L::column(kt, 32 * n, u, db, lane), f);
+                }
             }
         }
     };
@@ -281,8 +292,10 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
 #pragma unroll
                 for (int t = 0; t < L::kSteps; ++t) {
                     mma(s, L::row(qt, 32 * r, t, lane), k[n][t]);
-                    mma(d, L::row(gt, 32 * r, t, lane), S::kHoldV ? v[n][t] : L::row(held, wave * 32 * KB + 32 * n, t, lane));
+                    mma(d, L::row(gt, 32 * r, t, lane),
+                        S::kHoldV ? v[n][t] : L::row(held, wave * 32 * KB + 32 * n, t, lane));
                 }
+                reads_ahead<(S::kHoldV ? 2 : 3) * L::kSteps, 2 * L::kSteps * L::kMmas, 4>();
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
                     const int at = 32 * r + product_row(i, half);
@@ -318,6 +331,7 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
                         mma(dk[n][db], L::column(qt, 32 * r, u, db, lane), h);
                     }
                 }
+                reads_ahead<2 * L::kUses * DB * L::kColumnReads, 2 * L::kUses * DB * L::kMmas, 4 * L::kColumnReads>();
             }
     };
     if (begin < end) fetch(begin, q0, g0, stat0);
