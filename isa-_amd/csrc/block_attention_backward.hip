@@ -203,6 +203,11 @@ struct DkvShape {
     static constexpr int BR = kHoldV ? kKeyTile<T> : 32;
 };
 
+// Pieces of a key head's tiles that are cut, of which `plain` hold no sinks: those first.
+__device__ __forceinline__ int pieces_per_head(const AttnArgs& a, int plain) {
+    return (a.near > 1 ? plain * a.near : 0) + (a.far > 1 ? a.far_tiles * a.far : 0);
+}
+
 // The queries first .. end - 1 that see one of the keys j0 .. j1 - 1.
 struct Seen {
     int first, end;
@@ -346,8 +351,9 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
         if (it + 2 < end) fetch(it + 2, q0, g0, stat0);
         compute(it + 1, q1, g1, stat1);
     }
-    if (splits > 1) {  // [slot of the head][dk, dv][key block, dims' quarter][thread]
-        const int64_t mine_at = (static_cast<int64_t>(b) * a.kv_heads + kv_head) * per_head + slot;
+    if (splits > 1) {  // [piece of a cut tile][dk, dv][key block, dims' quarter][thread]
+        const int64_t mine_at = (static_cast<int64_t>(b) * a.kv_heads + kv_head) * pieces_per_head(a, plain) +
+                                (far && a.near > 1 ? plain * a.near : 0) + in;
         float* p = a.partial + mine_at * (2 * S::kKeys * D) + threadIdx.x * 4;
 #pragma unroll
         for (int n = 0; n < KB; ++n)
@@ -380,14 +386,14 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount)) void attention_dkv_
     using F = vec<float, 4>;
     constexpr int kQuads = S::KB * (D / 32) * 4;
     const int tiles = (a.keys + S::kKeys - 1) / S::kKeys, plain = tiles - a.far_tiles;
-    const int per_head = plain * a.near + a.far_tiles * a.far;
     const int quad = blockIdx.x % kQuads, which = blockIdx.x / kQuads % 2, task = blockIdx.x / kQuads / 2;
     const int summed = (a.near > 1 ? plain : 0) + (a.far > 1 ? a.far_tiles : 0);
     const int t = task % summed, head = task / summed;  // head: of all batches
     const bool far = a.near == 1 || t >= plain;
     const int in = far && a.near > 1 ? t - plain : t, splits = far ? a.far : a.near;
     const int tile = (far ? 0 : a.far_tiles) + in;
-    const int64_t slot = static_cast<int64_t>(head) * per_head + (far ? plain * a.near : 0) + in * splits;
+    const int64_t slot = static_cast<int64_t>(head) * pieces_per_head(a, plain) +
+                         (far && a.near > 1 ? plain * a.near : 0) + in * splits;
     const F* p = reinterpret_cast<const F*>(a.partial + slot * (2 * S::kKeys * D) + which * S::kKeys * D) +
                  quad * S::kThreadCount + threadIdx.x;
     F x{};
@@ -416,7 +422,7 @@ constexpr int kComputeUnits = 256;
 // range from all to nothing.
 struct Cuts {
     int tiles, far_tiles, near, far;
-    int64_t heads, slots;  // blocks of all heads
+    int64_t heads, slots, pieces;  // blocks of all heads, and those of tiles that are cut
     Cuts(const isa_block_attention* t, int keys_per_tile) {
         heads = t->batch * t->kv_heads;
         tiles = static_cast<int>(ceil_div(t->keys, keys_per_tile));
@@ -429,8 +435,12 @@ struct Cuts {
         const int64_t enough = limited ? kComputeUnits * 3 / 2 : 4 * kComputeUnits;
         near = plain && plain < enough ? static_cast<int>(std::min(ceil_div(enough, plain), most)) : 1;
         const int64_t piece = std::max<int64_t>(4, turns / near / 4);
-        far = far_tiles ? static_cast<int>(ceil_div(ceil_div(t->queries, turn) * group, piece)) : 1;
+        // (where tiles with sinks are many, they fill the chip uncut, and their sums would fill its memory)
+        const int64_t most_pieces = ceil_div(ceil_div(t->queries, turn) * group, piece);
+        far = far_tiles ? static_cast<int>(std::max<int64_t>(1, std::min(most_pieces, 4 * kComputeUnits / (far_tiles * heads)))) : 1;
         slots = heads * (static_cast<int64_t>(tiles - far_tiles) * near + static_cast<int64_t>(far_tiles) * far);
+        pieces = heads * ((near > 1 ? static_cast<int64_t>(tiles - far_tiles) * near : 0) +
+                          (far > 1 ? static_cast<int64_t>(far_tiles) * far : 0));
     }
     int64_t summed() const { return heads * ((near > 1 ? tiles - far_tiles : 0) + (far > 1 ? far_tiles : 0)); }
 };
@@ -481,7 +491,7 @@ extern "C" size_t isa_block_attention_backward_workspace(const isa_block_attenti
     for_shape(t, [&](auto, auto dim, auto shape) {
         using S = decltype(shape);
         const Cuts cuts(t, S::kKeys);
-        if (cuts.near > 1 || cuts.far > 1) bytes += cuts.slots * 2 * S::kKeys * decltype(dim)::value * sizeof(float);
+        bytes += cuts.pieces * 2 * S::kKeys * decltype(dim)::value * sizeof(float);
     });
     return bytes;
 }

@@ -179,6 +179,20 @@ def test_attention_refusals(lib):
     assert lib.isa_block_attention_backward_workspace(attention()) >= 2 * 4 * 8 * 4
 
 
+def test_attention_workspaces_stay_bounded(lib):
+    """A launch's partial sums are those of some thousand blocks at most, whatever the sizes."""
+    stride = {"q_strides": (0, 256, 64), "k_strides": (0, 128, 64), "v_strides": (0, 128, 64)}
+    for sinks in (0, 4, 1000, 1 << 20):
+        for window in (0, 1, 64, 5000):
+            for kind in (0, 1):
+                a = attention(type=kind, batch=1, queries=1 << 20, keys=1 << 20, window=window, sinks=sinks, **stride)
+                planes = 3 * 4 * 4 * (1 << 20)
+                assert planes <= lib.isa_block_attention_backward_workspace(a) <= planes + (400 << 20)
+                assert lib.isa_block_attention_forward_workspace(a) == 0
+            a = attention(batch=1, queries=1, keys=1 << 20, window=window, sinks=sinks, **stride)
+            assert lib.isa_block_attention_forward_workspace(a) <= 1 << 20
+
+
 def loss(**over):
     n = Loss(0, 4, 100, -100, 4096, 100, 4096)
     for k, v in over.items():

@@ -298,6 +298,36 @@ def test_graph_replays(cuda_device):
         assert torch.equal(out, call())
 
 
+def test_gradients_replay_from_a_graph(cuda_device):
+    """A captured forward and backward, replayed on new values between eager runs, give the eager bits."""
+    from isa.kernels.transformer_block import window_attention
+
+    q, k, v, g = inputs(cuda_device, 1, 400, 400, 4, 2, 64, BF16)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+
+    def call():
+        out = window_attention(*leaves, window=100, sinks=4)
+        return (out, *torch.autograd.grad(out, leaves, g))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for i in range(4):
+        print(f"[case] replay {i}", flush=True)
+        with torch.no_grad():
+            for t in (*leaves, g):
+                t.copy_(torch.randn_like(t))
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, w in zip(got, call()):
+            assert torch.equal(x, w)
+
+
 def test_refusals(cuda_device):
     from isa.kernels.transformer_block import window_attention
 
@@ -323,6 +353,41 @@ def test_refusals(cuda_device):
     refused("key_lengths", q, k, v, key_lengths=torch.ones(3, dtype=torch.int32, device=cuda_device))
     refused("key_lengths", q, k, v, key_lengths=torch.ones(2, device=cuda_device))
     refused("key_lengths", q, k, v, key_lengths=torch.ones(2, dtype=torch.int32))
+    q.requires_grad_(True)
+    (dq,) = torch.autograd.grad(window_attention(q, k, v).sum(), q)
+    assert not dq.requires_grad
+    with pytest.raises(RuntimeError, match="first derivatives only"):
+        torch.autograd.grad(window_attention(q, k, v).sum(), q, create_graph=True)
+    q.requires_grad_(False)
     # lengths out of range are held to it
     far = window_attention(q, k, v, key_lengths=torch.tensor([99, -5], device=cuda_device))
     close(far, attention64(q, k, v, None, 0, 0.125, [6, 0])[0], tolerances(F32)[0], "lengths held to the keys")
+
+
+LONG = [
+    # the walks over queries are cut: of tiles with sinks, of all tiles, of both, of none but the sinks'
+    (1, 1500, 1500, 4, 1, 64, 70, 200, None),
+    (1, 1100, 1100, 2, 2, 128, 40, 4, None),
+    (1, 700, 700, 3, 1, 96, None, 0, None),
+    (2, 900, 1400, 4, 2, 128, 300, 130, [1400, 640]),
+    (4, 600, 600, 16, 16, 32, 64, 33, None),
+    (1, 40, 3000, 4, 2, 64, 1000, 100, None),       # few rows against many keys: the keys are cut
+    (2, 3, 2500, 8, 1, 128, None, 0, [2500, 17]),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize("case", LONG, ids=str)
+def test_long_walks(cuda_device, case, dtype):
+    from isa.kernels.transformer_block import window_attention
+
+    b, m, n, h, kv, d, window, sinks, lengths = case
+    print(f"[case] attention {case} {dtype}", flush=True)
+    q, k, v, g = inputs(cuda_device, b, m, n, h, kv, d, dtype, seed=sum(case[:6]))
+    given = None if lengths is None else torch.tensor(lengths, device=cuda_device, dtype=torch.int32)
+    want = attention64(q, k, v, window, sinks, 1.0 / math.sqrt(d), lengths, g)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out = window_attention(*leaves, window=window, sinks=sinks, key_lengths=given)
+    forward, backward = tolerances(dtype)
+    for x, w, name in zip((out, *torch.autograd.grad(out, leaves, g)), want, ("out", "dq", "dk", "dv")):
+        close(x, w, forward if name == "out" else backward, name)
