@@ -74,6 +74,22 @@ __device__ __forceinline__ float dot(const RowFrags<T, D>& x, const RowFrags<T, 
     return sum;
 }
 
+// fp16 has 5 bits of exponent: gradients of a mean loss, some 1e-5, would leave ds a few bits. There ds is
+// taken of do scaled by a power of two to between 1 and 2 at its peak: a row's own for dq, that of all
+// rows of a key head for dk, which dq's waves leave behind.
+template <typename T>
+constexpr bool kScaled = std::is_same_v<T, f16>;
+
+__device__ __forceinline__ float to_one(float peak) {
+    const int e = static_cast<int>(__float_as_uint(peak) >> 23);  // (peak is not negative)
+    return e < 1 || e > 253 ? 1.0f : __uint_as_float(static_cast<unsigned>(254 - e) << 23);
+}
+
+// A wave's peaks of a key head: [tile of rows][wave].
+__device__ __forceinline__ int64_t peaks_of(const AttnArgs& a, int64_t rows_per_wave) {
+    return (static_cast<int64_t>(a.queries) * a.group + rows_per_wave - 1) / rows_per_wave;
+}
+
 template <typename T>
 __device__ __forceinline__ float probability(float s, const AttnArgs& a, float lse, float lse_rest) {
     float x = fmaf(s, a.c, -lse);
@@ -124,6 +140,20 @@ __global__ __launch_bounds__(kThreads<T>, (kDqWaves<T, D>)) void attention_dq_ke
     const float base = a.lse[2 * stat], log_sum = a.lse[2 * stat + 1];
     const float lse = sizeof(T) == 4 ? base : base + log_sum, lse_rest = log_sum;
     if (row <= last && lane < 32) put_planes<T>(a, stat, delta, base, log_sum);
+    float factor = 1.0f;
+    if constexpr (kScaled<T>) {
+        float peak = 0.0f;
+#pragma unroll
+        for (int t = 0; t < L::kSteps; ++t)
+#pragma unroll
+            for (int e = 0; e < L::N; ++e) peak = fmaxf(peak, fabsf(static_cast<float>(g[t][e])));
+        peak = half_max(peak);
+        factor = to_one(peak);
+        peak = wave_max(peak);
+        if (mine <= last && lane == 0)
+            a.peaks[(static_cast<int64_t>(b) * a.kv_heads + kv_head) * peaks_of(a, kTile) + mine / kTile] = peak;
+        if (!a.result) return;
+    }
 
     acc16 dq[DB] = {};
     const Loader<T, D, BN, kThreads<T>> kload(static_cast<const T*>(a.k) + b * a.ks[0] + kv_head * a.ks[2], a.ks[1], a.dim,
@@ -149,7 +179,10 @@ __global__ __launch_bounds__(kThreads<T>, (kDqWaves<T, D>)) void attention_dq_ke
             }
             reads_ahead<2 * L::kSteps, 2 * L::kSteps * L::kMmas, 4>();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = probability<T>(s[i], a, lse, lse_rest) * (d[i] - delta);
+            for (int i = 0; i < 16; ++i) {
+                s[i] = probability<T>(s[i], a, lse, lse_rest) * (d[i] - delta);
+                if constexpr (kScaled<T>) s[i] *= factor;
+            }
             if (!sight.all) {
                 const Range seen(a, span.of_sinks(it), span.sink, p, j0, half);
 #pragma unroll
@@ -185,7 +218,7 @@ __global__ __launch_bounds__(kThreads<T>, (kDqWaves<T, D>)) void attention_dq_ke
         if (it + 2 < span.count) fetch(it + 2, k0, v0);
         compute(it + 1, k1, v1);
     }
-    if (row <= last) store_row<T, DB>(static_cast<T*>(a.result) + at.packed(a, b), dq, a.scale, a.dim, lane);
+    if (row <= last) store_row<T, DB>(static_cast<T*>(a.result) + at.packed(a, b), dq, a.scale / factor, a.dim, lane);
 }
 
 // ---- dk and dv ------------------------------------------------------------------------------
@@ -256,6 +289,14 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
         v[n].load(key < length ? static_cast<const T*>(a.v) + b * a.vs[0] + kv_head * a.vs[2] + key * a.vs[1] : nullptr,
                   a.dim, lane);
     }
+    float factor = 1.0f;
+    if constexpr (kScaled<T>) {
+        const int64_t count = peaks_of(a, kTile);
+        const float* peaks = a.peaks + (static_cast<int64_t>(b) * a.kv_heads + kv_head) * count;
+        float peak = 0.0f;
+        for (int64_t n = lane; n < count; n += kWave) peak = fmaxf(peak, peaks[n]);
+        factor = to_one(wave_max(peak));
+    }
     const Seen seen(a, length, j0, j0 + S::kKeys);
     const int turns = (seen.end - seen.first + BR - 1) / BR, all_turns = turns * a.group;
     const int begin = static_cast<int>(static_cast<int64_t>(all_turns) * split / splits);
@@ -313,7 +354,7 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
                     for (int e = 0; e < 4; ++e) {
                         const float x = probability<T>(s[i + e], a, lse[e], rest[e]), y = x * (d[i + e] - delta[e]);
                         s[i + e] = x;
-                        d[i + e] = y;
+                        d[i + e] = kScaled<T> ? y * factor : y;
                     }
                 }
                 if (!all) {
@@ -363,7 +404,8 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
                 for (int i = 0; i < 16; i += 4) {
                     const int at = ((n * DB + db) * 4 + i / 4) * S::kThreadCount * 4;
                     using F = vec<float, 4>;
-                    *reinterpret_cast<F*>(p + at) = F{dk[n][db][i], dk[n][db][i + 1], dk[n][db][i + 2], dk[n][db][i + 3]};
+                    *reinterpret_cast<F*>(p + at) =
+                        F{dk[n][db][i], dk[n][db][i + 1], dk[n][db][i + 2], dk[n][db][i + 3]} * (1.0f / factor);
                     *reinterpret_cast<F*>(p + S::kKeys * D + at) =
                         F{dv[n][db][i], dv[n][db][i + 1], dv[n][db][i + 2], dv[n][db][i + 3]};
                 }
@@ -374,7 +416,7 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
         const int key = mine + 32 * n + lane % 32;
         if (key >= a.keys) continue;
         const int64_t out = ((static_cast<int64_t>(b) * a.keys + key) * a.kv_heads + kv_head) * a.dim;
-        store_row<T, DB>(static_cast<T*>(a.dk) + out, dk[n], a.scale, a.dim, lane);
+        store_row<T, DB>(static_cast<T*>(a.dk) + out, dk[n], a.scale / factor, a.dim, lane);
         store_row<T, DB>(static_cast<T*>(a.dv) + out, dv[n], 1.0f, a.dim, lane);
     }
 }
@@ -449,15 +491,21 @@ size_t plane_bytes(const isa_block_attention* t) {
     return ceil_div(t->batch * t->heads * t->queries, 64) * 64 * kPlanes * sizeof(float);
 }
 
+size_t peak_bytes(const isa_block_attention* t) {
+    if (t->type != ISA_BLOCK_F16) return 0;
+    const int64_t each = ceil_div(t->queries * (t->heads / t->kv_heads), kTile);
+    return ceil_div(t->batch * t->kv_heads * each, 64) * 64 * sizeof(float);
+}
+
 template <typename T, int D>
 void launch(AttnArgs a, const isa_block_attention* t, hipStream_t s) {
     using S = DkvShape<T, D>;
     const int64_t rows = static_cast<int64_t>(a.batch) * a.queries * a.heads;
     if (rows) {
         const int64_t tiles = ceil_div(static_cast<int64_t>(a.queries) * a.group, kRows<T>);
-        if (a.result)
+        if (a.result || kScaled<T>)
             attention_dq_kernel<T, D><<<dim3(static_cast<unsigned>(tiles * a.batch * a.kv_heads)), kThreads<T>, 0, s>>>(a);
-        else
+        else if constexpr (!kScaled<T>)
             attention_rows_kernel<T><<<dim3(static_cast<unsigned>(ceil_div(rows * 16, kRowThreads))), kRowThreads, 0, s>>>(a);
     }
     if (!a.dk || !a.keys) return;
@@ -487,7 +535,7 @@ using namespace isa_block;
 
 extern "C" size_t isa_block_attention_backward_workspace(const isa_block_attention* t) {
     if (!t || check_attention(t)) return 0;
-    size_t bytes = plane_bytes(t);
+    size_t bytes = plane_bytes(t) + peak_bytes(t);
     for_shape(t, [&](auto, auto dim, auto shape) {
         using S = decltype(shape);
         const Cuts cuts(t, S::kKeys);
@@ -522,7 +570,8 @@ extern "C" int isa_block_attention_backward(const isa_block_attention* t, const 
     a.dout = dout;
     a.lse = const_cast<float*>(lse);
     a.delta = static_cast<float*>(workspace);
-    a.partial = a.delta + plane_bytes(t) / sizeof(float);
+    a.peaks = a.delta + plane_bytes(t) / sizeof(float);
+    a.partial = a.peaks + peak_bytes(t) / sizeof(float);
     a.result = dq;
     a.dk = dk;
     a.dv = dv;

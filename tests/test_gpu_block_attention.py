@@ -391,3 +391,28 @@ def test_long_walks(cuda_device, case, dtype):
     forward, backward = tolerances(dtype)
     for x, w, name in zip((out, *torch.autograd.grad(out, leaves, g)), want, ("out", "dq", "dk", "dv")):
         close(x, w, forward if name == "out" else backward, name)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize("scale", [2.0 ** -17, 2.0 ** 12])
+def test_gradients_of_any_size(cuda_device, dtype, scale):
+    """Gradients of a mean loss are small, those of a scaled one large: the result scales with them, to
+    what its type holds (in fp16 2^-25 is half its smallest number)."""
+    from isa.kernels.transformer_block import window_attention
+
+    print(f"[case] gradients of {scale} {dtype}", flush=True)
+    for m, n, window, sinks in ((200, 200, 64, 3), (900, 900, 100, 4)):
+        q, k, v, g = inputs(cuda_device, 1, m, n, 4, 2, 64, dtype, seed=11)
+        g = (g.float() * scale).to(dtype)
+        want = attention64(q, k, v, window, sinks, 0.125, None, g)[1:]
+        leaves = [t.requires_grad_(True) for t in (q, k, v)]
+        out = window_attention(*leaves, window=window, sinks=sinks)
+        for x, w, name in zip(torch.autograd.grad(out, leaves, g), want, ("dq", "dk", "dv")):
+            floor = 2.0 ** -25 * math.sqrt(w.numel()) / float(w.norm()) if dtype == F16 else 0.0
+            close(x, w, tolerances(dtype)[1] + floor, name)
+        # keys and values alone, whose kernel takes the rows' sums from elsewhere
+        k2, v2 = (t.detach().clone().requires_grad_(True) for t in (k, v))
+        for x, w, name in zip(torch.autograd.grad(window_attention(q.detach(), k2, v2, window=window, sinks=sinks), (k2, v2), g),
+                              want[1:], ("dk alone", "dv alone")):
+            floor = 2.0 ** -25 * math.sqrt(w.numel()) / float(w.norm()) if dtype == F16 else 0.0
+            close(x, w, tolerances(dtype)[1] + floor, name)
