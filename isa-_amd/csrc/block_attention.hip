@@ -112,17 +112,21 @@ __device__ __forceinline__ void finish(Running<D / 32>& r, const AttnArgs& a, co
     }
 }
 
+// Waves to a SIMD that registers are to leave room for.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads<T>) void attention_forward_kernel(AttnArgs a) {
+constexpr int kForwardWaves = sizeof(T) == 4 && D <= 64 ? 3 : 1;
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads<T>, (kForwardWaves<T, D>)) void attention_forward_kernel(AttnArgs a) {
     using L = Tile<T, D>;
     constexpr int BN = kKeyTile<T>, NK = BN / 32, kRows = isa_block::kRows<T>;
-    __shared__ __attribute__((aligned(1024))) T k0[BN * L::kPitch], v0[BN * L::kPitch], k1[BN * L::kPitch],
-        v1[BN * L::kPitch];
+    constexpr int kSecond = kOneTile<T> ? 1 : BN * L::kPitch;
+    __shared__ __attribute__((aligned(1024))) T k0[BN * L::kPitch], v0[BN * L::kPitch], k1[kSecond], v1[kSecond];
     const int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), half = lane / 32;
     const int rows = a.queries * a.group, tiles = (rows + kRows - 1) / kRows;
-    const int id = xcd_order(blockIdx.x, gridDim.x), task = id / a.splits, split = id % a.splits;
-    const int kv_head = task / tiles % a.kv_heads, b = task / tiles / a.kv_heads;
-    const int row0 = (tiles - 1 - task % tiles) * kRows;  // rows that see the most keys first
+    const Piece piece(blockIdx.x, gridDim.x, a.batch * a.kv_heads, tiles * a.splits);
+    const int kv_head = piece.head % a.kv_heads, b = piece.head / a.kv_heads, split = piece.slot % a.splits;
+    const int row0 = (tiles - 1 - piece.slot / a.splits) * kRows;  // rows that see the most keys first
     const int shift = length_of(a, b) - a.queries, last = min(row0 + kRows, rows) - 1;
     const Span<BN> span(a, shift + row0 / a.group, shift + last / a.group);
     const int begin = span.count * split / a.splits, end = span.count * (split + 1) / a.splits;
@@ -139,16 +143,13 @@ __global__ __launch_bounds__(kThreads<T>) void attention_forward_kernel(AttnArgs
                                            threadIdx.x);
     const Loader<T, D, BN, kThreads<T>> vload(static_cast<const T*>(a.v) + b * a.vs[0] + kv_head * a.vs[2], a.vs[1], a.dim,
                                            threadIdx.x);
-    auto fetch = [&](int it, T* kt, T* vt) {
-        const int j0 = span.first(it), je = span.end(it);
-        kload.load(kt, 0, j0, je, wave);
-        vload.load(vt, 0, j0, je, wave);
-    };
-    auto compute = [&](int it, const T* kt, const T* vt) {
+    auto fetch_k = [&](int it, T* kt) { kload.load(kt, 0, span.first(it), span.end(it), wave); };
+    auto fetch_v = [&](int it, T* vt) { vload.load(vt, 0, span.first(it), span.end(it), wave); };
+    // false where no row of the wave sees a key of the tile
+    auto scores = [&](int it, const T* kt, acc16(&s)[NK]) {
         const int j0 = span.first(it);
         const Sight<BN> sight(a, span, it, j0, pmin, pmax);
-        if (sight.none) return;
-        acc16 s[NK];
+        if (sight.none) return false;
 #pragma unroll
         for (int n = 0; n < NK; ++n) {
             s[n] = acc16{};
@@ -164,19 +165,42 @@ __global__ __launch_bounds__(kThreads<T>) void attention_forward_kernel(AttnArgs
                 for (int i = 0; i < 16; ++i)
                     s[n][i] = seen.has(32 * n + product_row(i, 0)) ? s[n][i] : -INFINITY;
         }
-        attend<T, D, NK>(r, s, vt, a, span.of_sinks(it), lane);
+        return true;
     };
-    if (begin < end) fetch(begin, k0, v0);
-    for (int it = begin; it < end; it += 2) {
-        loads_arrived();
-        __syncthreads();
-        if (it + 1 < end) fetch(it + 1, k1, v1);
-        compute(it, k0, v0);
-        if (it + 1 >= end) break;
-        loads_arrived();
-        __syncthreads();
-        if (it + 2 < end) fetch(it + 2, k0, v0);
-        compute(it + 1, k1, v1);
+    if constexpr (kOneTile<T>) {  // V's copy runs beside the scores, the next K's beside V's product
+        if (begin < end) fetch_k(begin, k0);
+        for (int it = begin; it < end; ++it) {
+            loads_arrived();
+            __syncthreads();
+            fetch_v(it, v0);
+            acc16 s[NK];
+            const bool any = scores(it, k0, s);
+            loads_arrived();
+            __syncthreads();
+            if (it + 1 < end) fetch_k(it + 1, k0);
+            if (any) attend<T, D, NK>(r, s, v0, a, span.of_sinks(it), lane);
+        }
+    } else {
+        auto compute = [&](int it, const T* kt, const T* vt) {
+            acc16 s[NK];
+            if (scores(it, kt, s)) attend<T, D, NK>(r, s, vt, a, span.of_sinks(it), lane);
+        };
+        auto fetch = [&](int it, T* kt, T* vt) {
+            fetch_k(it, kt);
+            fetch_v(it, vt);
+        };
+        if (begin < end) fetch(begin, k0, v0);
+        for (int it = begin; it < end; it += 2) {
+            loads_arrived();
+            __syncthreads();
+            if (it + 1 < end) fetch(it + 1, k1, v1);
+            compute(it, k0, v0);
+            if (it + 1 >= end) break;
+            loads_arrived();
+            __syncthreads();
+            if (it + 2 < end) fetch(it + 2, k0, v0);
+            compute(it + 1, k1, v1);
+        }
     }
     if (row <= last) finish<T, D>(r, a, at, b, split, lane);
 }

@@ -101,8 +101,8 @@ __device__ __forceinline__ float weight(float s, float c, float c_rest, float ba
 // A row's 16-byte chunks lie in a power of two of slots, chunk c in slot c ^ key(row), so that both
 // kinds of reads use all banks: 16 rows' of one chunk, and 4 rows' of 4 adjacent chunks (the
 // transposing read: with keys that leave those 4 chunks in their 64 bytes it takes twice the time).
-// Tiles are loaded straight to LDS, 64 slots an
-// instruction; a buffer descriptor that ends with the last row makes what is behind it zeros.
+// Tiles are loaded straight to LDS, 64 slots an instruction; a buffer descriptor that ends with the last
+// row makes what is behind it zeros.
 
 constexpr int slots_for(int chunks) { return chunks <= 4 ? 4 : chunks <= 8 ? 8 : chunks <= 16 ? 16 : 32; }
 
@@ -119,26 +119,33 @@ struct Tile {
     using V = typename Frag<T>::V;
 
     // 256 bytes of banks: 4, 2, 1 or half a row
-    static __device__ __forceinline__ constexpr int key(int row) {
-        const int by_four = row / 4 % 4;
+    static __device__ __forceinline__ constexpr unsigned key(unsigned row) {
+        const unsigned by_four = row / 4 % 4;
         return kSlots == 4 ? by_four : kSlots == 8 ? row / 2 % 2 * 4 + by_four : row % 4 * 4 + by_four;
     }
 
+    // Below, what depends on the lane is one place, and a chunk's slot differs from it by an exclusive or
+    // with a constant: the rest of an address goes into the instruction. In fp32 each other VALU
+    // instruction is time that the products lose (they take the same units: 32x32x2 products of 3 waves
+    // a SIMD alone 139 TF/s, with 4 instructions to each 116, with 8 102).
+
     // of row (r0 + lane % 32), the dims of step t
-    static __device__ __forceinline__ V row(const T* tile, int r0, int t, int lane) {
-        const int r = lane % 32;
-        return *reinterpret_cast<const V*>(tile + r0 * kPitch + r * kPitch + ((2 * t + lane / 32) ^ key(r)) * N);
+    static __device__ __forceinline__ V row(const T* tile, int r0, int t, int lane_) {
+        const unsigned lane = lane_ % 64u, r = lane % 32;
+        const unsigned place = r * kPitch + (lane / 32 ^ key(r)) * N;
+        return *reinterpret_cast<const V*>(tile + r0 * kPitch + (place ^ 2 * t * N));
     }
 
     // of column (32 db + lane % 32), the rows r0 .. r0 + 31 that operand(x, u) holds in this half
-    static __device__ __forceinline__ V column(const T* tile, int r0, int u, int db, int lane) {
+    static __device__ __forceinline__ V column(const T* tile, int r0, int u, int db, int lane_) {
+        const unsigned lane = lane_ % 64u, half = lane / 32;
         if constexpr (sizeof(T) == 4) {
             V f;
-            const int at = 8 * db + lane % 32 / 4;
+            const unsigned place = 4 * half * kPitch + (lane % 32 / 4 ^ half) * N + lane % 4;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int r = 8 * u + 4 * (lane / 32) + e;
-                f[e] = tile[r0 * kPitch + r * kPitch + (at ^ key(r)) * N + lane % 4];
+                const int other = key(8 * u + e) ^ 8 * db;  // (that of row 4 is 1)
+                f[e] = tile[(r0 + 8 * u + e) * kPitch + other / 8 * 8 * N + (place ^ other % 8 * N)];
             }
             return f;
         } else {
@@ -150,11 +157,12 @@ struct Tile {
                 s4 part[2];
                 V f;
             } x;
-            const int at = 4 * db + lane / 16 % 2 * 2 + lane % 4 / 2;
+            const unsigned r = 4 * half + lane % 16 / 4;
+            const unsigned place = r * kPitch + (lane / 16 % 2 * 2 + lane % 4 / 2 ^ key(r)) * N + lane % 2 * 4;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int r = 8 * j + 4 * (lane / 32) + lane % 16 / 4;  // 16 u further on the key is the same
-                const T* p = tile + (r0 + 16 * u) * kPitch + r * kPitch + (at ^ key(r)) * N + lane % 2 * 4;
+                // (8 rows further on the key differs by 2, 16 further it is the same)
+                const T* p = tile + (r0 + 16 * u + 8 * j) * kPitch + (place ^ (4 * db ^ 2 * j) * N);
                 x.part[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds*)const_cast<T*>(p));
             }
             return x.f;
@@ -176,7 +184,8 @@ using LdsBytes = __attribute__((address_space(3))) char*;
 constexpr int kBufferFlags = 0x00027000;  // raw buffer of 32-bit data
 constexpr unsigned kOutside = 0x7fffffffu;
 
-// COUNT times BYTES a lane to `lds` (an array: its address is known) + first, `step` bytes apart, from the buffer of `size` bytes at `base` (uniform); what lies outside is zeros.
+// COUNT times BYTES a lane to `lds` (an array: its address is known) + first, `step` bytes apart, from the
+// buffer of `size` bytes at `base` (uniform); what lies outside is zeros.
 // (The buffer's type exists for the device alone: the host's pass over the kernels does without.)
 template <int BYTES, int COUNT>
 __device__ __forceinline__ void load_to_lds(void* lds, int first, int step, const void* base, int size,
@@ -230,12 +239,29 @@ __device__ __forceinline__ void load_floats(float* lds, int place, const float* 
 // All of this wave's loads to LDS have arrived.
 __device__ __forceinline__ void loads_arrived() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
 
-// Dispatch gives block i to XCD i % 8; this gives each XCD a run of adjacent work, whose keys its
-// L2 then holds once.
-__device__ __forceinline__ int xcd_order(int id, int n) {
-    const int per = n / 8, rest = n % 8, x = id % 8;
-    return x * per + min(x, rest) + id / 8;
-}
+// Which of a key head's `slots` pieces of work, the longest first, block `id` of heads * slots takes.
+// Dispatch gives block i to XCD i % 8 and there to compute unit i / 8 % 32. Heads are dealt to XCDs,
+// whose L2 then holds their keys once, and taken in bundles of as many as fill an XCD (8 blocks a unit),
+// the longest pieces of all heads of a bundle first; every other row of 32 blocks is turned round.
+// So a unit gets long and short pieces; head by head, 16 pieces to a head would put all of one length in
+// one unit (8 x 1024 tokens, 12 heads of 64 without a window: forward, dq, dk and dv in fp32 168 + 227 + 298 us
+// against 224 + 369 + 437, in bf16 27 + 35 against 36 + 46; with a window the two are alike).
+struct Piece {
+    int head, slot;
+    __device__ __forceinline__ Piece(int id, int total, int heads, int slots) {
+        constexpr int kXcds = 8, kUnits = 32;
+        const int x = id % kXcds, mine = (total - x + kXcds - 1) / kXcds;
+        int at = id / kXcds;
+        if (at / kUnits % 2) at = at / kUnits * kUnits + min(at / kUnits * kUnits + kUnits, mine) - 1 - at;
+        id = at * kXcds + x;
+        const int groups = min(heads & -heads, kXcds), each = heads / groups;  // a power of two that divides heads
+        const int group = id % groups, rank = id / groups;
+        const int bundle = min((kUnits * 8 + slots - 1) / slots, each), first = rank / (bundle * slots) * bundle;
+        const int here = min(bundle, each - first), in = rank - first * slots;
+        head = group * each + first + in % here;
+        slot = in / here;
+    }
+};
 
 // ---- which keys a block of rows sees --------------------------------------------------------
 
@@ -403,15 +429,24 @@ constexpr int kKeyTile = sizeof(T) == 4 ? 32 : 64;
 
 // Waves, of 32 rows each, that share a block's tiles. At the edges of a window they wait for each other
 // with nothing to compute; products in fp32 take 16 times as long as their operands' reads allow, so
-// there fewer share (GPT-L's step in fp32, window 256: forward and dq 114 + 164 us by fours, 107 + 148 by
-// twos, 121 + 169 alone; dk and dv 241, 205 and 188). 16-bit products need the sharing (2 x 4096 tokens of
-// 128-wide heads, window 1024: 97 + 127 + 172 us by fours, 122 + 172 + 269 by twos).
+// there fewer share (GPT-L's step in fp32, window 256, with two tiles of each operand: forward and dq
+// 114 + 164 us by fours, 107 + 148 by twos, 121 + 169 alone; dk and dv 241, 205 and 188). 16-bit products
+// need the sharing (2 x 4096 tokens of 128-wide heads, window 1024: 97 + 127 + 172 us by fours,
+// 122 + 172 + 269 by twos).
 template <typename T>
 constexpr int kWaves = sizeof(T) == 4 ? 2 : 4;
 template <typename T>
 constexpr int kThreads = kWaves<T> * kWave;
 template <typename T>
 constexpr int kRows = kWaves<T> * kTile;
+
+// One tile in LDS of each operand instead of two, in the forward and in dk's and dv's walk: the next one's copy
+// starts when the products that read it are done, beside those of the other operand. In fp32 those take long
+// enough for it to arrive, and LDS for two would be what limits the waves (8 x 1024 tokens of 64-wide heads,
+// window 256: forward 90 us against 116; 2 x 4096 of 128-wide ones, window 1024: 597 against 627, dk and dv
+// 1216 against 2201). dq, which reads K twice, gains nothing (924 against 890).
+template <typename T>
+constexpr bool kOneTile = sizeof(T) == 4;
 
 int check_attention(const isa_block_attention* t);
 AttnArgs attention_args(const isa_block_attention* t);

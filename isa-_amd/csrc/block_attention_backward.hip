@@ -98,11 +98,12 @@ __device__ __forceinline__ float probability(float s, const AttnArgs& a, float l
 }
 
 // Two waves to a SIMD, so that one's products run beside the other's softmax, where 256 registers hold
-// a wave's operands and sums.
+// a wave's operands and sums; three where 168 do (dk and dv of fp16 heads of 64, 8 x 1024 tokens without a
+// window: 47 us against 54).
 template <typename T, int D>
 constexpr int kDqWaves = sizeof(T) == 2 || D <= 64 ? 2 : 1;
 template <typename T, int D>
-constexpr int kDkvWaves = sizeof(T) == 2 || D <= 64 ? 2 : 1;
+constexpr int kDkvWaves = sizeof(T) == 2 ? (D <= 64 ? 3 : 2) : D <= 64 ? 2 : 1;
 
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads<T>, (kDqWaves<T, D>)) void attention_dq_kernel(AttnArgs a) {
@@ -112,9 +113,9 @@ __global__ __launch_bounds__(kThreads<T>, (kDqWaves<T, D>)) void attention_dq_ke
         v1[BN * L::kPitch];
     const int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), half = lane / 32;
     const int rows = a.queries * a.group, tiles = (rows + kRows - 1) / kRows;
-    const int id = xcd_order(blockIdx.x, gridDim.x);
-    const int kv_head = id / tiles % a.kv_heads, b = id / tiles / a.kv_heads;
-    const int row0 = (tiles - 1 - id % tiles) * kRows;
+    const Piece piece(blockIdx.x, gridDim.x, a.batch * a.kv_heads, tiles);
+    const int kv_head = piece.head % a.kv_heads, b = piece.head / a.kv_heads;
+    const int row0 = (tiles - 1 - piece.slot) * kRows;
     const int shift = length_of(a, b) - a.queries, last = min(row0 + kRows, rows) - 1;
     const Span<BN> span(a, shift + row0 / a.group, shift + last / a.group);
 
@@ -258,15 +259,15 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
     using L = Tile<T, D>;
     using S = DkvShape<T, D>;
     constexpr int BR = S::BR, DB = D / 32, KB = S::KB;
-    __shared__ __attribute__((aligned(1024))) T q0[BR * L::kPitch], g0[BR * L::kPitch], q1[BR * L::kPitch],
-        g1[BR * L::kPitch];
-    __shared__ __attribute__((aligned(1024))) float stat0[kPlanes * 64], stat1[kPlanes * 64];
+    constexpr int kSecond = kOneTile<T> ? 1 : BR * L::kPitch;
+    __shared__ __attribute__((aligned(1024))) T q0[BR * L::kPitch], g0[BR * L::kPitch], q1[kSecond], g1[kSecond];
+    __shared__ __attribute__((aligned(1024))) float stat0[kPlanes * 64], stat1[kOneTile<T> ? 1 : kPlanes * 64];
     const int outer = threadIdx.x % kWave, lane = outer, wave = uniform(threadIdx.x / kWave);
     const int tiles = (a.keys + S::kKeys - 1) / S::kKeys;
     // a key head's blocks: those of the tiles without sinks, then those of the tiles with
     const int plain = tiles - a.far_tiles, per_head = plain * a.near + a.far_tiles * a.far;
-    const int id = xcd_order(blockIdx.x, gridDim.x);
-    const int kv_head = id / per_head % a.kv_heads, b = id / per_head / a.kv_heads, slot = id % per_head;
+    const Piece piece(blockIdx.x, gridDim.x, a.batch * a.kv_heads, per_head);
+    const int kv_head = piece.head % a.kv_heads, b = piece.head / a.kv_heads, slot = piece.slot;
     const bool far = slot >= plain * a.near;
     const int splits = far ? a.far : a.near, in = far ? slot - plain * a.near : slot;
     const int tile = (far ? 0 : a.far_tiles) + in / splits, split = in % splits;
@@ -311,86 +312,129 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
         static_cast<const T*>(a.dout) + b * a.gs[0] + static_cast<int64_t>(kv_head) * a.group * a.gs[2], a.gs[1], a.dim,
         threadIdx.x);
     const float* stats = a.delta + (static_cast<int64_t>(b) * a.heads + kv_head * a.group) * a.queries;
-    auto fetch = [&](int it, T* qt, T* gt, float* stat) {
+    auto fetch_q = [&](int it, T* qt, float* stat) {
         const int head = it / turns, i0 = seen.first + (it - head * turns) * BR;
-        const int64_t qat = (head * a.qs[2] + i0 * a.qs[1]) * static_cast<int64_t>(sizeof(T));
-        const int64_t gat = (head * a.gs[2] + i0 * a.gs[1]) * static_cast<int64_t>(sizeof(T));
-        qload.load_from(qt, 0, qload.base + qat, seen.end - i0, wave);
-        gload.load_from(gt, 0, gload.base + gat, seen.end - i0, wave);
+        const int64_t from = (head * a.qs[2] + i0 * a.qs[1]) * static_cast<int64_t>(sizeof(T));
+        qload.load_from(qt, 0, qload.base + from, seen.end - i0, wave);
         const int64_t at = static_cast<int64_t>(head) * a.queries + i0;
 #pragma unroll
         for (int n = 0; n < (sizeof(T) == 4 ? 3 : 2); ++n)
             if (n % S::kWaveCount == wave) load_floats(stat, 64 * n, stats + n * plane, at, seen.end - i0, lane);
     };
-    auto compute = [&](int it, const T* qt, const T* gt, const float* stat) {
-        const int lane = opaque(outer), half = lane / 32;
-        const int i0 = seen.first + it % turns * BR;
-        const int pmin = shift + i0, pmax = shift + min(i0 + BR, seen.end) - 1;
-#pragma unroll
-        for (int r = 0; r < BR / 32; ++r)
-#pragma unroll
-            for (int n = 0; n < KB; ++n) {
-                const int first = mine + 32 * n, key = first + lane % 32;
-                const int plo = pmin + 32 * r, phi = min(plo + 31, pmax);
-                if (first > phi || (first + 31 <= plo - a.window && first >= a.sinks)) continue;
-                const bool all = first + 31 <= plo && (first + 32 <= a.sinks || first > phi - a.window);
-                acc16 s = {}, d = {};
-#pragma unroll
-                for (int t = 0; t < L::kSteps; ++t) {
-                    mma(s, L::row(qt, 32 * r, t, lane), k[n][t]);
-                    mma(d, L::row(gt, 32 * r, t, lane),
-                        S::kHoldV ? v[n][t] : L::row(held, wave * 32 * KB + 32 * n, t, lane));
-                }
-                reads_ahead<(S::kHoldV ? 2 : 3) * L::kSteps, 2 * L::kSteps * L::kMmas, 4>();
-#pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const int at = 32 * r + product_row(i, half);
-                    using F = vec<float, 4>;
-                    const F delta = *reinterpret_cast<const F*>(stat + 64 * kDelta + at);
-                    const F lse = *reinterpret_cast<const F*>(stat + 64 * kLse + at);
-                    F rest{};
-                    if constexpr (sizeof(T) == 4) rest = *reinterpret_cast<const F*>(stat + 64 * kLseRest + at);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float x = probability<T>(s[i + e], a, lse[e], rest[e]), y = x * (d[i + e] - delta[e]);
-                        s[i + e] = x;
-                        d[i + e] = kScaled<T> ? y * factor : y;
-                    }
-                }
-                if (!all) {
-                    // queries at key .. key + window - 1 see it, of a sink all from it on
-                    const int from = key - pmin - 32 * r - 4 * half;
-                    const unsigned count = key < a.sinks ? INT_MAX : a.window;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const bool seen = static_cast<unsigned>(product_row(i, 0) - from) < count;
-                        s[i] = seen ? s[i] : 0.0f;
-                        d[i] = seen ? d[i] : 0.0f;
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < L::kUses; ++u) {
-                    const typename Frag<T>::V f = operand<T>(s, u), h = operand<T>(d, u);
-#pragma unroll
-                    for (int db = 0; db < DB; ++db) {
-                        mma(dv[n][db], L::column(gt, 32 * r, u, db, lane), f);
-                        mma(dk[n][db], L::column(qt, 32 * r, u, db, lane), h);
-                    }
-                }
-                reads_ahead<2 * L::kUses * DB * L::kColumnReads, 2 * L::kUses * DB * L::kMmas, 4 * L::kColumnReads>();
-            }
+    auto fetch_g = [&](int it, T* gt) {
+        const int head = it / turns, i0 = seen.first + (it - head * turns) * BR;
+        const int64_t from = (head * a.gs[2] + i0 * a.gs[1]) * static_cast<int64_t>(sizeof(T));
+        gload.load_from(gt, 0, gload.base + from, seen.end - i0, wave);
     };
-    if (begin < end) fetch(begin, q0, g0, stat0);
-    for (int it = begin; it < end; it += 2) {
-        loads_arrived();
-        __syncthreads();
-        if (it + 1 < end) fetch(it + 1, q1, g1, stat1);
-        compute(it, q0, g0, stat0);
-        if (it + 1 >= end) break;
-        loads_arrived();
-        __syncthreads();
-        if (it + 2 < end) fetch(it + 2, q0, g0, stat0);
-        compute(it + 1, q1, g1, stat1);
+    // s = p and d = ds of 32 queries and 32 keys; false where none of them sees any
+    auto gradients = [&](int it, int r, int n, const T* qt, const T* gt, const float* stat, acc16& s, acc16& d, int lane) {
+        const int half = lane / 32, i0 = seen.first + it % turns * BR;
+        const int pmin = shift + i0, pmax = shift + min(i0 + BR, seen.end) - 1;
+        const int first = mine + 32 * n, key = first + lane % 32;
+        const int plo = pmin + 32 * r, phi = min(plo + 31, pmax);
+        if (first > phi || (first + 31 <= plo - a.window && first >= a.sinks)) return false;
+        const bool all = first + 31 <= plo && (first + 32 <= a.sinks || first > phi - a.window);
+        s = acc16{};
+        d = acc16{};
+#pragma unroll
+        for (int t = 0; t < L::kSteps; ++t) {
+            mma(s, L::row(qt, 32 * r, t, lane), k[n][t]);
+            mma(d, L::row(gt, 32 * r, t, lane), S::kHoldV ? v[n][t] : L::row(held, wave * 32 * KB + 32 * n, t, lane));
+        }
+        reads_ahead<(S::kHoldV ? 2 : 3) * L::kSteps, 2 * L::kSteps * L::kMmas, 4>();
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int at = 32 * r + product_row(i, half);
+            using F = vec<float, 4>;
+            const F delta = *reinterpret_cast<const F*>(stat + 64 * kDelta + at);
+            const F lse = *reinterpret_cast<const F*>(stat + 64 * kLse + at);
+            F rest{};
+            if constexpr (sizeof(T) == 4) rest = *reinterpret_cast<const F*>(stat + 64 * kLseRest + at);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = probability<T>(s[i + e], a, lse[e], rest[e]), y = x * (d[i + e] - delta[e]);
+                s[i + e] = x;
+                d[i + e] = kScaled<T> ? y * factor : y;
+            }
+        }
+        if (!all) {
+            // queries at key .. key + window - 1 see it, of a sink all from it on
+            const int from = key - pmin - 32 * r - 4 * half;
+            const unsigned count = key < a.sinks ? INT_MAX : a.window;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const bool seen = static_cast<unsigned>(product_row(i, 0) - from) < count;
+                s[i] = seen ? s[i] : 0.0f;
+                d[i] = seen ? d[i] : 0.0f;
+            }
+        }
+        return true;
+    };
+    if constexpr (kOneTile<T>) {  // Q's tile is free after dk, dO's after dv
+        static_assert(BR == kTile && KB == 1);
+        auto add = [&](acc16(&sum)[DB], const T* tile, const acc16& x, int lane) {
+#pragma unroll
+            for (int u = 0; u < L::kUses; ++u) {
+                const typename Frag<T>::V f = operand<T>(x, u);
+#pragma unroll
+                for (int db = 0; db < DB; ++db) mma(sum[db], L::column(tile, 0, u, db, lane), f);
+            }
+            reads_ahead<L::kUses * DB * L::kColumnReads, L::kUses * DB * L::kMmas, 4 * L::kColumnReads>();
+        };
+        if (begin < end) {
+            fetch_q(begin, q0, stat0);
+            fetch_g(begin, g0);
+        }
+        for (int it = begin; it < end; ++it) {
+            loads_arrived();
+            __syncthreads();
+            const int lane = opaque(outer);
+            acc16 s, d;
+            const bool any = gradients(it, 0, 0, q0, g0, stat0, s, d, lane);
+            if (any) add(dk[0], q0, d, lane);
+            __syncthreads();
+            if (it + 1 < end) fetch_q(it + 1, q0, stat0);
+            if (any) add(dv[0], g0, s, lane);
+            __syncthreads();
+            if (it + 1 < end) fetch_g(it + 1, g0);
+        }
+    } else {
+        auto fetch = [&](int it, T* qt, T* gt, float* stat) {
+            fetch_q(it, qt, stat);
+            fetch_g(it, gt);
+        };
+        auto compute = [&](int it, const T* qt, const T* gt, const float* stat) {
+            const int lane = opaque(outer);
+#pragma unroll
+            for (int r = 0; r < BR / 32; ++r)
+#pragma unroll
+                for (int n = 0; n < KB; ++n) {
+                    acc16 s, d;
+                    if (!gradients(it, r, n, qt, gt, stat, s, d, lane)) continue;
+#pragma unroll
+                    for (int u = 0; u < L::kUses; ++u) {
+                        const typename Frag<T>::V f = operand<T>(s, u), h = operand<T>(d, u);
+#pragma unroll
+                        for (int db = 0; db < DB; ++db) {
+                            mma(dv[n][db], L::column(gt, 32 * r, u, db, lane), f);
+                            mma(dk[n][db], L::column(qt, 32 * r, u, db, lane), h);
+                        }
+                    }
+                    reads_ahead<2 * L::kUses * DB * L::kColumnReads, 2 * L::kUses * DB * L::kMmas, 4 * L::kColumnReads>();
+                }
+        };
+        if (begin < end) fetch(begin, q0, g0, stat0);
+        for (int it = begin; it < end; it += 2) {
+            loads_arrived();
+            __syncthreads();
+            if (it + 1 < end) fetch(it + 1, q1, g1, stat1);
+            compute(it, q0, g0, stat0);
+            if (it + 1 >= end) break;
+            loads_arrived();
+            __syncthreads();
+            if (it + 2 < end) fetch(it + 2, q0, g0, stat0);
+            compute(it + 1, q1, g1, stat1);
+        }
     }
     if (splits > 1) {  // [piece of a cut tile][dk, dv][key block, dims' quarter][thread]
         const int64_t mine_at = (static_cast<int64_t>(b) * a.kv_heads + kv_head) * pieces_per_head(a, plain) +
@@ -460,8 +504,9 @@ constexpr int kComputeUnits = 256;
 // window, one with sinks by all that follow, which may be many times more: those are cut to a quarter
 // of the others' length, so that they fill what those leave. Others are cut where they are fewer than
 // one and a half to a compute unit, which two share (248 blocks of 128-wide bf16 heads, 2 x 4096
-// tokens: 235 us whole, 189 in halves and 27 to add those), or where without a window their lengths
-// range from all to nothing.
+// tokens: 235 us whole, 189 in halves and 27 to add those). Without a window their lengths range from
+// all to nothing, and they are cut where they are fewer than three to a compute unit (bf16, 1 x 4096
+// tokens, 12 heads of 64, 384 tiles: 119 us whole, 72 + 17 cut; 8 x 1024 tokens, 768: 40 whole, 45 + 31).
 struct Cuts {
     int tiles, far_tiles, near, far;
     int64_t heads, slots, pieces;  // blocks of all heads, and those of tiles that are cut
@@ -474,7 +519,7 @@ struct Cuts {
         far_tiles = limited ? static_cast<int>(std::min<int64_t>(ceil_div(t->sinks, keys_per_tile), tiles)) : 0;
         const int64_t plain = (tiles - far_tiles) * heads, turns = std::max<int64_t>(1, ceil_div(longest, turn) * group);
         const int64_t most = std::min<int64_t>(64, ceil_div(turns, 4));
-        const int64_t enough = limited ? kComputeUnits * 3 / 2 : 4 * kComputeUnits;
+        const int64_t enough = limited ? kComputeUnits * 3 / 2 : 3 * kComputeUnits;
         near = plain && plain < enough ? static_cast<int>(std::min(ceil_div(enough, plain), most)) : 1;
         const int64_t piece = std::max<int64_t>(4, turns / near / 4);
         // (where tiles with sinks are many, they fill the chip uncut, and their sums would fill its memory)
