@@ -87,7 +87,8 @@ __device__ __forceinline__ void attend(Running<D / 32>& r, acc16 (&s)[NK], const
 }
 
 // Where a row's sums go: its result, or with several blocks to a tile of rows their partial sums
-// [splits][rows of all heads][D + 2].
+// [splits][rows of all heads][D + 4]: the product, base, sum. A sum of 0 is that of a row that sees nothing; one
+// of NaN goes on to the result.
 template <typename T, int D>
 __device__ __forceinline__ void finish(Running<D / 32>& r, const AttnArgs& a, const RowAt& at, int b, int split,
                                        int lane) {
@@ -98,17 +99,17 @@ __device__ __forceinline__ void finish(Running<D / 32>& r, const AttnArgs& a, co
         float* p = a.partial + (split * rows + row / a.dim) * (D + 4);
         store_row<float, D / 32>(p, r.o, 1.0f, D, lane);
         if (lane < 32) {
-            p[D] = sum > 0.0f ? r.base : -INFINITY;
+            p[D] = sum == 0.0f ? -INFINITY : r.base;
             p[D + 1] = sum;
         }
         return;
     }
-    store_row<T, D / 32>(static_cast<T*>(a.result) + row, r.o, sum > 0.0f ? 1.0f / sum : 0.0f, a.dim, lane,
+    store_row<T, D / 32>(static_cast<T*>(a.result) + row, r.o, sum == 0.0f ? 0.0f : 1.0f / sum, a.dim, lane,
                          a.rest ? static_cast<T*>(a.rest) + row : nullptr);
     if (a.lse && lane < 32) {
         float* lse = a.lse + 2 * at.stat(a, b);
-        lse[0] = sum > 0.0f ? r.base : -INFINITY;
-        lse[1] = sum > 0.0f ? log2f(sum) : 0.0f;
+        lse[0] = sum == 0.0f ? -INFINITY : r.base;
+        lse[1] = sum == 0.0f ? 0.0f : log2f(sum);
     }
 }
 
@@ -232,7 +233,7 @@ __device__ __forceinline__ void put(float* to, const Running<DB>& r, int lane) {
     to[DB * 16 * kWave + kWave + lane] = r.sum;
 }
 
-// Joins the sums that another wave put.
+// Joins the sums that another wave put. Where neither has a maximum they are 0, or NaN if all scores were.
 template <int DB>
 __device__ __forceinline__ void join(Running<DB>& r, const float* from, int lane) {
     using F = vec<float, 4>;
@@ -240,8 +241,8 @@ __device__ __forceinline__ void join(Running<DB>& r, const float* from, int lane
     const float top = fmaxf(mine, other);
     const float keep = mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - top);
     const float take = other == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(other - top);
-    if (top == -INFINITY) return;
-    r.base = r.bound = top;
+    r.bound = top;
+    r.base = top == -INFINITY ? 0.0f : top;
     r.sum = r.sum * keep + from[DB * 16 * kWave + kWave + lane] * take;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -349,7 +350,7 @@ __global__ __launch_bounds__(kCombineWaves * kWave) void attention_combine_kerne
         for (int e = 0; e < E; ++e)
             if (e * 64 + lane < a.dim) o[e] = fmaf(p[s * step + e * 64 + lane], f, o[e]);
     }
-    const float factor = sum > 0.0f ? 1.0f / sum : 0.0f;
+    const float factor = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
     for (int e = 0; e < E; ++e)
         if (e * 64 + lane < a.dim) {
@@ -362,7 +363,7 @@ __global__ __launch_bounds__(kCombineWaves * kWave) void attention_combine_kerne
         const int64_t token = row / a.heads;
         float* lse = a.lse + 2 * ((token / a.queries * a.heads + row % a.heads) * a.queries + token % a.queries);
         lse[0] = top;
-        lse[1] = sum > 0.0f ? log2f(sum) : 0.0f;
+        lse[1] = sum == 0.0f ? 0.0f : log2f(sum);
     }
 }
 
