@@ -12,10 +12,13 @@
 #include <torch/csrc/utils/pybind.h>
 #include <torch/types.h>
 
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <array>
 #include <cmath>
+#include <functional>
 #include <optional>
 #include <sstream>
 #include <stdexcept>
@@ -91,9 +94,19 @@ bool tracked(std::initializer_list<const Tensor*> tensors) {
     return false;
 }
 
-void first_derivatives_only() {
+// A tangent that a tensor carries would be lost: whether or not it requires a gradient.
+template <typename Tensors>
+void no_tangents(const Tensors& tensors) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor& t : tensors)
+        if (t.defined() && t._fw_grad(/*level=*/0).defined())
+            refuse("the operators of isa.kernels.transformer_block have no forward-mode derivatives");
+}
+
+void first_derivatives_only(const variable_list& grads) {
     if (at::GradMode::is_enabled())
         refuse("the operators of isa.kernels.transformer_block have first derivatives only (create_graph is set)");
+    no_tangents(grads);
 }
 
 // t as [rows, dim] with adjacent elements in a row: a copy only where no view does it.
@@ -174,7 +187,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        first_derivatives_only();
+        first_derivatives_only(grads);
         const auto saved = ctx->get_saved_variables();
         const Tensor &h = saved[0], &stats = saved[2];
         const auto x_type = static_cast<at::ScalarType>(ctx->saved_data["x_type"].toInt());
@@ -208,6 +221,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 Tensor layer_norm(const Tensor& x, const Tensor& weight, const Maybe& bias, double eps) {
     const Tensor b = bias.value_or(Tensor());
     check_norm(nullptr, x, weight, b);
+    no_tangents(std::array{std::cref(x), std::cref(weight), std::cref(b)});
     if (tracked({&x, &weight, &b})) return LayerNorm::apply(x, weight, bias, Maybe(), eps)[0];
     return std::get<0>(norm_forward(nullptr, x, weight, b, eps, false));
 }
@@ -216,6 +230,7 @@ std::tuple<Tensor, Tensor> add_layer_norm(const Tensor& x, const Tensor& residua
                                           const Maybe& bias, double eps) {
     const Tensor b = bias.value_or(Tensor());
     check_norm(&x, residual, weight, b);
+    no_tangents(std::array{std::cref(x), std::cref(residual), std::cref(weight), std::cref(b)});
     if (tracked({&x, &residual, &weight, &b})) {
         const auto r = LayerNorm::apply(residual, weight, bias, Maybe(x), eps);
         return {r[0], r[1]};
@@ -303,7 +318,7 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        first_derivatives_only();
+        first_derivatives_only(grads);
         const auto s = ctx->get_saved_variables();
         const Tensor &q = s[0], &k = s[1], &v = s[2];
         const How how{ctx->saved_data["window"].toInt(), ctx->saved_data["sinks"].toInt(),
@@ -361,6 +376,7 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, std::
         if (type == at::kLong) lengths = lengths.clamp(0, kLongest).to(at::kInt);
         lengths = lengths.contiguous();
     }
+    no_tangents(std::array{std::cref(q), std::cref(k), std::cref(v)});
     if (tracked({&q, &k, &v}))
         return WindowAttention::apply(q, k, v, window.value_or(0), sinks, by, lengths.defined() ? Maybe(lengths) : Maybe());
     return std::get<0>(attention_forward(attention_operand(q), attention_operand(k), attention_operand(v),
@@ -436,7 +452,7 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        first_derivatives_only();
+        first_derivatives_only(grads);
         const auto s = ctx->get_saved_variables();
         const Tensor& rows = s[0];
         const c10::DeviceGuard guard(rows.device());
@@ -455,6 +471,7 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
 Tensor cross_entropy(const Tensor& logits, const Tensor& targets, int64_t ignore, const std::string& reduction_name) {
     const int reduction = reduction_of(reduction_name);
     check_loss(logits, targets);
+    no_tangents(std::array{std::cref(logits)});
     if (tracked({&logits})) return CrossEntropy::apply(logits, targets, ignore, static_cast<int64_t>(reduction));
     const Tensor out =
         std::get<0>(loss_forward(rows_of(logits), targets.reshape({-1}).contiguous(), ignore, reduction, false));
@@ -464,6 +481,7 @@ Tensor cross_entropy(const Tensor& logits, const Tensor& targets, int64_t ignore
 std::tuple<Tensor, Tensor> cross_entropy_with_grad(const Tensor& logits, const Tensor& targets, int64_t ignore,
                                                    double grad_scale) {
     check_loss(logits, targets);
+    no_tangents(std::array{std::cref(logits)});
     const at::NoGradGuard untracked;
     const Tensor rows = rows_of(logits.detach()), t = targets.reshape({-1}).contiguous();
     const c10::DeviceGuard guard(rows.device());

@@ -16,8 +16,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension (at most 16384
     elements), in x's type, with statistics in fp32.
 
-    x: float32, bfloat16 or float16; weight and bias: x's type or float32. First derivatives only, as
-    of all operators here."""
+    x: float32, bfloat16 or float16; weight and bias: x's type or float32. First derivatives only, and
+    by reverse mode: an input with a forward-mode tangent is refused. So it is with all operators here."""
     return _binding.layer_norm(x, weight, bias, eps)
 
 
