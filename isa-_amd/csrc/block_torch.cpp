@@ -9,11 +9,13 @@
 // Every call checks on the host what the kernels assume, allocates outputs and workspace with
 // torch's caching allocator and enqueues on the current stream of the tensors' device.
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/types.h>
 
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
 #include <array>
@@ -67,6 +69,14 @@ int type_of(const Tensor& t) {
     }
 }
 
+// A trace would hold the allocation of a result and not what fills it.
+void not_traced() {
+    using namespace c10::impl;
+    if (torch::jit::tracer::isTracing() || TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY) ||
+        TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE))
+        refuse("the operators of isa.kernels.transformer_block cannot be traced");
+}
+
 void require(const Tensor& t, const char* name) {
     if (!t.is_cuda()) refuse(name, " must be a CUDA tensor");
     if (type_of(t) < 0) refuse(name, " must be float32, bfloat16 or float16, got ", type_name(t));
@@ -107,6 +117,7 @@ void first_derivatives_only(const variable_list& grads) {
     if (at::GradMode::is_enabled())
         refuse("the operators of isa.kernels.transformer_block have first derivatives only (create_graph is set)");
     no_tangents(grads);
+    not_traced();
 }
 
 // t as [rows, dim] with adjacent elements in a row: a copy only where no view does it.
@@ -219,6 +230,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 };
 
 Tensor layer_norm(const Tensor& x, const Tensor& weight, const Maybe& bias, double eps) {
+    not_traced();
     const Tensor b = bias.value_or(Tensor());
     check_norm(nullptr, x, weight, b);
     no_tangents(std::array{std::cref(x), std::cref(weight), std::cref(b)});
@@ -228,6 +240,7 @@ Tensor layer_norm(const Tensor& x, const Tensor& weight, const Maybe& bias, doub
 
 std::tuple<Tensor, Tensor> add_layer_norm(const Tensor& x, const Tensor& residual, const Tensor& weight,
                                           const Maybe& bias, double eps) {
+    not_traced();
     const Tensor b = bias.value_or(Tensor());
     check_norm(&x, residual, weight, b);
     no_tangents(std::array{std::cref(x), std::cref(residual), std::cref(weight), std::cref(b)});
@@ -347,6 +360,7 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
 
 Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, std::optional<int64_t> window, int64_t sinks,
                         std::optional<double> scale, const Maybe& key_lengths) {
+    not_traced();
     require(q, "q");
     for (const auto& [t, name] : {std::pair<const Tensor&, const char*>{k, "k"}, {v, "v"}}) {
         require(t, name, q);
@@ -469,6 +483,7 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
 };
 
 Tensor cross_entropy(const Tensor& logits, const Tensor& targets, int64_t ignore, const std::string& reduction_name) {
+    not_traced();
     const int reduction = reduction_of(reduction_name);
     check_loss(logits, targets);
     no_tangents(std::array{std::cref(logits)});
@@ -480,6 +495,7 @@ Tensor cross_entropy(const Tensor& logits, const Tensor& targets, int64_t ignore
 
 std::tuple<Tensor, Tensor> cross_entropy_with_grad(const Tensor& logits, const Tensor& targets, int64_t ignore,
                                                    double grad_scale) {
+    not_traced();
     check_loss(logits, targets);
     no_tangents(std::array{std::cref(logits)});
     const at::NoGradGuard untracked;

@@ -17,7 +17,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     elements), in x's type, with statistics in fp32.
 
     x: float32, bfloat16 or float16; weight and bias: x's type or float32. First derivatives only, and
-    by reverse mode: an input with a forward-mode tangent is refused. So it is with all operators here."""
+    by reverse mode: an input with a forward-mode tangent is refused, and so are traces (torch.jit.trace, make_fx).
+    So it is with all operators here."""
     return _binding.layer_norm(x, weight, bias, eps)
 
 

@@ -1,5 +1,5 @@
 """What the block's operators do not give they refuse: forward-mode derivatives, whose tangent would be missing
-without a word."""
+without a word, and traces, which would hold an allocation and not what fills it."""
 
 from __future__ import annotations
 
@@ -54,3 +54,30 @@ def test_forward_mode_through_the_backward_is_refused(cuda_device):
             up = fwAD.make_dual(torch.ones_like(out), torch.ones_like(out))
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(out, leaves, up)
+
+
+@pytest.mark.parametrize("grad", [False, True], ids=["direct", "tracked"])
+def test_traces_are_refused(cuda_device, grad):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    for name, f, args in calls(cuda_device):
+        print(f"[case] trace of {name}", flush=True)
+        args = [a.requires_grad_(grad) for a in args]
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(f, tuple(args), check_trace=False)
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(f)(*args)
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(f, tracing_mode="fake")(*args)
+        assert torch.isfinite(f(*args)).all()
+
+
+def test_traces_of_the_backward_are_refused(cuda_device):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    for name, f, args in calls(cuda_device)[:4]:
+        print(f"[case] trace of {name}'s gradient", flush=True)
+        leaves = [a.requires_grad_(True) for a in args]
+        out = f(*leaves)
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(lambda g: torch.autograd.grad(out, leaves, g))(torch.ones_like(out))
