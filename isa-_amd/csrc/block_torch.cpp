@@ -120,8 +120,14 @@ void first_derivatives_only(const variable_list& grads) {
     not_traced();
 }
 
+// t's elements as they lie in memory: a view that stands for its negative (the imaginary part of a
+// conjugate) is written out, which contiguous() alone does not.
+Tensor plain(const Tensor& t) { return t.defined() ? t.resolve_neg() : t; }
+Tensor packed(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
+
 // t as [rows, dim] with adjacent elements in a row: a copy only where no view does it.
-Tensor rows_of(const Tensor& t) {
+Tensor rows_of(const Tensor& t_) {
+    const Tensor t = plain(t_);
     const int64_t dim = t.size(-1);
     Tensor r = t.dim() == 2 ? t : t.numel() ? t.reshape({-1, dim}) : t.reshape({t.numel() / dim, dim});
     return r.stride(1) == 1 || dim == 1 ? r : r.contiguous();
@@ -171,7 +177,7 @@ isa_block_norm norm_of(const Tensor& rows, int x_type, const Tensor& weight, con
 std::tuple<Tensor, Tensor, Tensor> norm_forward(const Tensor* x, const Tensor& residual, const Tensor& weight,
                                                 const Tensor& bias, double eps, bool with_stats) {
     const Tensor r = rows_of(residual), xs = x ? rows_of(*x) : Tensor();
-    const Tensor w = weight.contiguous(), b = bias.defined() ? bias.contiguous() : bias;
+    const Tensor w = packed(weight), b = packed(bias);
     const c10::DeviceGuard guard(r.device());
     const isa_block_norm n = norm_of(r, x ? type_of(*x) : type_of(r), w, b, eps);
     Tensor y = at::empty(residual.sizes(), residual.options()), h, stats;
@@ -202,10 +208,10 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         const auto saved = ctx->get_saved_variables();
         const Tensor &h = saved[0], &stats = saved[2];
         const auto x_type = static_cast<at::ScalarType>(ctx->saved_data["x_type"].toInt());
-        const Tensor rows = rows_of(h), weight = saved[1].contiguous();
+        const Tensor rows = rows_of(h), weight = packed(saved[1]);
         const c10::DeviceGuard guard(h.device());
-        const Tensor dy = grads[0].defined() ? grads[0].contiguous() : at::zeros(h.sizes(), h.options());
-        const Tensor dh = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : Tensor();
+        const Tensor dy = grads[0].defined() ? packed(grads[0]) : at::zeros(h.sizes(), h.options());
+        const Tensor dh = grads.size() > 1 ? packed(grads[1]) : Tensor();
         const bool separate = x_type != h.scalar_type();
         Tensor dr = at::empty(h.sizes(), h.options()), dx, dw, db, workspace;
         if (separate) dx = at::empty(h.sizes(), h.options().dtype(x_type));
@@ -263,7 +269,8 @@ void strides_of(const Tensor& t, int64_t (&s)[3]) {
 
 // t, or a copy where its heads' elements are apart, 16-byte loads would not be aligned or tokens
 // overlap (as broadcast ones do) or lie too far apart.
-Tensor attention_operand(const Tensor& t) {
+Tensor attention_operand(const Tensor& t_) {
+    const Tensor t = plain(t_);
     if (t.numel() == 0) return t;
     int64_t s[3];
     strides_of(t, s);
@@ -388,7 +395,7 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, std::
             refuse("key_lengths must be int32 or int64 [", q.size(0), "], got ", type_name(lengths), " ", lengths.sizes());
         if (lengths.device() != q.device()) refuse("key_lengths must be on ", q.device(), ", got ", lengths.device());
         if (type == at::kLong) lengths = lengths.clamp(0, kLongest).to(at::kInt);
-        lengths = lengths.contiguous();
+        lengths = packed(lengths);
     }
     no_tangents(std::array{std::cref(q), std::cref(k), std::cref(v)});
     if (tracked({&q, &k, &v}))
@@ -456,7 +463,7 @@ std::tuple<Tensor, Tensor, Tensor> loss_forward(const Tensor& rows, const Tensor
 struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
     static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& targets, int64_t ignore,
                           int64_t reduction) {
-        const Tensor rows = rows_of(logits), t = targets.reshape({-1}).contiguous();
+        const Tensor rows = rows_of(logits), t = packed(targets.reshape({-1}));
         auto [out, stats, count] = loss_forward(rows, t, ignore, static_cast<int>(reduction), true);
         ctx->save_for_backward({rows, t, stats, count});
         ctx->saved_data["ignore"] = ignore;
@@ -471,7 +478,7 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
         const Tensor& rows = s[0];
         const c10::DeviceGuard guard(rows.device());
         const isa_block_loss l = loss_of(rows, s[1], ctx->saved_data["ignore"].toInt());
-        const Tensor grad = like_rows(rows), up = grads[0].to(at::kFloat).contiguous();
+        const Tensor grad = like_rows(rows), up = packed(grads[0].to(at::kFloat));
         check(isa_block_loss_backward(&l, static_cast<int>(ctx->saved_data["reduction"].toInt()),
                                       static_cast<const float*>(s[2].data_ptr()),
                                       static_cast<const float*>(s[3].data_ptr()),
@@ -489,7 +496,7 @@ Tensor cross_entropy(const Tensor& logits, const Tensor& targets, int64_t ignore
     no_tangents(std::array{std::cref(logits)});
     if (tracked({&logits})) return CrossEntropy::apply(logits, targets, ignore, static_cast<int64_t>(reduction));
     const Tensor out =
-        std::get<0>(loss_forward(rows_of(logits), targets.reshape({-1}).contiguous(), ignore, reduction, false));
+        std::get<0>(loss_forward(rows_of(logits), packed(targets.reshape({-1})), ignore, reduction, false));
     return reduction == ISA_BLOCK_NONE ? shaped(out, targets.sizes()) : out;
 }
 
@@ -499,7 +506,7 @@ std::tuple<Tensor, Tensor> cross_entropy_with_grad(const Tensor& logits, const T
     check_loss(logits, targets);
     no_tangents(std::array{std::cref(logits)});
     const at::NoGradGuard untracked;
-    const Tensor rows = rows_of(logits.detach()), t = targets.reshape({-1}).contiguous();
+    const Tensor rows = rows_of(logits.detach()), t = packed(targets.reshape({-1}));
     const c10::DeviceGuard guard(rows.device());
     const isa_block_loss l = loss_of(rows, t, ignore);
     const Tensor out = at::empty({}, rows.options().dtype(at::kFloat)), grad = like_rows(rows);
