@@ -29,25 +29,47 @@ class LayerNorm(nn.LayerNorm):
 
 
 class WindowCache:
-    """The keys and values of a batch's sequences, each of its own length (on the device)."""
+    """The keys and values of a batch's sequences, each of its own length (on the device).
+
+    A caller may set `lengths` (a padded prompt's true ones, or zeros to start anew)."""
 
     def __init__(self, batch: int, capacity: int, kv_heads: int, head_dim: int, *, dtype=torch.float32, device="cuda"):
         shape = (batch, capacity, kv_heads, head_dim)
         self.k = torch.zeros(shape, dtype=dtype, device=device)
         self.v = torch.zeros(shape, dtype=dtype, device=device)
-        self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):  # its changes are counted (see longest)
+            self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self._rows = torch.arange(batch, device=device)[:, None]
+        self._recorded = False  # by a HIP graph, whose replays are not counted
+        self._keep(0)
+
+    def _keep(self, longest: int) -> None:
+        known = not (self._recorded or self.lengths.is_inference())
+        self._longest, self._known = longest, (self.lengths, self.lengths._version if known else None)
+
+    def longest(self) -> Optional[int]:
+        """The longest sequence's length; None while a HIP graph is recorded. Kept on the host: the device is
+        asked only after a caller set `lengths`, and after a graph recorded an append."""
+        if self.lengths.is_cuda and torch.cuda.is_current_stream_capturing():
+            self._recorded = True
+            return None
+        tensor, version = self._known
+        if self._recorded or tensor is not self.lengths or version is None or version != self.lengths._version:
+            self._keep(int(self.lengths.max()) if self.lengths.numel() else 0)
+        return self._longest
 
     @torch.no_grad()
     def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
-        """Adds tokens [batch, n, kv_heads, head_dim] behind each sequence's end; the caller keeps
-        sequences within the capacity."""
-        if k.shape[1] > self.k.shape[1]:
-            raise RuntimeError(f"{k.shape[1]} tokens do not fit a cache of {self.k.shape[1]}")
-        at = self.lengths.long()[:, None] + torch.arange(k.shape[1], device=k.device)
+        """Adds tokens [batch, n, kv_heads, head_dim] behind each sequence's end, if all fit. (Where a
+        HIP graph replays appends, the caller keeps them within the capacity.)"""
+        n, used, capacity = k.shape[1], self.longest() or 0, self.k.shape[1]
+        if used + n > capacity:
+            raise RuntimeError(f"{n} tokens do not fit a cache of {capacity} that holds {used}")
+        at = self.lengths.long()[:, None] + torch.arange(n, device=k.device)
         self.k[self._rows, at] = k.to(self.k.dtype)
         self.v[self._rows, at] = v.to(self.v.dtype)
-        self.lengths += k.shape[1]
+        self.lengths += n
+        self._keep(used + n)
 
 
 class WindowAttention(nn.Module):
