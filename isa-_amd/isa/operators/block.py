@@ -60,8 +60,8 @@ class WindowCache:
 
     @torch.no_grad()
     def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
-        """Adds tokens [batch, n, kv_heads, head_dim] behind each sequence's end, if all fit. (Where a
-        HIP graph replays appends, the caller keeps them within the capacity.)"""
+        """Adds tokens [batch, n, kv_heads, head_dim] behind each sequence's end, if all fit, without their
+        gradients. (Where a HIP graph replays appends, the caller keeps them within the capacity.)"""
         n, used, capacity = k.shape[1], self.longest() or 0, self.k.shape[1]
         if used + n > capacity:
             raise RuntimeError(f"{n} tokens do not fit a cache of {capacity} that holds {used}")
@@ -70,6 +70,19 @@ class WindowCache:
         self.v[self._rows, at] = v.to(self.v.dtype)
         self.lengths += n
         self._keep(used + n)
+
+
+class _OverACache(torch.autograd.Function):
+    """Attention's output over a cache. A cache holds values alone: a backward pass would leave out what reaches
+    a token's key and value through it, so there is none."""
+
+    @staticmethod
+    def forward(ctx, out, k, v):
+        return out.view_as(out)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("attention over a WindowCache has no gradients: train without a cache")
 
 
 class WindowAttention(nn.Module):
@@ -96,6 +109,8 @@ class WindowAttention(nn.Module):
             cache.append(k, v)
             a = window_attention(q.to(cache.k.dtype), cache.k, cache.v, window=self.window, sinks=self.sinks,
                                  key_lengths=cache.lengths)
+            if torch.is_grad_enabled():
+                a = _OverACache.apply(a, k, v)
         return self.proj(a.reshape(b, n, -1).to(x.dtype))
 
 
