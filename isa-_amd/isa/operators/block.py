@@ -143,6 +143,9 @@ class GPT(nn.Module):
 
     def forward(self, ids: torch.Tensor, caches: Optional[list] = None) -> torch.Tensor:
         """Logits [batch, n, vocab]; with caches (one a block) ids continue their sequences."""
+        used, positions = caches[0].longest() or 0 if caches else 0, self.positions.num_embeddings
+        if used + ids.shape[1] > positions:
+            raise RuntimeError(f"{ids.shape[1]} tokens after {used} do not fit the table of {positions} positions")
         at = torch.arange(ids.shape[1], device=ids.device)
         if caches is not None:
             at = caches[0].lengths.long()[:, None] + at

@@ -70,3 +70,16 @@ def test_inference_mode(made_inside):
         with pytest.raises(RuntimeError, match="do not fit"):
             c.append(*tokens(1))
         assert c.lengths.tolist() == [8, 8]
+
+
+def test_sequences_end_with_the_table_of_positions():
+    """(blocks that would need a GPU are left out: the refusal comes before them)"""
+    model = GPT(20, 6, 16, torch.nn.ModuleList())
+    with pytest.raises(RuntimeError, match="table of 6 positions"):
+        model(torch.zeros(2, 7, dtype=torch.int64))
+    c = cache()
+    c.append(*tokens(5))
+    with pytest.raises(RuntimeError, match="table of 6 positions"):
+        model(torch.zeros(2, 2, dtype=torch.int64), [c])
+    with pytest.raises(RuntimeError, match="CUDA"):  # one more fits, and gets to the last norm
+        model(torch.zeros(2, 1, dtype=torch.int64), [c])
