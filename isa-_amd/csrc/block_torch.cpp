@@ -434,10 +434,13 @@ isa_block_loss loss_of(const Tensor& rows, const Tensor& targets, int64_t ignore
     return l;
 }
 
-// A new tensor as t [rows, vocab], its rows as far apart (so both are aligned alike).
+// A new tensor as t [rows, vocab]. Where that adds an eighth at most, rows of both are aligned alike: as far
+// apart (a padded vocabulary, whose rows then stay on whole cache lines), or by the same remainder of 16 bytes.
 Tensor like_rows(const Tensor& t) {
-    if (t.size(0) < 2 || t.stride(0) <= t.size(1)) return at::empty(t.sizes(), t.options());
-    return at::empty_strided(t.sizes(), {t.stride(0), 1}, t.options());
+    const int64_t vocab = t.size(1), apart = t.stride(0);
+    if (t.size(0) < 2 || apart <= vocab) return at::empty(t.sizes(), t.options());
+    const int64_t extra = apart - vocab, odd = extra % (16 / t.element_size()), most = vocab / 8;
+    return at::empty_strided(t.sizes(), {vocab + (extra <= most ? extra : odd <= most ? odd : 0), 1}, t.options());
 }
 
 Tensor shaped(const Tensor& rows, at::IntArrayRef sizes) { return rows.sizes() == sizes ? rows : rows.reshape(sizes); }

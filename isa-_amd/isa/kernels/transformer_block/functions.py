@@ -61,7 +61,11 @@ def cross_entropy(logits: torch.Tensor, targets: torch.Tensor, *, ignore_index: 
 
     logits: [..., vocab], float32, bfloat16 or float16; targets: int64 [...]. Rows whose target is
     ignore_index count nowhere; reduction is "mean" (over the others), "sum" or "none". Any other
-    target outside the vocabulary makes its row's loss and gradients NaN."""
+    target outside the vocabulary makes its row's loss and gradients NaN.
+
+    Rows may lie apart (a padded vocabulary, a sequence's last tokens). Leading dimensions that no single
+    stride spans are copied first: instead of logits[:, :-1] of several sequences, take all of the logits and
+    targets whose last column is ignore_index."""
     return _binding.cross_entropy(logits, targets, ignore_index, reduction)
 
 
