@@ -111,6 +111,16 @@ __device__ __forceinline__ float share_of(const LossArgs& a, int64_t r) {
     return share;
 }
 
+// The row that a block takes, in a grid of two dimensions: one may hold less than 2^32 threads, which a block a row
+// passes at 2^22 rows of 1024.
+__device__ __forceinline__ int64_t block_row() { return static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x; }
+
+dim3 grid_of(int64_t rows) {
+    constexpr int64_t kWide = int64_t{1} << 21;
+    const int64_t wide = std::min(rows, kWide);
+    return dim3(static_cast<unsigned>(wide), static_cast<unsigned>(ceil_div(rows, wide)));
+}
+
 // C > 0: a thread holds C chunks of the row. C == 0: the row is read once for the statistics,
 // with a running maximum, and once more for the gradient.
 template <typename T, int C, int THREADS>
@@ -118,7 +128,8 @@ __global__ __launch_bounds__(THREADS) void loss_kernel(LossArgs a) {
     using R = Row<T>;
     constexpr int N = R::N;
     __shared__ float slots[2][THREADS / kWave];
-    const int64_t r = blockIdx.x;
+    const int64_t r = block_row();
+    if (r >= a.rows) return;  // (a whole block)
     const R row(static_cast<const T*>(a.logits) + r * a.stride, a.vocab);
     const int chunks = row.chunks();
     const int64_t target = a.targets[r];
@@ -205,7 +216,8 @@ template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void loss_backward_kernel(LossArgs a) {
     using R = Row<T>;
     constexpr int N = R::N;
-    const int64_t r = blockIdx.x;
+    const int64_t r = block_row();
+    if (r >= a.rows) return;  // (a whole block)
     const R row(static_cast<const T*>(a.logits) + r * a.stride, a.vocab);
     const int chunks = row.chunks();
     const int64_t target = a.targets[r];
@@ -246,7 +258,7 @@ __global__ __launch_bounds__(kMostThreads) void loss_sum_kernel(const float* row
 
 template <typename T, int C, int THREADS>
 void launch(const LossArgs& a, hipStream_t s) {
-    loss_kernel<T, C, THREADS><<<dim3(static_cast<unsigned>(a.rows)), dim3(THREADS), 0, s>>>(a);
+    loss_kernel<T, C, THREADS><<<grid_of(a.rows), dim3(THREADS), 0, s>>>(a);
 }
 
 // Chunks of the longest row, one more where rows start inside a chunk.
@@ -276,7 +288,7 @@ void launch_rows(const LossArgs& a, hipStream_t s) {
 
 template <typename T>
 void launch_backward(const LossArgs& a, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>(a.rows));
+    const dim3 grid = grid_of(a.rows);
     if (chunks_of<T>(a) <= 1024)
         loss_backward_kernel<T, 256><<<grid, 256, 0, s>>>(a);
     else
