@@ -271,7 +271,7 @@ void strides_of(const Tensor& t, int64_t (&s)[3]) {
 // overlap (as broadcast ones do) or lie too far apart.
 Tensor attention_operand(const Tensor& t_) {
     const Tensor t = plain(t_);
-    if (t.numel() == 0) return t;
+    if (t.numel() == 0) return at::empty(t.sizes(), t.options());  // whatever its strides
     int64_t s[3];
     strides_of(t, s);
     const bool tokens = t.size(1) < 2 || (s[1] >= t.size(3) && s[1] * t.element_size() < kFar);
