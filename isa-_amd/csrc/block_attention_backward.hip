@@ -223,14 +223,14 @@ __global__ __launch_bounds__(kThreads<T>, (kDqWaves<T, D>)) void attention_dq_ke
 }
 
 // ---- dk and dv ------------------------------------------------------------------------------
-// A block takes kKeys keys of a key head, a wave 32 KB of them, and walks the tiles of BR queries of
+// A block takes kKeys keys of a key head, a wave 32 of them, and walks the tiles of BR queries of
 // each head that see one of the keys. The blocks of one tile of keys, if several, take equal parts
 // of that walk and leave partial sums.
 
 template <typename T, int D>
 struct DkvShape {
-    static constexpr int kWaveCount = sizeof(T) == 4 ? 1 : 4, KB = 1;
-    static constexpr int kKeys = kWaveCount * 32 * KB, kThreadCount = kWaveCount * kWave;
+    static constexpr int kWaveCount = sizeof(T) == 4 ? 1 : 4;
+    static constexpr int kKeys = kWaveCount * 32, kThreadCount = kWaveCount * kWave;
     // 16-bit rows of 128: V waits in LDS instead of in registers, and tiles of 32 queries leave room for
     // it, so that two blocks still share a compute unit
     static constexpr bool kHoldV = !(sizeof(T) == 2 && D == 128);
@@ -258,7 +258,7 @@ template <typename T, int D>
 __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) void attention_dkv_kernel(AttnArgs a) {
     using L = Tile<T, D>;
     using S = DkvShape<T, D>;
-    constexpr int BR = S::BR, DB = D / 32, KB = S::KB;
+    constexpr int BR = S::BR, DB = D / 32;
     constexpr int kSecond = kOneTile<T> ? 1 : BR * L::kPitch;
     __shared__ __attribute__((aligned(1024))) T q0[BR * L::kPitch], g0[BR * L::kPitch], q1[kSecond], g1[kSecond];
     __shared__ __attribute__((aligned(1024))) float stat0[kPlanes * 64], stat1[kOneTile<T> ? 1 : kPlanes * 64];
@@ -273,23 +273,19 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
     const int tile = (far ? 0 : a.far_tiles) + in / splits, split = in % splits;
     const int j0 = tile * S::kKeys, length = length_of(a, b), shift = length - a.queries;
 
-    const int mine = j0 + wave * 32 * KB;
+    const int mine = j0 + wave * 32;
     __shared__ __attribute__((aligned(1024))) T held[S::kHoldV ? 1 : S::kKeys * L::kPitch];
     if constexpr (!S::kHoldV) {
         const Loader<T, D, S::kKeys, S::kThreadCount> vload(
             static_cast<const T*>(a.v) + b * a.vs[0] + kv_head * a.vs[2], a.vs[1], a.dim, threadIdx.x);
         vload.load(held, 0, j0, length, wave);
     }
-    RowFrags<T, D> k[KB], v[KB];
-#pragma unroll
-    for (int n = 0; n < KB; ++n) {
-        const int64_t key = mine + 32 * n + lane % 32;
-        k[n].load(key < length ? static_cast<const T*>(a.k) + b * a.ks[0] + kv_head * a.ks[2] + key * a.ks[1] : nullptr,
-                  a.dim, lane);
-        if constexpr (!S::kHoldV) continue;
-        v[n].load(key < length ? static_cast<const T*>(a.v) + b * a.vs[0] + kv_head * a.vs[2] + key * a.vs[1] : nullptr,
-                  a.dim, lane);
-    }
+    RowFrags<T, D> k, v;
+    const int key = mine + lane % 32;
+    k.load(key < length ? static_cast<const T*>(a.k) + b * a.ks[0] + kv_head * a.ks[2] + key * a.ks[1] : nullptr, a.dim, lane);
+    if constexpr (S::kHoldV)
+        v.load(key < length ? static_cast<const T*>(a.v) + b * a.vs[0] + kv_head * a.vs[2] + key * a.vs[1] : nullptr, a.dim,
+               lane);
     float factor = 1.0f;
     if constexpr (kScaled<T>) {
         const int64_t count = peaks_of(a, kTile);
@@ -303,7 +299,7 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
     const int begin = static_cast<int>(static_cast<int64_t>(all_turns) * split / splits);
     const int end = static_cast<int>(static_cast<int64_t>(all_turns) * (split + 1) / splits);
 
-    acc16 dk[KB][DB] = {}, dv[KB][DB] = {};
+    acc16 dk[DB] = {}, dv[DB] = {};
     const int64_t plane = plane_rows(a);
     const Loader<T, D, BR, S::kThreadCount> qload(
         static_cast<const T*>(a.q) + b * a.qs[0] + static_cast<int64_t>(kv_head) * a.group * a.qs[2], a.qs[1], a.dim,
@@ -327,19 +323,18 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
         gload.load_from(gt, 0, gload.base + from, seen.end - i0, wave);
     };
     // s = p and d = ds of 32 queries and 32 keys; false where none of them sees any
-    auto gradients = [&](int it, int r, int n, const T* qt, const T* gt, const float* stat, acc16& s, acc16& d, int lane) {
+    auto gradients = [&](int it, int r, const T* qt, const T* gt, const float* stat, acc16& s, acc16& d, int lane) {
         const int half = lane / 32, i0 = seen.first + it % turns * BR;
         const int pmin = shift + i0, pmax = shift + min(i0 + BR, seen.end) - 1;
-        const int first = mine + 32 * n, key = first + lane % 32;
-        const int plo = pmin + 32 * r, phi = min(plo + 31, pmax);
-        if (first > phi || (first + 31 <= plo - a.window && first >= a.sinks)) return false;
-        const bool all = first + 31 <= plo && (first + 32 <= a.sinks || first > phi - a.window);
+        const int key = mine + lane % 32, plo = pmin + 32 * r, phi = min(plo + 31, pmax);
+        if (mine > phi || (mine + 31 <= plo - a.window && mine >= a.sinks)) return false;
+        const bool all = mine + 31 <= plo && (mine + 32 <= a.sinks || mine > phi - a.window);
         s = acc16{};
         d = acc16{};
 #pragma unroll
         for (int t = 0; t < L::kSteps; ++t) {
-            mma(s, L::row(qt, 32 * r, t, lane), k[n][t]);
-            mma(d, L::row(gt, 32 * r, t, lane), S::kHoldV ? v[n][t] : L::row(held, wave * 32 * KB + 32 * n, t, lane));
+            mma(s, L::row(qt, 32 * r, t, lane), k[t]);
+            mma(d, L::row(gt, 32 * r, t, lane), S::kHoldV ? v[t] : L::row(held, wave * 32, t, lane));
         }
         reads_ahead<(S::kHoldV ? 2 : 3) * L::kSteps, 2 * L::kSteps * L::kMmas, 4>();
 #pragma unroll
@@ -371,7 +366,7 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
         return true;
     };
     if constexpr (kOneTile<T>) {  // Q's tile is free after dk, dO's after dv
-        static_assert(BR == kTile && KB == 1);
+        static_assert(BR == kTile);
         auto add = [&](acc16(&sum)[DB], const T* tile, const acc16& x, int lane) {
 #pragma unroll
             for (int u = 0; u < L::kUses; ++u) {
@@ -390,11 +385,11 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
             __syncthreads();
             const int lane = opaque(outer);
             acc16 s, d;
-            const bool any = gradients(it, 0, 0, q0, g0, stat0, s, d, lane);
-            if (any) add(dk[0], q0, d, lane);
+            const bool any = gradients(it, 0, q0, g0, stat0, s, d, lane);
+            if (any) add(dk, q0, d, lane);
             __syncthreads();
             if (it + 1 < end) fetch_q(it + 1, q0, stat0);
-            if (any) add(dv[0], g0, s, lane);
+            if (any) add(dv, g0, s, lane);
             __syncthreads();
             if (it + 1 < end) fetch_g(it + 1, g0);
         }
@@ -406,22 +401,20 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
         auto compute = [&](int it, const T* qt, const T* gt, const float* stat) {
             const int lane = opaque(outer);
 #pragma unroll
-            for (int r = 0; r < BR / 32; ++r)
+            for (int r = 0; r < BR / 32; ++r) {
+                acc16 s, d;
+                if (!gradients(it, r, qt, gt, stat, s, d, lane)) continue;
 #pragma unroll
-                for (int n = 0; n < KB; ++n) {
-                    acc16 s, d;
-                    if (!gradients(it, r, n, qt, gt, stat, s, d, lane)) continue;
+                for (int u = 0; u < L::kUses; ++u) {
+                    const typename Frag<T>::V f = operand<T>(s, u), h = operand<T>(d, u);
 #pragma unroll
-                    for (int u = 0; u < L::kUses; ++u) {
-                        const typename Frag<T>::V f = operand<T>(s, u), h = operand<T>(d, u);
-#pragma unroll
-                        for (int db = 0; db < DB; ++db) {
-                            mma(dv[n][db], L::column(gt, 32 * r, u, db, lane), f);
-                            mma(dk[n][db], L::column(qt, 32 * r, u, db, lane), h);
-                        }
+                    for (int db = 0; db < DB; ++db) {
+                        mma(dv[db], L::column(gt, 32 * r, u, db, lane), f);
+                        mma(dk[db], L::column(qt, 32 * r, u, db, lane), h);
                     }
-                    reads_ahead<2 * L::kUses * DB * L::kColumnReads, 2 * L::kUses * DB * L::kMmas, 4 * L::kColumnReads>();
                 }
+                reads_ahead<2 * L::kUses * DB * L::kColumnReads, 2 * L::kUses * DB * L::kMmas, 4 * L::kColumnReads>();
+            }
         };
         if (begin < end) fetch(begin, q0, g0, stat0);
         for (int it = begin; it < end; it += 2) {
@@ -436,33 +429,25 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
             compute(it + 1, q1, g1, stat1);
         }
     }
-    if (splits > 1) {  // [piece of a cut tile][dk, dv][key block, dims' quarter][thread]
+    if (splits > 1) {  // [piece of a cut tile][dk, dv][dims' quarter of 32][thread]
         const int64_t mine_at = (static_cast<int64_t>(b) * a.kv_heads + kv_head) * pieces_per_head(a, plain) +
                                 (far && a.near > 1 ? plain * a.near : 0) + in;
         float* p = a.partial + mine_at * (2 * S::kKeys * D) + threadIdx.x * 4;
 #pragma unroll
-        for (int n = 0; n < KB; ++n)
+        for (int db = 0; db < DB; ++db)
 #pragma unroll
-            for (int db = 0; db < DB; ++db)
-#pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const int at = ((n * DB + db) * 4 + i / 4) * S::kThreadCount * 4;
-                    using F = vec<float, 4>;
-                    *reinterpret_cast<F*>(p + at) =
-                        F{dk[n][db][i], dk[n][db][i + 1], dk[n][db][i + 2], dk[n][db][i + 3]} * (1.0f / factor);
-                    *reinterpret_cast<F*>(p + S::kKeys * D + at) =
-                        F{dv[n][db][i], dv[n][db][i + 1], dv[n][db][i + 2], dv[n][db][i + 3]};
-                }
+            for (int i = 0; i < 16; i += 4) {
+                const int at = (db * 4 + i / 4) * S::kThreadCount * 4;
+                using F = vec<float, 4>;
+                *reinterpret_cast<F*>(p + at) = F{dk[db][i], dk[db][i + 1], dk[db][i + 2], dk[db][i + 3]} * (1.0f / factor);
+                *reinterpret_cast<F*>(p + S::kKeys * D + at) = F{dv[db][i], dv[db][i + 1], dv[db][i + 2], dv[db][i + 3]};
+            }
         return;
     }
-#pragma unroll
-    for (int n = 0; n < KB; ++n) {
-        const int key = mine + 32 * n + lane % 32;
-        if (key >= a.keys) continue;
-        const int64_t out = ((static_cast<int64_t>(b) * a.keys + key) * a.kv_heads + kv_head) * a.dim;
-        store_row<T, DB>(static_cast<T*>(a.dk) + out, dk[n], a.scale / factor, a.dim, lane);
-        store_row<T, DB>(static_cast<T*>(a.dv) + out, dv[n], 1.0f, a.dim, lane);
-    }
+    if (key >= a.keys) return;
+    const int64_t out = ((static_cast<int64_t>(b) * a.keys + key) * a.kv_heads + kv_head) * a.dim;
+    store_row<T, DB>(static_cast<T*>(a.dk) + out, dk, a.scale / factor, a.dim, lane);
+    store_row<T, DB>(static_cast<T*>(a.dv) + out, dv, 1.0f, a.dim, lane);
 }
 
 // The partial sums of a tile's blocks, added in their order: a block takes 4 dims of each key.
@@ -470,7 +455,7 @@ template <typename T, int D>
 __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount)) void attention_dkv_sum_kernel(AttnArgs a) {
     using S = DkvShape<T, D>;
     using F = vec<float, 4>;
-    constexpr int kQuads = S::KB * (D / 32) * 4;
+    constexpr int kQuads = D / 8;
     const int tiles = (a.keys + S::kKeys - 1) / S::kKeys, plain = tiles - a.far_tiles;
     const int quad = blockIdx.x % kQuads, which = blockIdx.x / kQuads % 2, task = blockIdx.x / kQuads / 2;
     const int summed = (a.near > 1 ? plain : 0) + (a.far > 1 ? a.far_tiles : 0);
@@ -486,8 +471,7 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount)) void attention_dkv_
 #pragma unroll 8
     for (int s = 0; s < splits; ++s) x += p[static_cast<int64_t>(s) * (S::kKeys * D / 2)];
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const int n = quad / (D / 8), dims = quad % (D / 8) * 8 + lane / 32 * 4;
-    const int key = tile * S::kKeys + wave * 32 * S::KB + 32 * n + lane % 32;
+    const int dims = quad * 8 + lane / 32 * 4, key = tile * S::kKeys + wave * 32 + lane % 32;
     if (key >= a.keys || dims >= a.dim) return;
     const int64_t out = ((static_cast<int64_t>(head / a.kv_heads) * a.keys + key) * a.kv_heads + head % a.kv_heads) * a.dim;
     Pack<T, 4> y;
@@ -561,7 +545,7 @@ void launch(AttnArgs a, const isa_block_attention* t, hipStream_t s) {
     attention_dkv_kernel<T, D><<<dim3(static_cast<unsigned>(cuts.slots)), S::kThreadCount, 0, s>>>(a);
     if (cuts.summed())
         attention_dkv_sum_kernel<T, D>
-            <<<dim3(static_cast<unsigned>(cuts.summed() * 2 * S::KB * (D / 8))), S::kThreadCount, 0, s>>>(a);
+            <<<dim3(static_cast<unsigned>(cuts.summed() * 2 * (D / 8))), S::kThreadCount, 0, s>>>(a);
 }
 
 template <typename F>
