@@ -18,7 +18,7 @@ using acc16 = vec<float, 16>;
 struct AttnArgs {
     const void *q, *k, *v, *out, *dout;
     void *result, *rest, *dk, *dv;  // result: out, or dq
-    float *lse, *delta, *partial, *peaks;
+    float *lse, *delta, *partial;
     const int32_t* lengths;
     int64_t qs[3], ks[3], vs[3], gs[3];
     int batch, queries, keys, heads, kv_heads, group, dim, window, sinks;

@@ -74,20 +74,37 @@ __device__ __forceinline__ float dot(const RowFrags<T, D>& x, const RowFrags<T, 
     return sum;
 }
 
-// fp16 has 5 bits of exponent: gradients of a mean loss, some 1e-5, would leave ds a few bits. There ds is
-// taken of do scaled by a power of two to between 1 and 2 at its peak: a row's own for dq, that of all
-// rows of a key head for dk, which dq's waves leave behind.
+// fp16 has 5 bits of exponent: gradients of a mean loss, some 1e-5, would leave ds a few bits, and values of some
+// 1000 could take it past the range. A lane's ds belong to one row (dq) or one key (dk), and so do its sums of
+// them times the other operand: both are held times a power of two that brings the largest ds so far
+// to between 1 and kMostDs, so that rows' and keys' sizes do not meet. (2 x 4096 tokens, 16 heads on 4 of 128,
+// window 1024: dq 128 us, dk and dv 165, as bf16 without a scale takes.)
 template <typename T>
 constexpr bool kScaled = std::is_same_v<T, f16>;
+constexpr float kFirstFactor = 0x1p126f;  // of a lane that has seen no ds (past 2^-113)
+constexpr float kMostDs = 0x1p13f;
 
 __device__ __forceinline__ float to_one(float peak) {
     const int e = static_cast<int>(__float_as_uint(peak) >> 23);  // (peak is not negative)
     return e < 1 || e > 253 ? 1.0f : __uint_as_float(static_cast<unsigned>(254 - e) << 23);
 }
 
-// A wave's peaks of a key head: [tile of rows][wave].
-__device__ __forceinline__ int64_t peaks_of(const AttnArgs& a, int64_t rows_per_wave) {
-    return (static_cast<int64_t>(a.queries) * a.group + rows_per_wave - 1) / rows_per_wave;
+template <int DB>
+__device__ __forceinline__ void scale_to_one(acc16& ds, float& factor, acc16 (&sums)[DB]) {
+    float peak = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) peak = fmaxf(peak, fabsf(ds[i]));
+    peak = half_max(peak);
+    if (__any(peak * factor > kMostDs)) {
+        const float next = peak * factor > kMostDs ? to_one(peak) : factor, change = next / factor;
+        factor = next;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sums[db][i] *= change;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) ds[i] *= factor;
 }
 
 template <typename T>
@@ -141,21 +158,7 @@ __global__ __launch_bounds__(kThreads<T>, (kDqWaves<T, D>)) void attention_dq_ke
     const float base = a.lse[2 * stat], log_sum = a.lse[2 * stat + 1];
     const float lse = sizeof(T) == 4 ? base : base + log_sum, lse_rest = log_sum;
     if (row <= last && lane < 32) put_planes<T>(a, stat, delta, base, log_sum);
-    float factor = 1.0f;
-    if constexpr (kScaled<T>) {
-        float peak = 0.0f;
-#pragma unroll
-        for (int t = 0; t < L::kSteps; ++t)
-#pragma unroll
-            for (int e = 0; e < L::N; ++e) peak = fmaxf(peak, fabsf(static_cast<float>(g[t][e])));
-        peak = half_max(peak);
-        factor = to_one(peak);
-        peak = wave_max(peak);
-        if (mine <= last && lane == 0)
-            a.peaks[(static_cast<int64_t>(b) * a.kv_heads + kv_head) * peaks_of(a, kTile) + mine / kTile] = peak;
-        if (!a.result) return;
-    }
-
+    float factor = kScaled<T> ? kFirstFactor : 1.0f;
     acc16 dq[DB] = {};
     const Loader<T, D, BN, kThreads<T>> kload(static_cast<const T*>(a.k) + b * a.ks[0] + kv_head * a.ks[2], a.ks[1], a.dim,
                                            threadIdx.x);
@@ -180,15 +183,13 @@ __global__ __launch_bounds__(kThreads<T>, (kDqWaves<T, D>)) void attention_dq_ke
             }
             reads_ahead<2 * L::kSteps, 2 * L::kSteps * L::kMmas, 4>();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[i] = probability<T>(s[i], a, lse, lse_rest) * (d[i] - delta);
-                if constexpr (kScaled<T>) s[i] *= factor;
-            }
+            for (int i = 0; i < 16; ++i) s[i] = probability<T>(s[i], a, lse, lse_rest) * (d[i] - delta);
             if (!sight.all) {
                 const Range seen(a, span.of_sinks(it), span.sink, p, j0, half);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] = seen.has(32 * n + product_row(i, 0)) ? s[i] : 0.0f;
             }
+            if constexpr (kScaled<T>) scale_to_one(s, factor, dq);
 #pragma unroll
             for (int u = 0; u < L::kUses; ++u) {
                 const typename Frag<T>::V f = operand<T>(s, u);
@@ -286,14 +287,7 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
     if constexpr (S::kHoldV)
         v.load(key < length ? static_cast<const T*>(a.v) + b * a.vs[0] + kv_head * a.vs[2] + key * a.vs[1] : nullptr, a.dim,
                lane);
-    float factor = 1.0f;
-    if constexpr (kScaled<T>) {
-        const int64_t count = peaks_of(a, kTile);
-        const float* peaks = a.peaks + (static_cast<int64_t>(b) * a.kv_heads + kv_head) * count;
-        float peak = 0.0f;
-        for (int64_t n = lane; n < count; n += kWave) peak = fmaxf(peak, peaks[n]);
-        factor = to_one(wave_max(peak));
-    }
+    float factor = kScaled<T> ? kFirstFactor : 1.0f;
     const Seen seen(a, length, j0, j0 + S::kKeys);
     const int turns = (seen.end - seen.first + BR - 1) / BR, all_turns = turns * a.group;
     const int begin = static_cast<int>(static_cast<int64_t>(all_turns) * split / splits);
@@ -347,9 +341,8 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
             if constexpr (sizeof(T) == 4) rest = *reinterpret_cast<const F*>(stat + 64 * kLseRest + at);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float x = probability<T>(s[i + e], a, lse[e], rest[e]), y = x * (d[i + e] - delta[e]);
-                s[i + e] = x;
-                d[i + e] = kScaled<T> ? y * factor : y;
+                s[i + e] = probability<T>(s[i + e], a, lse[e], rest[e]);
+                d[i + e] = s[i + e] * (d[i + e] - delta[e]);
             }
         }
         if (!all) {
@@ -363,6 +356,7 @@ __global__ __launch_bounds__((DkvShape<T, D>::kThreadCount), (kDkvWaves<T, D>)) 
                 d[i] = seen ? d[i] : 0.0f;
             }
         }
+        if constexpr (kScaled<T>) scale_to_one(d, factor, dk);
         return true;
     };
     if constexpr (kOneTile<T>) {  // Q's tile is free after dk, dO's after dv
@@ -520,21 +514,15 @@ size_t plane_bytes(const isa_block_attention* t) {
     return ceil_div(t->batch * t->heads * t->queries, 64) * 64 * kPlanes * sizeof(float);
 }
 
-size_t peak_bytes(const isa_block_attention* t) {
-    if (t->type != ISA_BLOCK_F16) return 0;
-    const int64_t each = ceil_div(t->queries * (t->heads / t->kv_heads), kTile);
-    return ceil_div(t->batch * t->kv_heads * each, 64) * 64 * sizeof(float);
-}
-
 template <typename T, int D>
 void launch(AttnArgs a, const isa_block_attention* t, hipStream_t s) {
     using S = DkvShape<T, D>;
     const int64_t rows = static_cast<int64_t>(a.batch) * a.queries * a.heads;
     if (rows) {
         const int64_t tiles = ceil_div(static_cast<int64_t>(a.queries) * a.group, kRows<T>);
-        if (a.result || kScaled<T>)
+        if (a.result)
             attention_dq_kernel<T, D><<<dim3(static_cast<unsigned>(tiles * a.batch * a.kv_heads)), kThreads<T>, 0, s>>>(a);
-        else if constexpr (!kScaled<T>)
+        else
             attention_rows_kernel<T><<<dim3(static_cast<unsigned>(ceil_div(rows * 16, kRowThreads))), kRowThreads, 0, s>>>(a);
     }
     if (!a.dk || !a.keys) return;
@@ -564,7 +552,7 @@ using namespace isa_block;
 
 extern "C" size_t isa_block_attention_backward_workspace(const isa_block_attention* t) {
     if (!t || check_attention(t)) return 0;
-    size_t bytes = plane_bytes(t) + peak_bytes(t);
+    size_t bytes = plane_bytes(t);
     for_shape(t, [&](auto, auto dim, auto shape) {
         using S = decltype(shape);
         const Cuts cuts(t, S::kKeys);
@@ -599,8 +587,7 @@ extern "C" int isa_block_attention_backward(const isa_block_attention* t, const 
     a.dout = dout;
     a.lse = const_cast<float*>(lse);
     a.delta = static_cast<float*>(workspace);
-    a.peaks = a.delta + plane_bytes(t) / sizeof(float);
-    a.partial = a.peaks + peak_bytes(t) / sizeof(float);
+    a.partial = a.delta + plane_bytes(t) / sizeof(float);
     a.result = dq;
     a.dk = dk;
     a.dv = dv;
