@@ -27,11 +27,15 @@ constexpr int kCombineWaves = 4;
 // A row's running softmax: base = c times a maximum, the weights' sum, and the product.
 template <int DB>
 struct Running {
-    float base = 0.0f, bound = -INFINITY, sum = 0.0f;
+    float top = 0.0f, base = 0.0f, bound = -INFINITY, sum = 0.0f;
     acc16 o[DB] = {};
 };
 
 constexpr float kSlack = 8.0f;
+
+// Past it base's rounding, which all weights of a row have in them as a factor until they are divided by their
+// sum, may be a power of two that passes the type's range.
+constexpr float kFar = 0x1p24f;
 
 // Weights of 32 NK keys join the running sums of their rows.
 template <typename T, int D, int NK>
@@ -59,7 +63,8 @@ __device__ __forceinline__ void attend(Running<D / 32>& r, acc16 (&s)[NK], const
     for (int n = 0; n < NK; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i) t = fmaxf(t, s[n][i]);
-    t = half_max(t) * a.c;
+    const float top = half_max(t);
+    t = top * a.c;
     if (__any(t > r.bound)) {
         const bool moves = t > r.bound;
         // 1 in rows whose base stays, 0 in those that had none
@@ -67,6 +72,7 @@ __device__ __forceinline__ void attend(Running<D / 32>& r, acc16 (&s)[NK], const
         if (moves) {
             r.bound = t + kSlack;
             r.base = t;
+            r.top = top;
         }
         r.sum *= decay;
 #pragma unroll
@@ -74,10 +80,19 @@ __device__ __forceinline__ void attend(Running<D / 32>& r, acc16 (&s)[NK], const
 #pragma unroll
             for (int i = 0; i < 16; ++i) r.o[db][i] *= decay;
     }
+    float base = r.base;
+    if (__any(fabsf(base) > kFar)) {  // there the scores' differences are taken first
+        const bool far = fabsf(base) > kFar;
+        base = far ? 0.0f : base;
+#pragma unroll
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[n][i] -= far ? r.top : 0.0f;
+    }
 #pragma unroll
     for (int n = 0; n < NK; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[n][i] = weight<T>(s[n][i], a.c, a.c_rest, r.base);
+        for (int i = 0; i < 16; ++i) s[n][i] = weight<T>(s[n][i], a.c, a.c_rest, base);
     add_weighted<T, D, NK>(r, s, vtile, lane);
     if (sizeof(T) == 2 && sinks) {
 #pragma unroll

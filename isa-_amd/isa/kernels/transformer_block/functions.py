@@ -49,7 +49,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     end is not read. A query that sees no key (more queries than keys) gives zeros and takes no
     gradient.
 
-    Softmax and sums are fp32; scale is 1 / sqrt(head_dim) unless given. In 16-bit types the weights
+    Softmax and sums are fp32; scale is 1 / sqrt(head_dim) unless given. Scores may have any finite size;
+    but where a row's highest one times scale passes 2^23, its gradients are made of that score's rounding
+    and may be infinite or NaN. In 16-bit types the weights
     p, and in the backward p and ds, are rounded to that type for the matrix cores. Of a key that some
     but not all queries of a tile see, an infinity or NaN in v reaches the others too."""
     return _binding.window_attention(q, k, v, window, sinks, scale, key_lengths)
