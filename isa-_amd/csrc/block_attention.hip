@@ -17,6 +17,12 @@
 // Masks are evaluated only in tiles that some row of a wave sees in part. A running sum is
 // rescaled only where a score passes the last maximum by 8 powers of two: until then the weights
 // are at most 256 times too large, which costs fp32 sums and both 16-bit types nothing.
+//
+// In 16-bit types p is rounded to the type for the product, as ds is in the backward: products of fp32 operands run
+// at an eighth of the rate, and one more product for what the rounding leaves would be half as many again.
+// It is taken only of sinks, which hold most of a row's weight. Against 64 bits rounded once, errors
+// are 1.3 times as large for out and 1.4 to 1.5 for the gradients (300 tokens, window 64), with strong sinks 1.0
+// for out and 1.1 for dq.
 #include "block_attention.hpp"
 
 namespace isa_block {
@@ -25,9 +31,15 @@ namespace {
 constexpr int kCombineWaves = 4;
 
 // A row's running softmax: base = c times a maximum, the weights' sum, and the product.
+//
+// In 16-bit types `sum` is that of the rounded weights, as the product takes them, and `whole` that of the
+// weights themselves, which lse is made of where it is asked for: the backward's p are not those of the forward's
+// rounding, and divided by a sum of these all of a row's p, dv and ds would be off by what its largest
+// weight was (bf16 rows with a weight of 0.97: dq 3.4e-3 off, with `whole` 2.6e-3, of which its own rounding is 1.7e-3;
+// the adding takes 4% of a training forward of 128-wide heads, nothing that shows of 64-wide ones).
 template <int DB>
 struct Running {
-    float top = 0.0f, base = 0.0f, bound = -INFINITY, sum = 0.0f;
+    float top = 0.0f, base = 0.0f, bound = -INFINITY, sum = 0.0f, whole = 0.0f;
     acc16 o[DB] = {};
 };
 
@@ -54,8 +66,11 @@ __device__ __forceinline__ void add_weighted(Running<D / 32>& r, const acc16 (&p
     reads_ahead<kProducts * L::kColumnReads, kProducts * L::kMmas, 4 * L::kColumnReads>();
 }
 
+template <typename T>
+constexpr bool kTwoSums = sizeof(T) == 2;
+
 // Scores of 32 NK keys (lane: a query) join the running sums of their rows.
-template <typename T, int D, int NK>
+template <typename T, int D, int NK, bool WHOLE>
 __device__ __forceinline__ void attend(Running<D / 32>& r, acc16 (&s)[NK], const T* vtile, const AttnArgs& a, bool sinks,
                                        int lane) {
     float t = s[0][0];
@@ -75,6 +90,7 @@ __device__ __forceinline__ void attend(Running<D / 32>& r, acc16 (&s)[NK], const
             r.top = top;
         }
         r.sum *= decay;
+        if constexpr (WHOLE) r.whole *= decay;
 #pragma unroll
         for (int db = 0; db < D / 32; ++db)
 #pragma unroll
@@ -93,6 +109,14 @@ __device__ __forceinline__ void attend(Running<D / 32>& r, acc16 (&s)[NK], const
     for (int n = 0; n < NK; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[n][i] = weight<T>(s[n][i], a.c, a.c_rest, base);
+    if constexpr (WHOLE) {
+        float part[4] = {};
+#pragma unroll
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) part[i % 4] += s[n][i];
+        r.whole += (part[0] + part[1]) + (part[2] + part[3]);
+    }
     add_weighted<T, D, NK>(r, s, vtile, lane);
     if (sizeof(T) == 2 && sinks) {
 #pragma unroll
@@ -102,12 +126,12 @@ __device__ __forceinline__ void attend(Running<D / 32>& r, acc16 (&s)[NK], const
 }
 
 // Where a row's sums go: its result, or with several blocks to a tile of rows their partial sums
-// [splits][rows of all heads][D + 4]: the product, base, sum. A sum of 0 is that of a row that sees nothing; one
+// [splits][rows of all heads][D + 4]: the product, base, sum, whole. A sum of 0 is that of a row that sees nothing; one
 // of NaN goes on to the result.
-template <typename T, int D>
+template <typename T, int D, bool WHOLE>
 __device__ __forceinline__ void finish(Running<D / 32>& r, const AttnArgs& a, const RowAt& at, int b, int split,
                                        int lane) {
-    const float sum = half_sum(r.sum);
+    const float sum = half_sum(r.sum), whole = WHOLE ? half_sum(r.whole) : sum;
     const int64_t row = at.packed(a, b);
     if (a.splits > 1) {
         const int64_t rows = static_cast<int64_t>(a.batch) * a.queries * a.heads;
@@ -116,6 +140,7 @@ __device__ __forceinline__ void finish(Running<D / 32>& r, const AttnArgs& a, co
         if (lane < 32) {
             p[D] = sum == 0.0f ? -INFINITY : r.base;
             p[D + 1] = sum;
+            p[D + 2] = whole;
         }
         return;
     }
@@ -124,7 +149,7 @@ __device__ __forceinline__ void finish(Running<D / 32>& r, const AttnArgs& a, co
     if (a.lse && lane < 32) {
         float* lse = a.lse + 2 * at.stat(a, b);
         lse[0] = sum == 0.0f ? -INFINITY : r.base;
-        lse[1] = sum == 0.0f ? 0.0f : log2f(sum);
+        lse[1] = sum == 0.0f ? 0.0f : log2f(whole);
     }
 }
 
@@ -132,7 +157,7 @@ __device__ __forceinline__ void finish(Running<D / 32>& r, const AttnArgs& a, co
 template <typename T, int D>
 constexpr int kForwardWaves = sizeof(T) == 4 && D <= 64 ? 3 : 1;
 
-template <typename T, int D>
+template <typename T, int D, bool WHOLE>
 __global__ __launch_bounds__(kThreads<T>, (kForwardWaves<T, D>)) void attention_forward_kernel(AttnArgs a) {
     using L = Tile<T, D>;
     constexpr int BN = kKeyTile<T>, NK = BN / 32, kRows = isa_block::kRows<T>;
@@ -194,12 +219,12 @@ __global__ __launch_bounds__(kThreads<T>, (kForwardWaves<T, D>)) void attention_
             loads_arrived();
             __syncthreads();
             if (it + 1 < end) fetch_k(it + 1, k0);
-            if (any) attend<T, D, NK>(r, s, v0, a, span.of_sinks(it), lane);
+            if (any) attend<T, D, NK, WHOLE>(r, s, v0, a, span.of_sinks(it), lane);
         }
     } else {
         auto compute = [&](int it, const T* kt, const T* vt) {
             acc16 s[NK];
-            if (scores(it, kt, s)) attend<T, D, NK>(r, s, vt, a, span.of_sinks(it), lane);
+            if (scores(it, kt, s)) attend<T, D, NK, WHOLE>(r, s, vt, a, span.of_sinks(it), lane);
         };
         auto fetch = [&](int it, T* kt, T* vt) {
             fetch_k(it, kt);
@@ -218,7 +243,7 @@ __global__ __launch_bounds__(kThreads<T>, (kForwardWaves<T, D>)) void attention_
             compute(it + 1, k1, v1);
         }
     }
-    if (row <= last) finish<T, D>(r, a, at, b, split, lane);
+    if (row <= last) finish<T, D, WHOLE>(r, a, at, b, split, lane);
 }
 
 // ---- few rows: tokens over a cache ---------------------------------------------------------------
@@ -235,7 +260,7 @@ struct TokenShape {
     static constexpr int kThreadCount = kWaveCount * kWave;
 };
 
-template <int DB>
+template <int DB, bool WHOLE>
 __device__ __forceinline__ void put(float* to, const Running<DB>& r, int lane) {
     using F = vec<float, 4>;
 #pragma unroll
@@ -246,10 +271,11 @@ __device__ __forceinline__ void put(float* to, const Running<DB>& r, int lane) {
                 F{r.o[db][i], r.o[db][i + 1], r.o[db][i + 2], r.o[db][i + 3]};
     to[DB * 16 * kWave + lane] = r.bound == -INFINITY ? -INFINITY : r.base;
     to[DB * 16 * kWave + kWave + lane] = r.sum;
+    if constexpr (WHOLE) to[DB * 16 * kWave + 2 * kWave + lane] = r.whole;
 }
 
 // Joins the sums that another wave put. Where neither has a maximum they are 0, or NaN if all scores were.
-template <int DB>
+template <int DB, bool WHOLE>
 __device__ __forceinline__ void join(Running<DB>& r, const float* from, int lane) {
     using F = vec<float, 4>;
     const float other = from[DB * 16 * kWave + lane], mine = r.bound == -INFINITY ? -INFINITY : r.base;
@@ -259,6 +285,7 @@ __device__ __forceinline__ void join(Running<DB>& r, const float* from, int lane
     r.bound = top;
     r.base = top == -INFINITY ? 0.0f : top;
     r.sum = r.sum * keep + from[DB * 16 * kWave + kWave + lane] * take;
+    if constexpr (WHOLE) r.whole = r.whole * keep + from[DB * 16 * kWave + 2 * kWave + lane] * take;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -269,7 +296,7 @@ __device__ __forceinline__ void join(Running<DB>& r, const float* from, int lane
         }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool WHOLE>
 __global__ __launch_bounds__((TokenShape<T, D>::kThreadCount)) void attention_token_kernel(AttnArgs a) {
     using L = Tile<T, D>;
     using S = TokenShape<T, D>;
@@ -316,7 +343,7 @@ __global__ __launch_bounds__((TokenShape<T, D>::kThreadCount)) void attention_to
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[0][i] = seen.has(product_row(i, 0)) ? s[0][i] : -INFINITY;
         }
-        attend<T, D, 1>(r, s, vt + wave * kElements, a, span.of_sinks(it), lane);
+        attend<T, D, 1, WHOLE>(r, s, vt + wave * kElements, a, span.of_sinks(it), lane);
     };
     if (begin < end) fetch(begin, k0, v0);
     for (int it = begin; it < end; it += 2) {
@@ -329,17 +356,17 @@ __global__ __launch_bounds__((TokenShape<T, D>::kThreadCount)) void attention_to
         compute(it + 1, k1, v1);
     }
     // joined by halves through the tiles' memory, a wave's sums in each of the four
-    static_assert((DB * 16 + 2) * kWave * sizeof(float) <= sizeof(k0) && W <= 8);
+    static_assert((DB * 16 + 3) * kWave * sizeof(float) <= sizeof(k0) && W <= 8);
     auto place = [&](int n) { return reinterpret_cast<float*>(n == 0 ? k0 : n == 1 ? v0 : n == 2 ? k1 : v1); };
     __syncthreads();
 #pragma unroll
     for (int n = W / 2; n >= 1; n /= 2) {
-        if (wave >= n && wave < 2 * n) put<DB>(place(wave - n), r, lane);
+        if (wave >= n && wave < 2 * n) put<DB, WHOLE>(place(wave - n), r, lane);
         __syncthreads();
-        if (wave < n) join<DB>(r, place(wave), lane);
+        if (wave < n) join<DB, WHOLE>(r, place(wave), lane);
         __syncthreads();
     }
-    if (wave == 0 && row <= last) finish<T, D>(r, a, at, b, split, lane);
+    if (wave == 0 && row <= last) finish<T, D, WHOLE>(r, a, at, b, split, lane);
 }
 
 // Rows from the partial sums of `splits` blocks (at most 64): a wave each, a lane for a block's sum.
@@ -374,11 +401,12 @@ __global__ __launch_bounds__(kCombineWaves * kWave) void attention_combine_kerne
             static_cast<T*>(a.result)[row * a.dim + e * 64 + lane] = y;
             if (a.rest) static_cast<T*>(a.rest)[row * a.dim + e * 64 + lane] = static_cast<T>(x - static_cast<float>(y));
         }
+    const float whole = a.lse ? wave_sum(have ? p[lane * step + D + 2] * mine : 0.0f) : 0.0f;
     if (a.lse && lane == 0) {
         const int64_t token = row / a.heads;
         float* lse = a.lse + 2 * ((token / a.queries * a.heads + row % a.heads) * a.queries + token % a.queries);
         lse[0] = top;
-        lse[1] = sum == 0.0f ? 0.0f : log2f(sum);
+        lse[1] = sum == 0.0f ? 0.0f : log2f(whole);
     }
 }
 
@@ -510,10 +538,17 @@ extern "C" int isa_block_attention_forward(const isa_block_attention* t, void* o
         constexpr int D = decltype(dim)::value;
         const int64_t tiles = few_rows(t) ? 1 : ceil_div(static_cast<int64_t>(a.queries) * a.group, kRows<T>);
         const dim3 blocks(static_cast<unsigned>(tiles * a.batch * a.kv_heads * a.splits));
-        if (few_rows(t))
-            attention_token_kernel<T, D><<<blocks, TokenShape<T, D>::kThreadCount, 0, s>>>(a);
+        auto launch = [&](auto with_whole) {
+            constexpr bool kWhole = decltype(with_whole)::value;
+            if (few_rows(t))
+                attention_token_kernel<T, D, kWhole><<<blocks, TokenShape<T, D>::kThreadCount, 0, s>>>(a);
+            else
+                attention_forward_kernel<T, D, kWhole><<<blocks, kThreads<T>, 0, s>>>(a);
+        };
+        if (kTwoSums<T> && a.lse)
+            launch(std::bool_constant<kTwoSums<T>>{});
         else
-            attention_forward_kernel<T, D><<<blocks, kThreads<T>, 0, s>>>(a);
+            launch(std::false_type{});
         if (a.splits > 1) {
             const int64_t rows = static_cast<int64_t>(a.batch) * a.queries * a.heads;
             attention_combine_kernel<T, D>
