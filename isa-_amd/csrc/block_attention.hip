@@ -108,7 +108,7 @@ __device__ __forceinline__ void attend(Running<D / 32>& r, acc16 (&s)[NK], const
 #pragma unroll
     for (int n = 0; n < NK; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[n][i] = weight<T>(s[n][i], a.c, a.c_rest, base);
+        for (int i = 0; i < 16; ++i) s[n][i] = weight(s[n][i], a.c, base);
     if constexpr (WHOLE) {
         float part[4] = {};
 #pragma unroll
@@ -496,9 +496,7 @@ AttnArgs attention_args(const isa_block_attention* t) {
     a.window = t->window ? static_cast<int>(t->window) : kMaxLength;
     a.sinks = t->window ? static_cast<int>(t->sinks) : 0;  // all keys are in the window
     a.scale = t->scale;
-    const double c = static_cast<double>(t->scale) * 1.44269504088896340736;
-    a.c = static_cast<float>(c);
-    a.c_rest = static_cast<float>(c - a.c);
+    a.c = static_cast<float>(static_cast<double>(t->scale) * 1.44269504088896340736);
     a.splits = 1;
     // a single token's stride says nothing
     if (t->keys <= 1) a.ks[1] = a.vs[1] = t->head_dim;

@@ -25,7 +25,7 @@ struct AttnArgs {
     int splits;         // forward: blocks that share a tile of rows
     int near, far;      // dk, dv: blocks that share a tile of keys, and one that holds sinks
     int far_tiles;      // tiles of keys that hold sinks
-    float c, c_rest, scale;  // scale log2 e as two floats
+    float c, scale;  // c = scale log2 e
 };
 
 // ---- fragments: 16 bytes a lane: of an operand's row lane % 32, one of the two chunks of a step -----
@@ -88,13 +88,10 @@ __device__ __forceinline__ float add_all(vec<float, 4> x, float sum) { return su
 // The row of a 32-row product that register i of a lane in `half` holds.
 __device__ __forceinline__ constexpr int product_row(int i, int half) { return 8 * (i / 4) + 4 * half + i % 4; }
 
-// exp2(s c - base). In fp32 c is two floats: its rounding alone, times a score, would be an error of
-// the size of all others together.
-template <typename T>
-__device__ __forceinline__ float weight(float s, float c, float c_rest, float base) {
-    float x = fmaf(s, c, -base);
-    if constexpr (sizeof(T) == 4) x = s == -INFINITY ? x : fmaf(s, c_rest, x);  // (masked)
-    return __builtin_amdgcn_exp2f(x);
+// c is one float in all types: its rounding scales all of a row's scores alike, and with c as two floats fp32's
+// errors were the same to 3%.
+__device__ __forceinline__ float weight(float s, float c, float base) {
+    return __builtin_amdgcn_exp2f(fmaf(s, c, -base));
 }
 
 // ---- tiles in LDS -----------------------------------------------------------------------------

@@ -109,9 +109,8 @@ __device__ __forceinline__ void scale_to_one(acc16& ds, float& factor, acc16 (&s
 
 template <typename T>
 __device__ __forceinline__ float probability(float s, const AttnArgs& a, float lse, float lse_rest) {
-    float x = fmaf(s, a.c, -lse);
-    if constexpr (sizeof(T) == 4) x = fmaf(s, a.c_rest, x) - lse_rest;
-    return __builtin_amdgcn_exp2f(x);
+    const float x = fmaf(s, a.c, -lse);
+    return __builtin_amdgcn_exp2f(sizeof(T) == 4 ? x - lse_rest : x);
 }
 
 // Two waves to a SIMD, so that one's products run beside the other's softmax, where 256 registers hold
