@@ -32,11 +32,13 @@ constexpr int kCombineWaves = 4;
 
 // A row's running softmax: base = c times a maximum, the weights' sum, and the product.
 //
-// In 16-bit types `sum` is that of the rounded weights, as the product takes them, and `whole` that of the
-// weights themselves, which lse is made of where it is asked for: the backward's p are not those of the forward's
-// rounding, and divided by a sum of these all of a row's p, dv and ds would be off by what its largest
-// weight was (bf16 rows with a weight of 0.97: dq 3.4e-3 off, with `whole` 2.6e-3, of which its own rounding is 1.7e-3;
-// the adding takes 4% of a training forward of 128-wide heads, nothing that shows of 64-wide ones).
+// `sum` is that of the weights as the product takes them, which out is divided by; `whole`, where lse is asked
+// for, that of the weights as the backward makes them, from its own scores and unrounded:
+//  * in 16-bit types not of the rounded ones. All of a row's p, dv and ds would be off by what its largest weight
+//    was rounded by (bf16 rows with a weight of 0.97: dq 3.4e-3 off, with `whole` 2.6e-3, of which its own rounding
+//    is 1.7e-3; the adding takes 4% of a training forward of 128-wide heads, nothing that shows of 64-wide ones);
+//  * in fp32, where few rows' scores are four sums, of scores as one, which round as the backward's do (7 x 26 tokens
+//    of 128-wide heads, weights near 1: dv 2.8e-6 off, with `whole` 1.2e-7).
 template <int DB>
 struct Running {
     float top = 0.0f, base = 0.0f, bound = -INFINITY, sum = 0.0f, whole = 0.0f;
@@ -66,13 +68,13 @@ __device__ __forceinline__ void add_weighted(Running<D / 32>& r, const acc16 (&p
     reads_ahead<kProducts * L::kColumnReads, kProducts * L::kMmas, 4 * L::kColumnReads>();
 }
 
-template <typename T>
-constexpr bool kTwoSums = sizeof(T) == 2;
+// What `whole` is made of.
+enum Whole { kNone, kWeights, kOtherScores };
 
 // Scores of 32 NK keys (lane: a query) join the running sums of their rows.
-template <typename T, int D, int NK, bool WHOLE>
+template <typename T, int D, int NK, Whole WHOLE>
 __device__ __forceinline__ void attend(Running<D / 32>& r, acc16 (&s)[NK], const T* vtile, const AttnArgs& a, bool sinks,
-                                       int lane) {
+                                       int lane, const acc16* others = nullptr) {
     float t = s[0][0];
 #pragma unroll
     for (int n = 0; n < NK; ++n)
@@ -90,31 +92,33 @@ __device__ __forceinline__ void attend(Running<D / 32>& r, acc16 (&s)[NK], const
             r.top = top;
         }
         r.sum *= decay;
-        if constexpr (WHOLE) r.whole *= decay;
+        if constexpr (WHOLE != kNone) r.whole *= decay;
 #pragma unroll
         for (int db = 0; db < D / 32; ++db)
 #pragma unroll
             for (int i = 0; i < 16; ++i) r.o[db][i] *= decay;
     }
-    float base = r.base;
+    float base = r.base, less = 0.0f;
     if (__any(fabsf(base) > kFar)) {  // there the scores' differences are taken first
         const bool far = fabsf(base) > kFar;
         base = far ? 0.0f : base;
+        less = far ? r.top : 0.0f;
 #pragma unroll
         for (int n = 0; n < NK; ++n)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[n][i] -= far ? r.top : 0.0f;
+            for (int i = 0; i < 16; ++i) s[n][i] -= less;
     }
 #pragma unroll
     for (int n = 0; n < NK; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[n][i] = weight(s[n][i], a.c, base);
-    if constexpr (WHOLE) {
+    if constexpr (WHOLE != kNone) {
         float part[4] = {};
 #pragma unroll
         for (int n = 0; n < NK; ++n)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) part[i % 4] += s[n][i];
+            for (int i = 0; i < 16; ++i)
+                part[i % 4] += WHOLE == kWeights ? s[n][i] : weight(others[n][i] - less, a.c, base);
         r.whole += (part[0] + part[1]) + (part[2] + part[3]);
     }
     add_weighted<T, D, NK>(r, s, vtile, lane);
@@ -128,10 +132,10 @@ __device__ __forceinline__ void attend(Running<D / 32>& r, acc16 (&s)[NK], const
 // Where a row's sums go: its result, or with several blocks to a tile of rows their partial sums
 // [splits][rows of all heads][D + 4]: the product, base, sum, whole. A sum of 0 is that of a row that sees nothing; one
 // of NaN goes on to the result.
-template <typename T, int D, bool WHOLE>
+template <typename T, int D, Whole WHOLE>
 __device__ __forceinline__ void finish(Running<D / 32>& r, const AttnArgs& a, const RowAt& at, int b, int split,
                                        int lane) {
-    const float sum = half_sum(r.sum), whole = WHOLE ? half_sum(r.whole) : sum;
+    const float sum = half_sum(r.sum), whole = WHOLE == kNone ? sum : half_sum(r.whole);
     const int64_t row = at.packed(a, b);
     if (a.splits > 1) {
         const int64_t rows = static_cast<int64_t>(a.batch) * a.queries * a.heads;
@@ -157,7 +161,7 @@ __device__ __forceinline__ void finish(Running<D / 32>& r, const AttnArgs& a, co
 template <typename T, int D>
 constexpr int kForwardWaves = sizeof(T) == 4 && D <= 64 ? 3 : 1;
 
-template <typename T, int D, bool WHOLE>
+template <typename T, int D, Whole WHOLE>
 __global__ __launch_bounds__(kThreads<T>, (kForwardWaves<T, D>)) void attention_forward_kernel(AttnArgs a) {
     using L = Tile<T, D>;
     constexpr int BN = kKeyTile<T>, NK = BN / 32, kRows = isa_block::kRows<T>;
@@ -260,7 +264,7 @@ struct TokenShape {
     static constexpr int kThreadCount = kWaveCount * kWave;
 };
 
-template <int DB, bool WHOLE>
+template <int DB, Whole WHOLE>
 __device__ __forceinline__ void put(float* to, const Running<DB>& r, int lane) {
     using F = vec<float, 4>;
 #pragma unroll
@@ -271,11 +275,11 @@ __device__ __forceinline__ void put(float* to, const Running<DB>& r, int lane) {
                 F{r.o[db][i], r.o[db][i + 1], r.o[db][i + 2], r.o[db][i + 3]};
     to[DB * 16 * kWave + lane] = r.bound == -INFINITY ? -INFINITY : r.base;
     to[DB * 16 * kWave + kWave + lane] = r.sum;
-    if constexpr (WHOLE) to[DB * 16 * kWave + 2 * kWave + lane] = r.whole;
+    if constexpr (WHOLE != kNone) to[DB * 16 * kWave + 2 * kWave + lane] = r.whole;
 }
 
 // Joins the sums that another wave put. Where neither has a maximum they are 0, or NaN if all scores were.
-template <int DB, bool WHOLE>
+template <int DB, Whole WHOLE>
 __device__ __forceinline__ void join(Running<DB>& r, const float* from, int lane) {
     using F = vec<float, 4>;
     const float other = from[DB * 16 * kWave + lane], mine = r.bound == -INFINITY ? -INFINITY : r.base;
@@ -285,7 +289,7 @@ __device__ __forceinline__ void join(Running<DB>& r, const float* from, int lane
     r.bound = top;
     r.base = top == -INFINITY ? 0.0f : top;
     r.sum = r.sum * keep + from[DB * 16 * kWave + kWave + lane] * take;
-    if constexpr (WHOLE) r.whole = r.whole * keep + from[DB * 16 * kWave + 2 * kWave + lane] * take;
+    if constexpr (WHOLE != kNone) r.whole = r.whole * keep + from[DB * 16 * kWave + 2 * kWave + lane] * take;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -296,7 +300,7 @@ __device__ __forceinline__ void join(Running<DB>& r, const float* from, int lane
         }
 }
 
-template <typename T, int D, bool WHOLE>
+template <typename T, int D, Whole WHOLE>
 __global__ __launch_bounds__((TokenShape<T, D>::kThreadCount)) void attention_token_kernel(AttnArgs a) {
     using L = Tile<T, D>;
     using S = TokenShape<T, D>;
@@ -334,16 +338,24 @@ __global__ __launch_bounds__((TokenShape<T, D>::kThreadCount)) void attention_to
         // fp32 scores as four sums: one chain of 64 products was most of the error of a token (12 heads of 64,
         // 516 keys: out 4.1e-7 to 7.0e-7 off, with four sums 2.1e-7 to 3.0e-7, the time is the same)
         constexpr int kSums = sizeof(T) == 4 ? 4 : 1;
-        acc16 sums[kSums] = {}, s[1];
+        acc16 sums[kSums] = {}, s[1], chain[1] = {};
 #pragma unroll
-        for (int t = 0; t < L::kSteps; ++t) mma(sums[t % kSums], L::row(kt + wave * kElements, 0, t, lane), q[t]);
+        for (int t = 0; t < L::kSteps; ++t) {
+            const auto keys = L::row(kt + wave * kElements, 0, t, lane);
+            mma(sums[t % kSums], keys, q[t]);
+            if constexpr (WHOLE == kOtherScores) mma(chain[0], keys, q[t]);
+        }
         s[0] = kSums == 4 ? (sums[0] + sums[1 % kSums]) + (sums[2 % kSums] + sums[3 % kSums]) : sums[0];
         if (!sight.all) {
             const Range seen(a, span.of_sinks(it), span.sink, p, j0, half);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[0][i] = seen.has(product_row(i, 0)) ? s[0][i] : -INFINITY;
+            for (int i = 0; i < 16; ++i) {
+                const bool has = seen.has(product_row(i, 0));
+                s[0][i] = has ? s[0][i] : -INFINITY;
+                if constexpr (WHOLE == kOtherScores) chain[0][i] = has ? chain[0][i] : -INFINITY;
+            }
         }
-        attend<T, D, 1, WHOLE>(r, s, vt + wave * kElements, a, span.of_sinks(it), lane);
+        attend<T, D, 1, WHOLE>(r, s, vt + wave * kElements, a, span.of_sinks(it), lane, chain);
     };
     if (begin < end) fetch(begin, k0, v0);
     for (int it = begin; it < end; it += 2) {
@@ -536,17 +548,13 @@ extern "C" int isa_block_attention_forward(const isa_block_attention* t, void* o
         constexpr int D = decltype(dim)::value;
         const int64_t tiles = few_rows(t) ? 1 : ceil_div(static_cast<int64_t>(a.queries) * a.group, kRows<T>);
         const dim3 blocks(static_cast<unsigned>(tiles * a.batch * a.kv_heads * a.splits));
-        auto launch = [&](auto with_whole) {
-            constexpr bool kWhole = decltype(with_whole)::value;
-            if (few_rows(t))
-                attention_token_kernel<T, D, kWhole><<<blocks, TokenShape<T, D>::kThreadCount, 0, s>>>(a);
-            else
-                attention_forward_kernel<T, D, kWhole><<<blocks, kThreads<T>, 0, s>>>(a);
-        };
-        if (kTwoSums<T> && a.lse)
-            launch(std::bool_constant<kTwoSums<T>>{});
+        const auto launch = [&](auto kernel, int threads) { kernel<<<blocks, threads, 0, s>>>(a); };
+        constexpr Whole kTokens = sizeof(T) == 4 ? kOtherScores : kWeights, kRowsOf = sizeof(T) == 4 ? kNone : kWeights;
+        if (few_rows(t))
+            launch(a.lse ? attention_token_kernel<T, D, kTokens> : attention_token_kernel<T, D, kNone>,
+                   TokenShape<T, D>::kThreadCount);
         else
-            launch(std::false_type{});
+            launch(a.lse ? attention_forward_kernel<T, D, kRowsOf> : attention_forward_kernel<T, D, kNone>, kThreads<T>);
         if (a.splits > 1) {
             const int64_t rows = static_cast<int64_t>(a.batch) * a.queries * a.heads;
             attention_combine_kernel<T, D>

@@ -95,3 +95,22 @@ def test_scales(cuda_device, dtype, scale):
         floor = 2.0 ** -25 * w.numel() ** 0.5 / float(w.norm()) if dtype == torch.float16 else 0.0
         close(x, w, (forward if name in ("out", "dv") else backward) + floor, name)
     close(token[0], want[0][:, -1:], forward, "a token")
+
+
+@pytest.mark.parametrize("shape", [(7, 26, 8, 8, 128), (2, 8, 8, 2, 128), (3, 30, 4, 4, 64)], ids=str)
+def test_fp32_weights_near_one_of_few_rows(cuda_device, shape):
+    """Few rows go through the kernel for tokens; the backward makes p of its own scores and of that kernel's lse. A
+    row's largest weight is near 1 if both round the scores alike, whatever their size (some 100 here): a
+    weight is then off by an ulp or two of exp2, its sums of up to 32 terms by as much. 8 u for dv, which is
+    most of the first key's; a score rounded otherwise is off by some u of 100 itself."""
+    b, n, h, kv, d = shape
+    print(f"[case] fp32, weights near 1, {shape}", flush=True)
+    g = torch.Generator().manual_seed(5)
+    q, k, v, dout = (torch.randn(b, n, heads, d, generator=g) for heads in (h, kv, kv, h))
+    s = torch.randn(d, generator=g) * (1.5 * (64 / d) ** 0.5)
+    q, k = q + s, k * 0.3
+    k[:, :1] += s
+    q, k, v, dout = (t.to(cuda_device) for t in (q, k, v, dout))
+    want = attention64(q, k, v, None, 0, d ** -0.5, None, dout)
+    got = run(q, k, v, dout)
+    close(got[3], want[3], 8 * UNIT[torch.float32], "dv")
