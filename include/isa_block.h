@@ -112,7 +112,8 @@ int isa_block_attention_backward(const isa_block_attention* att, const void* out
 
 /* ---- cross-entropy ---------------------------------------------------------------------
  *   row r: loss_r = log(sum_j exp(x_rj)) - x_r,target; 0 where target == ignore_index
- * A target outside 0 .. vocab - 1 that is not ignore_index makes its row's loss and gradients NaN. */
+ * A target outside 0 .. vocab - 1 that is not ignore_index makes its row's loss and gradients NaN.
+ * rows <= 2^24 (they are counted in fp32). */
 typedef struct isa_block_loss {
     int type; /* of the logits and their gradient */
     int64_t rows, vocab;

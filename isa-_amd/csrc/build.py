@@ -1,9 +1,9 @@
 """Build the HIP libraries (gfx950) in-tree with hipcc.
 
 Usage: ``python isa-_amd/csrc/build.py`` (also called by ``__graft_entry__.build()``).
-Each library lands next to its ctypes loader: ``libisa_ekv_hip.so`` in
-``isa/kernels/transformer_ffn/``, ``libisa_block_hip.so`` in ``isa/kernels/transformer_block/``
-with ``_binding.so``, torch's binding to it.
+Each library lands next to its loader: ``libisa_ekv_hip.so`` in ``isa/kernels/transformer_ffn/``, which
+loads it with ctypes; ``libisa_block_hip.so`` in ``isa/kernels/transformer_block/`` with ``_binding.so``,
+torch's binding to it, a module that the package imports.
 """
 
 from __future__ import annotations
