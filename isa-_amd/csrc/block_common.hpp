@@ -25,6 +25,38 @@ struct alignas(sizeof(T) * N) Pack {
 
 constexpr int kWave = 64;
 
+// N elements as one load or store at any element's address; of `left` < N elements, one by one.
+template <typename T, int N>
+struct Loose {
+    typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void load_loose(Pack<T, N>& p, const T* from, int left) {
+    if (left >= N) {
+        const typename Loose<T, N>::type x = *reinterpret_cast<const typename Loose<T, N>::type*>(from);
+#pragma unroll
+        for (int e = 0; e < N; ++e) p.v[e] = x[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) p.v[e] = e < left ? from[e] : static_cast<T>(0.0f);
+    }
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_loose(T* to, const Pack<T, N>& p, int left) {
+    if (left >= N) {
+        typename Loose<T, N>::type x;
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = p.v[e];
+        *reinterpret_cast<typename Loose<T, N>::type*>(to) = x;
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (e < left) to[e] = p.v[e];
+    }
+}
+
 // v_permlane32_swap exchanges the upper half of one register with the lower half of another:
 // given the same value twice, one result has the lower half's values in both halves, the
 // other the upper half's.

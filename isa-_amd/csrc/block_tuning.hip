@@ -1,0 +1,283 @@
+// Losses of tuning a model by rewards or by pairs of answers, and their gradients: the C entries.
+//
+// The policy loss is a function of each row's l alone: one pass over the logits, as the cross-entropy's, bound by
+// HBM. The preference loss's slope needs the sums of whole sequences: one pass reads the logits for l and the
+// rows' statistics, a block a pair makes the slopes, a second pass reads them again and writes the gradient.
+#include "block_loss.hpp"
+
+namespace isa_block {
+namespace {
+
+constexpr int kPairThreads = 256;
+
+struct PairArgs {
+    const double* row_logp;  // [2 pairs][tokens]
+    const float* ref;
+    int64_t pairs, tokens;
+    float *loss, *logp, *slope;  // [pairs], [2 pairs], [2 pairs] or null
+    float beta;
+};
+
+__device__ __forceinline__ double sequence_sum(const double* rows, int64_t n, double* slots) {
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += kPairThreads) s += rows[i];
+    slots[threadIdx.x] = s;
+    __syncthreads();
+    for (int half = kPairThreads / 2; half; half /= 2) {
+        if (static_cast<int>(threadIdx.x) < half) slots[threadIdx.x] += slots[threadIdx.x + half];
+        __syncthreads();
+    }
+    return slots[0];
+}
+
+__global__ __launch_bounds__(kPairThreads) void preference_pair_kernel(PairArgs a) {
+    __shared__ double slots[2][kPairThreads];
+    for (int64_t p = blockIdx.x; p < a.pairs; p += gridDim.x) {
+        const double chosen = sequence_sum(a.row_logp + p * a.tokens, a.tokens, slots[0]);
+        const double other = sequence_sum(a.row_logp + (a.pairs + p) * a.tokens, a.tokens, slots[1]);
+        if (threadIdx.x == 0) {
+            const double m = a.beta * ((chosen - a.ref[p]) - (other - a.ref[a.pairs + p]));
+            const double slope = -a.beta / (1.0 + exp(m));
+            a.loss[p] = static_cast<float>((m < 0.0 ? -m : 0.0) + log1p(exp(-fabs(m))));
+            a.logp[p] = static_cast<float>(chosen);
+            a.logp[a.pairs + p] = static_cast<float>(other);
+            if (a.slope) {
+                a.slope[p] = static_cast<float>(slope);
+                a.slope[a.pairs + p] = static_cast<float>(-slope);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+__global__ __launch_bounds__(kPairThreads) void preference_sum_kernel(const float* loss, int64_t pairs, int mean,
+                                                                      float* out) {
+    __shared__ double slots[kPairThreads];
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < pairs; i += kPairThreads) s += loss[i];
+    slots[threadIdx.x] = s;
+    __syncthreads();
+    for (int half = kPairThreads / 2; half; half /= 2) {
+        if (static_cast<int>(threadIdx.x) < half) slots[threadIdx.x] += slots[threadIdx.x + half];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) out[0] = static_cast<float>(mean ? slots[0] / pairs : slots[0]);
+}
+
+int check(const isa_train_policy* p) {
+    if (!p) return fail("policy is null");
+    if (int rc = check(&p->loss)) return rc;
+    if (p->loss.rows && (!p->old_logp || !p->advantages)) return fail("old_logp and advantages must be set");
+    if (!(p->low >= 0.0f && p->high >= p->low)) return fail("the ratio's bounds must be 0 <= low <= high");
+    if (!(p->kl >= 0.0f)) return fail("kl must not be negative");
+    if (p->loss.rows && p->kl != 0.0f && !p->ref_logp) return fail("kl needs ref_logp");
+    return 0;
+}
+
+LossArgs args_of(const isa_train_policy* p) {
+    LossArgs a = args_of(&p->loss);
+    a.old_logp = p->old_logp;
+    a.advantages = p->advantages;
+    a.ref_logp = p->ref_logp;
+    a.low = p->low;
+    a.high = p->high;
+    a.kl = p->kl;
+    return a;
+}
+
+int check(const isa_train_preference* p) {
+    if (!p) return fail("preference is null");
+    if (int rc = check(&p->loss)) return rc;
+    if (p->pairs < 0 || p->tokens < 0 || p->pairs > kMaxRows || p->tokens > kMaxRows ||
+        p->loss.rows != 2 * p->pairs * p->tokens)
+        return fail("rows must be 2 pairs tokens");
+    if (p->pairs && !p->ref_logp) return fail("ref_logp must be set");
+    if (!(p->beta > 0.0f) || p->beta > 3e38f) return fail("beta must be positive and finite");
+    return 0;
+}
+
+// The workspace's parts: rows' l, their statistics, the pairs' losses, the sequences' slopes.
+struct PreferenceSpace {
+    size_t stats, loss, slope, bytes;
+    explicit PreferenceSpace(const isa_train_preference* p) {
+        stats = static_cast<size_t>(p->loss.rows) * sizeof(double);
+        loss = stats + static_cast<size_t>(p->loss.rows) * 2 * sizeof(float);
+        slope = loss + static_cast<size_t>(p->pairs) * sizeof(float);
+        bytes = slope + static_cast<size_t>(2 * p->pairs) * sizeof(float) + 256;
+    }
+};
+
+int check_workspace(const isa_train_preference* p, const void* workspace, size_t bytes) {
+    if (bytes < PreferenceSpace(p).bytes) return fail("workspace too small: %zu bytes", bytes);
+    if (!workspace || !aligned(workspace, 256)) return fail("workspace must be 256-byte aligned");
+    return 0;
+}
+
+// l of rows, sequences' sums, losses and slopes of pairs.
+int run_pairs(const isa_train_preference* p, float* stats, float* pair_loss, float* logp, float* slope,
+              void* workspace, hipStream_t s) {
+    LossArgs a = args_of(&p->loss);
+    a.row_logp = static_cast<double*>(workspace);
+    a.stats = stats;
+    if (p->loss.rows) run_rows<Of::kCrossEntropy>(p->loss.type, a, s);
+    if (int rc = launched("loss_kernel")) return rc;
+    const PairArgs b{a.row_logp, p->ref_logp, p->pairs, p->tokens, pair_loss, logp, slope, p->beta};
+    const int64_t blocks = std::min<int64_t>(p->pairs, 4096);
+    if (blocks) preference_pair_kernel<<<dim3(static_cast<unsigned>(blocks)), dim3(kPairThreads), 0, s>>>(b);
+    return launched("preference_pair_kernel");
+}
+
+int run_pairs_backward(const isa_train_preference* p, const float* stats, const float* slope, const float* by, int step,
+                       float scale, void* grad, int64_t grad_stride, hipStream_t s) {
+    LossArgs a = args_of(&p->loss);
+    a.stats = const_cast<float*>(stats);
+    a.slope = slope;
+    a.tokens = p->tokens;
+    a.pairs = p->pairs;
+    a.scale_by = by;
+    a.scale_step = step;
+    a.scale = scale;
+    a.grad = grad;
+    a.grad_stride = grad_stride;
+    a.backwards = true;  // those that were read last are in the caches
+    run_backward<true>(p->loss.type, a, s);
+    return launched("loss_backward_kernel");
+}
+
+}  // namespace
+}  // namespace isa_block
+
+using namespace isa_block;
+
+extern "C" int isa_train_policy_forward(const isa_train_policy* p, int reduction, float* out, float* logp, float* stats,
+                                        float* slope, float* count, void* workspace, size_t workspace_bytes,
+                                        void* stream) {
+    if (int rc = check(p)) return rc;
+    const isa_block_loss* l = &p->loss;
+    if (reduction < ISA_BLOCK_MEAN || reduction > ISA_BLOCK_NONE) return fail("unknown reduction %d", reduction);
+    if (reduction == ISA_BLOCK_NONE && l->rows == 0) return 0;
+    if (!out || (l->rows && !logp)) return fail("out and logp must be set");
+    if ((stats == nullptr) != (slope == nullptr) || (stats == nullptr) != (count == nullptr))
+        return fail("stats, slope and count go together");
+    if (int rc = check_workspace(l, workspace, workspace_bytes)) return rc;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    float* ws = static_cast<float*>(workspace);
+    if (!count) count = ws;
+    if (reduction == ISA_BLOCK_MEAN) {
+        loss_count_kernel<<<1, kMostThreads, 0, s>>>(l->targets, l->rows, l->ignore_index, count);
+        if (int rc = launched("loss_count_kernel")) return rc;
+    }
+    LossArgs a = args_of(p);
+    a.row_loss = reduction == ISA_BLOCK_NONE ? out : ws + 64;
+    a.logp = logp;
+    a.stats = stats;
+    a.row_slope = slope;
+    if (l->rows) run_rows<Of::kPolicy>(l->type, a, s);
+    if (int rc = launched("loss_kernel")) return rc;
+    if (reduction == ISA_BLOCK_NONE) return 0;
+    loss_sum_kernel<<<1, kMostThreads, 0, s>>>(ws + 64, l->rows, reduction == ISA_BLOCK_MEAN ? count : nullptr, out);
+    return launched("loss_sum_kernel");
+}
+
+extern "C" int isa_train_policy_backward(const isa_block_loss* l, int reduction, const float* stats, const float* slope,
+                                         const float* count, const float* grad_out, void* grad, int64_t grad_stride,
+                                         void* stream) {
+    if (int rc = check(l)) return rc;
+    if (reduction < ISA_BLOCK_MEAN || reduction > ISA_BLOCK_NONE) return fail("unknown reduction %d", reduction);
+    if (l->rows == 0) return 0;
+    if (!stats || !slope || !grad_out || !grad || (reduction == ISA_BLOCK_MEAN && !count))
+        return fail("stats, slope, grad_out, grad_logits and a mean's count must be set");
+    if (!aligned(grad, type_bytes(l->type))) return fail("grad_logits is not aligned to its type");
+    LossArgs a = args_of(l);
+    a.stats = const_cast<float*>(stats);
+    a.slope = slope;
+    a.tokens = 1;
+    a.pairs = l->rows;
+    a.count = reduction == ISA_BLOCK_MEAN ? count : nullptr;
+    a.scale_by = grad_out;
+    a.scale_step = reduction == ISA_BLOCK_NONE;
+    a.scale = 1.0f;
+    a.grad = grad;
+    a.grad_stride = grad_stride;
+    run_backward<true>(l->type, a, static_cast<hipStream_t>(stream));
+    return launched("loss_backward_kernel");
+}
+
+extern "C" int isa_train_policy_with_grad(const isa_train_policy* p, float grad_scale, float* out, float* logp,
+                                          void* grad, int64_t grad_stride, void* workspace, size_t workspace_bytes,
+                                          void* stream) {
+    if (int rc = check(p)) return rc;
+    const isa_block_loss* l = &p->loss;
+    if (!out || (l->rows && (!grad || !logp))) return fail("out, logp and grad_logits must be set");
+    if (l->rows && !aligned(grad, type_bytes(l->type))) return fail("grad_logits is not aligned to its type");
+    if (int rc = check_workspace(l, workspace, workspace_bytes)) return rc;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    float* ws = static_cast<float*>(workspace);
+    loss_count_kernel<<<1, kMostThreads, 0, s>>>(l->targets, l->rows, l->ignore_index, ws);
+    if (int rc = launched("loss_count_kernel")) return rc;
+    LossArgs a = args_of(p);
+    a.row_loss = ws + 64;
+    a.logp = logp;
+    a.count = ws;
+    a.scale = grad_scale;
+    a.grad = grad;
+    a.grad_stride = grad_stride;
+    if (l->rows) run_rows<Of::kPolicy>(l->type, a, s);
+    if (int rc = launched("loss_kernel")) return rc;
+    loss_sum_kernel<<<1, kMostThreads, 0, s>>>(ws + 64, l->rows, ws, out);
+    return launched("loss_sum_kernel");
+}
+
+extern "C" size_t isa_train_preference_workspace(const isa_train_preference* p) {
+    return check(p) ? 0 : PreferenceSpace(p).bytes;
+}
+
+extern "C" int isa_train_preference_forward(const isa_train_preference* p, int reduction, float* out, float* logp,
+                                            float* stats, float* slope, void* workspace, size_t workspace_bytes,
+                                            void* stream) {
+    if (int rc = check(p)) return rc;
+    if (reduction < ISA_BLOCK_MEAN || reduction > ISA_BLOCK_NONE) return fail("unknown reduction %d", reduction);
+    if (reduction == ISA_BLOCK_NONE && p->pairs == 0) return 0;
+    if (!out || (p->pairs && !logp)) return fail("out and logp must be set");
+    if (p->loss.rows && (stats == nullptr) != (slope == nullptr)) return fail("stats and slope go together");
+    if (int rc = check_workspace(p, workspace, workspace_bytes)) return rc;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    char* ws = static_cast<char*>(workspace);
+    float* pair_loss = reduction == ISA_BLOCK_NONE ? out : reinterpret_cast<float*>(ws + PreferenceSpace(p).loss);
+    if (int rc = run_pairs(p, stats, pair_loss, logp, slope, ws, s)) return rc;
+    if (reduction == ISA_BLOCK_NONE) return 0;
+    preference_sum_kernel<<<1, kPairThreads, 0, s>>>(pair_loss, p->pairs, reduction == ISA_BLOCK_MEAN, out);
+    return launched("preference_sum_kernel");
+}
+
+extern "C" int isa_train_preference_backward(const isa_train_preference* p, int reduction, const float* stats,
+                                             const float* slope, const float* grad_out, void* grad, int64_t grad_stride,
+                                             void* stream) {
+    if (int rc = check(p)) return rc;
+    if (reduction < ISA_BLOCK_MEAN || reduction > ISA_BLOCK_NONE) return fail("unknown reduction %d", reduction);
+    if (p->loss.rows == 0) return 0;
+    if (!stats || !slope || !grad_out || !grad) return fail("stats, slope, grad_out and grad_logits must be set");
+    if (!aligned(grad, type_bytes(p->loss.type))) return fail("grad_logits is not aligned to its type");
+    return run_pairs_backward(p, stats, slope, grad_out, reduction == ISA_BLOCK_NONE,
+                              reduction == ISA_BLOCK_MEAN ? 1.0f / static_cast<float>(p->pairs) : 1.0f, grad, grad_stride,
+                              static_cast<hipStream_t>(stream));
+}
+
+extern "C" int isa_train_preference_with_grad(const isa_train_preference* p, float grad_scale, float* out, float* logp,
+                                              void* grad, int64_t grad_stride, void* workspace, size_t workspace_bytes,
+                                              void* stream) {
+    if (int rc = check(p)) return rc;
+    if (!out || (p->pairs && !logp) || (p->loss.rows && !grad)) return fail("out, logp and grad_logits must be set");
+    if (p->loss.rows && !aligned(grad, type_bytes(p->loss.type))) return fail("grad_logits is not aligned to its type");
+    if (int rc = check_workspace(p, workspace, workspace_bytes)) return rc;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const PreferenceSpace at(p);
+    char* ws = static_cast<char*>(workspace);
+    float *stats = reinterpret_cast<float*>(ws + at.stats), *pair_loss = reinterpret_cast<float*>(ws + at.loss),
+          *slope = reinterpret_cast<float*>(ws + at.slope);
+    if (int rc = run_pairs(p, stats, pair_loss, logp, slope, ws, s)) return rc;
+    preference_sum_kernel<<<1, kPairThreads, 0, s>>>(pair_loss, p->pairs, 1, out);
+    if (int rc = launched("preference_sum_kernel")) return rc;
+    if (p->loss.rows == 0) return 0;
+    return run_pairs_backward(p, stats, slope, nullptr, 0, grad_scale / static_cast<float>(p->pairs), grad, grad_stride, s);
+}

@@ -23,12 +23,13 @@ REPO = PKG_ROOT.parent
 SOURCES = [CSRC / "ekv_lut.hip"]
 INCLUDE = REPO / "include"
 OUT = PKG_ROOT / "isa" / "kernels" / "transformer_ffn" / "libisa_ekv_hip.so"
-BLOCK_SOURCES = [CSRC / f"block_{name}.hip" for name in ("api", "norm", "attention", "attention_backward", "loss")]
+BLOCK_SOURCES = [CSRC / f"block_{name}.hip" for name in ("api", "norm", "attention", "attention_backward", "loss", "embedding",
+                                                        "dropout", "tuning")]
 # products keep their sums in ordinary registers, which the softmax between two products works on: with
 # accumulation registers every one of them is moved there and back
 BLOCK_FLAGS = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 BLOCK_OUT = PKG_ROOT / "isa" / "kernels" / "transformer_block" / "libisa_block_hip.so"
-BINDING_SOURCE = CSRC / "block_torch.cpp"
+BINDING_SOURCES = [CSRC / "block_torch.cpp", CSRC / "block_torch_train.cpp"]
 BINDING_OUT = BLOCK_OUT.with_name("_binding.so")
 ARCH = os.environ.get("ISA_EKV_OFFLOAD_ARCH", "gfx950")
 
@@ -78,7 +79,7 @@ def _block(verbose: bool, pool: ThreadPoolExecutor) -> None:
     os.replace(tmp, BLOCK_OUT)
 
 
-def _binding_object(obj: Path, verbose: bool) -> None:
+def _binding_object(source: Path, obj: Path, verbose: bool) -> None:
     import torch
     from torch.utils.cpp_extension import include_paths
 
@@ -87,28 +88,29 @@ def _binding_object(obj: Path, verbose: bool) -> None:
     rocm = Path(hipcc()).resolve().parents[1] / "include"
     includes = [f"-I{INCLUDE}", *(f"-isystem{p}" for p in (*include_paths(), sysconfig.get_paths()["include"], rocm))]
     _run(["g++", "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-          *flags, *includes, "-c", "-o", str(obj), str(BINDING_SOURCE)], verbose)
+          *flags, *includes, "-c", "-o", str(obj), str(source)], verbose)
 
 
-def _link_binding(obj: Path, verbose: bool) -> None:
+def _link_binding(objects: list, verbose: bool) -> None:
     import torch
 
     lib = Path(torch.__file__).resolve().parent / "lib"
     tmp = BINDING_OUT.with_suffix(".so.tmp")
-    _run(["g++", "-shared", "-o", str(tmp), str(obj), f"-L{BLOCK_OUT.parent}", "-lisa_block_hip", f"-L{lib}", "-lc10",
+    _run(["g++", "-shared", "-o", str(tmp), *map(str, objects), f"-L{BLOCK_OUT.parent}", "-lisa_block_hip", f"-L{lib}", "-lc10",
           "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"], verbose)
     os.replace(tmp, BINDING_OUT)
 
 
 def build(verbose: bool = False) -> Path:
     """Compile the libraries and the binding, side by side; returns the projection's library."""
-    with tempfile.TemporaryDirectory() as work, ThreadPoolExecutor(max_workers=2 + len(BLOCK_SOURCES)) as pool:
-        obj = Path(work) / "binding.o"
-        others = [pool.submit(_ekv, verbose), pool.submit(_binding_object, obj, verbose)]
+    with tempfile.TemporaryDirectory() as work, ThreadPoolExecutor(max_workers=1 + len(BINDING_SOURCES) + len(BLOCK_SOURCES)) as pool:
+        objects = [Path(work) / f"{src.stem}.o" for src in BINDING_SOURCES]
+        others = [pool.submit(_ekv, verbose),
+                  *(pool.submit(_binding_object, src, obj, verbose) for src, obj in zip(BINDING_SOURCES, objects))]
         _block(verbose, pool)
         for job in others:
             job.result()
-        _link_binding(obj, verbose)
+        _link_binding(objects, verbose)
     return OUT
 
 

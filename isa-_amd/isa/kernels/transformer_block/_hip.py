@@ -1,4 +1,4 @@
-"""Loads libisa_block_hip.so (include/isa_block.h) and torch's binding to it, `_binding.so`.
+"""Loads libisa_block_hip.so (include/isa_block.h, include/isa_train.h) and torch's binding to it, `_binding.so`.
 
 They are the only compute path: importing fails loudly when one is missing or was built for
 another ABI. torch is imported first, so that both use the HIP runtime that it loaded.
@@ -22,7 +22,8 @@ def load():
     except ImportError as e:
         raise HipExtensionError(f"{LIB_PATH.name} or its binding cannot be loaded from {LIB_PATH.parent} ({e}); build "
                                 "them with `python isa-_amd/csrc/build.py` (or __graft_entry__.build())") from e
-    if _binding.abi_version() != _binding.ABI_VERSION:
-        raise HipExtensionError(f"{LIB_PATH} has ABI version {_binding.abi_version()}, its binding expects "
-                                f"{_binding.ABI_VERSION}; rebuild them")
+    has = (_binding.abi_version(), _binding.train_abi_version())
+    expects = (_binding.ABI_VERSION, _binding.TRAIN_ABI_VERSION)
+    if has != expects:
+        raise HipExtensionError(f"{LIB_PATH} has ABI versions {has}, its binding expects {expects}; rebuild them")
     return _binding
