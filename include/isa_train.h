@@ -37,17 +37,21 @@ typedef struct isa_train_embedding {
 } isa_train_embedding;
 #define ISA_TRAIN_EMBEDDING_MAX_ROWS (1 << 24) /* of a table */
 
-/* y [tokens][dim] */
-int isa_train_embedding_forward(const isa_train_embedding* e, void* y, void* stream);
+/* y [tokens][dim]. For a backward call: lists (256-byte aligned), which the call fills with the tokens of each row of
+ * the tables whose gradient will be asked for (weight, places: 0 or 1), without those whose id is `skip` (-1: none) or
+ * whose id or place is outside its table; else null, 0, 0. */
+size_t isa_train_embedding_lists(const isa_train_embedding* e, int weight, int places);
+int isa_train_embedding_forward(const isa_train_embedding* e, void* y, int weight, int places, int64_t skip,
+                                void* lists, size_t lists_bytes, void* stream);
 
-/* The gradient of a table of `rows` rows: grad [rows][dim] of grad_y [tokens][dim],
- *   grad_v = scale (sum of grad_y_t over the tokens with key_t = v)
- * in fp32, each row rounded once. keys [tokens], or null: key_t = t mod period. Keys outside 0 .. rows - 1 and
- * `skip` (-1: none) take no part. */
-size_t isa_train_embedding_backward_workspace(int64_t tokens, int64_t rows, int64_t dim, int has_keys);
-int isa_train_embedding_backward(int type, int64_t tokens, int64_t rows, int64_t dim, const int64_t* keys,
-                                 int64_t period, int64_t skip, float scale, const void* grad_y, void* grad,
-                                 void* workspace, size_t workspace_bytes, void* stream);
+/* The tables' gradients of grad_y [tokens][dim], in fp32 with each row rounded once:
+ *   grad_weight [vocab][dim]: scale (sum of grad_y_t over a row's list),  grad_places [places][dim]: the sum alone
+ * e, ids and place_ids as they were in the forward call that filled lists, with the same `weight` and `places` here as
+ * listed_weight and listed_places. Either gradient may be null: not computed. The tables are not read. */
+size_t isa_train_embedding_backward_workspace(const isa_train_embedding* e, int weight, int places);
+int isa_train_embedding_backward(const isa_train_embedding* e, const void* lists, size_t lists_bytes,
+                                 const void* grad_y, void* grad_weight, void* grad_places, int listed_weight,
+                                 int listed_places, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- dropout -----------------------------------------------------------------------------
  * Element (r, c) of [rows][dim] is dropped iff its 16-bit number is below `threshold`; what is kept is multiplied

@@ -6,10 +6,10 @@
 // whose rows are zeros. The gradient's sums use no atomics: tokens are sorted by their row, in order within
 // one, and a row's sum is taken in that order.
 //
-// The sort is one launch without any exchange between its blocks: a block owns a range of rows, reads all
-// keys, counts those below its range (where its part of the list starts) and places those inside.
+// The sort needs no exchange between its blocks: a block owns a range of rows, reads all keys, counts those
+// below its range (where its part of the list starts) and places those inside. It runs in the lookup's launch.
 // A row with many tokens would be one wave's long walk: lists longer than a tile are summed by tiles of
-// the sorted list, whose sums of a row are added up in a third launch.
+// the sorted list, in the rows' launch, and a third launch adds up their sums. Both tables share the launches.
 #include "block_common.hpp"
 
 #include <algorithm>
@@ -22,6 +22,40 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxBlocks = 8192;
 
+// ---- columns ------------------------------------------------------------------------------
+
+// 16 bytes of a row of `dim` elements from column `at` on, which ends with the row: a row's last piece starts
+// earlier where its width is no multiple, and two lanes then have the same elements with the same values. So all loads
+// and stores are whole vectors, at any element's address. SHORT: rows of less than 16 bytes, element by element.
+template <typename T>
+constexpr int kPiece = 16 / sizeof(T);
+
+template <typename T, bool SHORT>
+__device__ __forceinline__ int piece_at(int column, int dim) {
+    return SHORT ? 0 : std::min(column, dim - kPiece<T>);
+}
+
+template <typename T, bool SHORT>
+__device__ __forceinline__ void load_piece(vec<T, kPiece<T>>& p, const T* from, int dim) {
+    if constexpr (SHORT) {
+#pragma unroll
+        for (int e = 0; e < kPiece<T>; ++e) p[e] = e < dim ? from[e] : static_cast<T>(0.0f);
+    } else {
+        p = *reinterpret_cast<const typename Loose<T, kPiece<T>>::type*>(from);
+    }
+}
+
+template <typename T, bool SHORT>
+__device__ __forceinline__ void store_piece(T* to, const vec<T, kPiece<T>>& p, int dim) {
+    if constexpr (SHORT) {
+#pragma unroll
+        for (int e = 0; e < kPiece<T>; ++e)
+            if (e < dim) to[e] = p[e];
+    } else {
+        *reinterpret_cast<typename Loose<T, kPiece<T>>::type*>(to) = p;
+    }
+}
+
 // ---- lookup -------------------------------------------------------------------------------
 
 struct LookupArgs {
@@ -33,32 +67,47 @@ struct LookupArgs {
     float scale;
 };
 
-// A row of y is taken by `lanes` threads of a block, 16 bytes at a time.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void lookup_kernel(LookupArgs a, int lanes) {
-    constexpr int N = 16 / sizeof(T);
-    const int per_block = kThreads / lanes, lane = threadIdx.x % lanes;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * per_block;
-    for (int64_t t = static_cast<int64_t>(blockIdx.x) * per_block + threadIdx.x / lanes; t < a.tokens; t += step) {
-        const int64_t id = a.ids[t];
-        const int64_t place = !a.places ? 0 : a.place_ids ? a.place_ids[t] : t % a.period;
-        const bool inside = id >= 0 && id < a.vocab && (!a.places || (place >= 0 && place < a.places));
-        const T* w = static_cast<const T*>(a.weight) + (inside ? id : 0) * a.weight_stride;
-        const T* p = static_cast<const T*>(a.place_weight) + (inside ? place : 0) * a.places_stride;
-        T* y = static_cast<T*>(a.y) + t * a.dim;
-        for (int at = lane * N; at < a.dim; at += lanes * N) {
-            Pack<T, N> r, q;
-            if (inside) {
-                load_loose(r, w + at, a.dim - at);
-                if (a.places) load_loose(q, p + at, a.dim - at);
+// `lanes` threads of a block take K adjacent tokens at a time, whose ids and then whose rows are in flight together.
+template <typename T, bool PLACES, bool SHORT, int K, int THREADS>
+__device__ __forceinline__ void look_up(const LookupArgs& a, int lanes, int block, int blocks) {
+    constexpr int N = kPiece<T>;
+    const int per_block = THREADS / lanes, group = threadIdx.x / lanes, lane = threadIdx.x - group * lanes;
+    if (group >= per_block) return;
+    const int64_t step = static_cast<int64_t>(blocks) * per_block * K;
+    for (int64_t t = (static_cast<int64_t>(block) * per_block + group) * K; t < a.tokens; t += step) {
+        const T *w[K], *p[K];
+        bool inside[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int64_t token = std::min(t + k, a.tokens - 1);
+            const int64_t id = a.ids[token];
+            inside[k] = id >= 0 && id < a.vocab;
+            if constexpr (PLACES) {
+                const int64_t place = a.place_ids ? a.place_ids[token] : token % a.period;
+                inside[k] = inside[k] && place >= 0 && place < a.places;
+                p[k] = static_cast<const T*>(a.place_weight) + (inside[k] ? place * a.places_stride : 0);
+            }
+            w[k] = static_cast<const T*>(a.weight) + (inside[k] ? id * a.weight_stride : 0);
+        }
+        for (int column = lane * N; column < a.dim; column += lanes * N) {
+            const int at = piece_at<T, SHORT>(column, a.dim);
+            vec<T, N> r[K], q[K];
+#pragma unroll
+            for (int k = 0; k < K; ++k) {  // (a table without rows has nothing to read)
+                if (a.vocab) load_piece<T, SHORT>(r[k], w[k] + at, a.dim);
+                if constexpr (PLACES) load_piece<T, SHORT>(q[k], p[k] + at, a.dim);
             }
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                float x = a.scale * static_cast<float>(r.v[e]);
-                if (a.places) x = fmaf(a.scale, static_cast<float>(r.v[e]), static_cast<float>(q.v[e]));
-                r.v[e] = static_cast<T>(inside ? x : NAN);
+            for (int k = 0; k < K; ++k) {
+                if (t + k >= a.tokens) break;
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const float x = static_cast<float>(r[k][e]);
+                    const float y = PLACES ? fmaf(a.scale, x, static_cast<float>(q[k][e])) : a.scale * x;
+                    r[k][e] = static_cast<T>(inside[k] ? y : NAN);
+                }
+                store_piece<T, SHORT>(static_cast<T*>(a.y) + (t + k) * a.dim + at, r[k], a.dim);
             }
-            store_loose(y + at, r, a.dim - at);
         }
     }
 }
@@ -68,33 +117,78 @@ __global__ __launch_bounds__(kThreads) void lookup_kernel(LookupArgs a, int lane
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / kWave;
 constexpr int kSortRange = 512;  // rows of a block: 32 KiB of counters, so that blocks share a compute unit
-constexpr int kSortBlocks = 256;
+constexpr int kSortBlocks = 128;
+constexpr int kSortBatch = 8;  // keys of a lane in flight
+constexpr int kSortFound = 448;  // tokens of its range that a wave keeps: 28 KiB
+constexpr int kSortListed = (1 << 30) / kSortRange * 4;  // tokens of a wave that 32 bits number beside their rows
 
 struct SortArgs {
     const int64_t* keys;
-    int64_t tokens, rows, skip;
-    int range;
+    uint32_t skip;
+    int tokens, rows, range, blocks;
     int* order;   // [tokens]: tokens by row, then by their own place
     int* starts;  // [rows + 1]: where a row's begin in `order`
 };
 
-__global__ __launch_bounds__(kSortThreads) void sort_kernel(SortArgs a) {
-    __shared__ int counts[kSortWaves][kSortRange];
+// A key as a row, or one that no block has.
+__device__ __forceinline__ uint32_t row_of(int64_t key, const SortArgs& a) {
+    const uint32_t low = static_cast<uint32_t>(key), high = static_cast<uint32_t>(static_cast<uint64_t>(key) >> 32);
+    return high != 0 || low >= static_cast<uint32_t>(a.rows) || low == a.skip ? ~0u : low;
+}
+
+// The tokens of one step of a wave into their rows' lists: `local` is a token's row in the range, if inside.
+__device__ __forceinline__ void place_tokens(const SortArgs& a, int* next, uint32_t local, bool inside, int token, int lane) {
+    uint64_t left = __ballot(inside);
+    while (left) {  // once for each row that some lane's token has
+        const int leader = __builtin_ctzll(left);
+        const uint32_t which = __builtin_amdgcn_readlane(local, leader);
+        const uint64_t same = __ballot(inside && local == which);
+        int place = 0;
+        if (lane == leader) place = atomicAdd(&next[which], static_cast<int>(__popcll(same)));
+        place = __builtin_amdgcn_readlane(place, leader);
+        if (inside && local == which) a.order[place + __popcll(same & ((uint64_t{1} << lane) - 1))] = token;
+        left &= ~same;
+    }
+}
+
+__device__ void sort_range(const SortArgs& a, int block) {
+    __shared__ int counts[kSortWaves * kSortRange];
+    __shared__ uint32_t found[kSortWaves][kSortFound];
     __shared__ int sums[kSortWaves];
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const int64_t low = static_cast<int64_t>(blockIdx.x) * a.range;
-    const int range = static_cast<int>(std::min<int64_t>(a.range, a.rows - low));
-    for (int i = threadIdx.x; i < kSortWaves * kSortRange; i += kSortThreads) counts[i / kSortRange][i % kSortRange] = 0;
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t low = static_cast<uint32_t>(block) * a.range;
+    const uint32_t range = std::min<uint32_t>(a.range, a.rows - low);
+    for (uint32_t i = threadIdx.x; i < kSortWaves * range; i += kSortThreads) counts[i] = 0;
     __syncthreads();
+    int* mine = counts + wave * range;
     // a wave's tokens are adjacent ones
-    const int64_t each = ceil_div(ceil_div(a.tokens, kSortWaves), kWave) * kWave;
-    const int64_t from = wave * each, to = std::min<int64_t>(from + each, a.tokens);
-    int below = 0;
-    for (int64_t i = from + lane; i < to; i += kWave) {
-        const int64_t key = a.keys[i];
-        if (key < 0 || key >= a.rows || key == a.skip) continue;
-        if (key < low) ++below;
-        else if (key < low + range) atomicAdd(&counts[wave][key - low], 1);  // counts have one value in any order
+    const int each = static_cast<int>(ceil_div(ceil_div(a.tokens, kSortWaves), kWave) * kWave);
+    const int64_t from = static_cast<int64_t>(wave) * each;
+    const int n = static_cast<int>(std::max<int64_t>(0, std::min<int64_t>(each, a.tokens - from)));
+    const int64_t* keys = a.keys + from;
+    const uint64_t before_me = (uint64_t{1} << lane) - 1;
+    int below = 0, listed = 0;
+    for (int first = 0; first < n; first += kSortBatch * kWave) {
+        int64_t key[kSortBatch];
+#pragma unroll
+        for (int k = 0; k < kSortBatch; ++k) {
+            const int i = first + k * kWave + lane;
+            key[k] = i < n ? keys[i] : -1;
+        }
+#pragma unroll
+        for (int k = 0; k < kSortBatch; ++k) {
+            const uint32_t row = row_of(key[k], a), local = row - low;
+            const bool inside = local < range;
+            if (row < low) ++below;
+            if (const uint64_t mask = __ballot(inside)) {
+                const int at = listed + static_cast<int>(__popcll(mask & before_me));
+                if (inside) {
+                    atomicAdd(&mine[local], 1);  // counts have one value in any order
+                    if (at < kSortFound) found[wave][at] = static_cast<uint32_t>(first + k * kWave + lane) * kSortRange + local;
+                }
+                listed += static_cast<int>(__popcll(mask));
+            }
+        }
     }
 #pragma unroll
     for (int by = 1; by < kWave; by *= 2) below += __shfl_xor(below, by);
@@ -105,12 +199,12 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(SortArgs a) {
     for (int k = 0; k < kSortWaves; ++k) before += sums[k];
     __syncthreads();
     // where each row's tokens start, and in them each wave's
-    int mine = 0;
-    const int row = threadIdx.x;
+    const uint32_t row = threadIdx.x;
+    int count = 0;
     if (row < range)
 #pragma unroll
-        for (int k = 0; k < kSortWaves; ++k) mine += counts[k][row];
-    int scan = mine;
+        for (int k = 0; k < kSortWaves; ++k) count += counts[k * range + row];
+    int scan = count;
 #pragma unroll
     for (int by = 1; by < kWave; by *= 2) {
         const int other = __shfl_up(scan, by);
@@ -118,41 +212,64 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(SortArgs a) {
     }
     if (lane == kWave - 1) sums[wave] = scan;
     __syncthreads();
-    int at = before + scan - mine;
+    int at = before + scan - count;
 #pragma unroll
     for (int k = 0; k < kSortWaves; ++k)
         if (k < wave) at += sums[k];
     if (row < range) {
         a.starts[low + row] = at;
-        if (low + row == a.rows - 1) a.starts[a.rows] = at + mine;
+        if (low + row == static_cast<uint32_t>(a.rows) - 1) a.starts[a.rows] = at + count;
 #pragma unroll
         for (int k = 0; k < kSortWaves; ++k) {
-            const int n = counts[k][row];
-            counts[k][row] = at;
-            at += n;
+            const int c = counts[k * range + row];
+            counts[k * range + row] = at;
+            at += c;
         }
     }
     __syncthreads();
-    for (int64_t first = from; first < to; first += kWave) {
-        const int64_t i = first + lane;
-        const int64_t key = i < to ? a.keys[i] : -1;
-        const bool inside = key >= low && key < low + range && key != a.skip && key >= 0;
-        const int local = inside ? static_cast<int>(key - low) : -1;
-        uint64_t left = __ballot(inside);
-        while (left) {  // once for each row that some lane's token has
-            const int leader = __builtin_ctzll(left);
-            const int which = __shfl(local, leader);
-            const uint64_t same = __ballot(local == which);
-            int place = 0;
-            if (lane == leader) place = atomicAdd(&counts[wave][which], static_cast<int>(__popcll(same)));
-            place = __shfl(place, leader);
-            if (local == which) a.order[place + __popcll(same & ((uint64_t{1} << lane) - 1))] = static_cast<int>(i);
-            left &= ~same;
+    // the tokens that were found, in their order, or all keys again where those did not fit
+    if (listed <= kSortFound && n <= kSortListed) {
+        for (int i = lane; i - lane < listed; i += kWave) {
+            const bool inside = i < listed;
+            const uint32_t f = inside ? found[wave][i] : 0;
+            place_tokens(a, mine, f % kSortRange, inside, static_cast<int>(from) + static_cast<int>(f / kSortRange), lane);
+        }
+        return;
+    }
+    for (int first = 0; first < n; first += kSortBatch * kWave) {
+        int64_t key[kSortBatch];
+#pragma unroll
+        for (int k = 0; k < kSortBatch; ++k) {
+            const int i = first + k * kWave + lane;
+            key[k] = i < n ? keys[i] : -1;
+        }
+#pragma unroll
+        for (int k = 0; k < kSortBatch; ++k) {
+            const uint32_t local = row_of(key[k], a) - low;
+            place_tokens(a, mine, local, local < range, static_cast<int>(from) + first + k * kWave + lane, lane);
         }
     }
 }
 
+// The lookup and, for a backward pass, both tables' sorts: they need the ids alone, and their few blocks, whose time
+// is latency, run beside the lookup's: two blocks of 1024 threads share a compute unit, hence at most 64 registers.
+// THREADS 256: a lookup without sorts.
+template <typename T, bool PLACES, bool SHORT, int K, int THREADS>
+__global__ __launch_bounds__(THREADS, THREADS == kSortThreads ? 8 : 1) void lookup_kernel(LookupArgs a, int lanes, SortArgs first, SortArgs second) {
+    int block = static_cast<int>(blockIdx.x), blocks = static_cast<int>(gridDim.x);
+    if constexpr (THREADS == kSortThreads) {
+        if (block < first.blocks) return sort_range(first, block);
+        block -= first.blocks;
+        if (block < second.blocks) return sort_range(second, block);
+        block -= second.blocks;
+        blocks -= first.blocks + second.blocks;
+    }
+    look_up<T, PLACES, SHORT, K, THREADS>(a, lanes, block, blocks);
+}
+
 // ---- sums -----------------------------------------------------------------------------------
+
+constexpr int kJoinThreads = 512, kJoinTiles = 4;
 
 struct SumArgs {
     const int64_t* keys;        // null: key_t = t mod period
@@ -160,162 +277,369 @@ struct SumArgs {
     const void* dy;
     void* grad;
     float* partial;  // [tiles][2][dim]
-    int64_t tokens, rows, period, tiles;
-    int dim, tile;
+    int* joins;      // [tiles]: the row longer than a tile that starts in a tile, or -1
+    int rows, period, times;  // without keys: tokens / period
+    int dim, tile, tiles;
+    int each;                // rows of a group of lanes
+    int tile_blocks, blocks;  // of the tiles, in all
     float scale;
 };
 
 // The list of tokens sorted by row: as sorted, or known where keys count 0 .. period - 1 again and again.
-__device__ __forceinline__ int64_t start_of(const SumArgs& a, int64_t row) {
-    return a.starts ? a.starts[row] : std::min(row, a.period) * (a.tokens / a.period);
+__device__ __forceinline__ int start_of(const SumArgs& a, int row) {
+    return a.starts ? a.starts[row] : std::min(row, a.period) * a.times;
 }
-__device__ __forceinline__ int64_t token_at(const SumArgs& a, int64_t place) {
+__device__ __forceinline__ int token_at(const SumArgs& a, int place) {
     if (a.order) return a.order[place];
-    const int64_t times = a.tokens / a.period;
-    return place % times * a.period + place / times;
+    return place % a.times * a.period + place / a.times;
 }
-__device__ __forceinline__ int64_t row_at(const SumArgs& a, int64_t place) {
-    return a.order ? a.keys[a.order[place]] : place / (a.tokens / a.period);
+__device__ __forceinline__ int row_at(const SumArgs& a, int place) {
+    return a.order ? static_cast<int>(a.keys[a.order[place]]) : place / a.times;
 }
 
-template <typename T, int N>
-__device__ __forceinline__ void add_rows(const SumArgs& a, int64_t from, int64_t to, int at, float (&sum)[N]) {
-    const T* dy = static_cast<const T*>(a.dy) + at;
-    const int left = a.dim - at;
-#pragma unroll 4
-    for (int64_t i = from; i < to; ++i) {
-        Pack<T, N> p;
-        load_loose(p, dy + token_at(a, i) * a.dim, left);
+// `from`'s value in a group of LANES lanes: uniform in a wave where that is the group.
+template <int LANES>
+__device__ __forceinline__ int lane_value(int x, int from) {
+    if constexpr (LANES == kWave) return __builtin_amdgcn_readlane(x, from);
+    return __shfl(x, from, LANES);
+}
+
+// A group of LANES lanes, whose lanes hold C pieces of a row each, LANES apart. (Lanes past a row's end read its
+// last piece, too, and write nothing.)
+template <typename T, int LANES, int C, bool SHORT>
+struct Group {
+    static constexpr int N = kPiece<T>;
+    static constexpr int kBatch = C <= 2 ? 8 : 4;  // rows in flight
+    const SumArgs& a;
+    int lane, first;  // lane of the group, column of its first piece
+    int at[C];        // where its pieces start
+    int base, token;  // the tokens of places base .. base + LANES - 1, one a lane
+    float sum[C][N];
+
+    __device__ Group(const SumArgs& args, int columns) : a(args), lane(threadIdx.x % LANES), base(-LANES - 1), token(0) {
+        first = columns + lane * N;
 #pragma unroll
-        for (int e = 0; e < N; ++e) sum[e] += static_cast<float>(p.v[e]);
+        for (int c = 0; c < C; ++c) at[c] = piece_at<T, SHORT>(first + c * LANES * N, a.dim);
     }
-}
-
-template <typename T, int N>
-__device__ __forceinline__ void store_sum(const SumArgs& a, int64_t row, int at, const float (&sum)[N]) {
-    Pack<T, N> p;
+    __device__ void clear() {
 #pragma unroll
-    for (int e = 0; e < N; ++e) p.v[e] = static_cast<T>(a.scale * sum[e]);
-    store_loose(static_cast<T*>(a.grad) + row * a.dim + at, p, a.dim - at);
-}
-
-// Rows of at most a tile's tokens: `lanes` threads a row.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void row_sum_kernel(SumArgs a, int lanes) {
-    constexpr int N = 16 / sizeof(T);
-    const int per_block = kThreads / lanes, lane = threadIdx.x % lanes;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * per_block;
-    for (int64_t v = static_cast<int64_t>(blockIdx.x) * per_block + threadIdx.x / lanes; v < a.rows; v += step) {
-        const int64_t from = start_of(a, v), to = start_of(a, v + 1);
-        if (to - from > a.tile) continue;
-        for (int at = lane * N; at < a.dim; at += lanes * N) {
-            float sum[N] = {};
-            add_rows<T>(a, from, to, at, sum);
-            store_sum<T>(a, v, at, sum);
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum[c][e] = 0.0f;
+    }
+    // rows [place, place + K) of the list, of which the group's lanes know the tokens
+    template <int K>
+    __device__ __forceinline__ void add_batch(int place) {
+        vec<T, N> p[K][C];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int64_t t = lane_value<LANES>(token, place - base + k);
+            const T* row = static_cast<const T*>(a.dy) + t * a.dim;
+#pragma unroll
+            for (int c = 0; c < C; ++c) load_piece<T, SHORT>(p[k][c], row + at[c], a.dim);
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int e = 0; e < N; ++e) sum[c][e] += static_cast<float>(p[k][c][e]);
+    }
+    __device__ __forceinline__ void add(int from, int to, int end) {
+        for (int i = from; i < to; i += kBatch) {
+            const int n = std::min(kBatch, to - i);
+            if (i < base || i + n > base + LANES) {  // places up to `end`, which later calls may want
+                base = i;
+                token = i + lane < end ? token_at(a, i + lane) : 0;
+            }
+            if (n == kBatch) {
+                add_batch<kBatch>(i);
+                continue;
+            }
+            int done = 0;
+            if (kBatch > 4 && n & 4) add_batch<4>(i), done = 4;
+            if (n & 2) add_batch<2>(i + done), done += 2;
+            if (n & 1) add_batch<1>(i + done);
         }
     }
-}
+    __device__ void store(int row) const {
+        T* out = static_cast<T*>(a.grad) + static_cast<int64_t>(row) * a.dim;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            if (first + c * LANES * N >= a.dim) break;
+            vec<T, N> p;
+#pragma unroll
+            for (int e = 0; e < N; ++e) p[e] = static_cast<T>(a.scale * sum[c][e]);
+            store_piece<T, SHORT>(out + at[c], p, a.dim);
+        }
+    }
+    __device__ void store_partial(int64_t slot) const {
+        float* out = a.partial + slot * a.dim;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            if (first + c * LANES * N >= a.dim) break;
+#pragma unroll
+            for (int h = 0; h < N; h += 4) {
+                vec<float, 4> p;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[e] = sum[c][h + e];
+                if constexpr (SHORT) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (h + e < a.dim) out[h + e] = p[e];
+                } else {
+                    *reinterpret_cast<Loose<float, 4>::type*>(out + at[c] + h) = p;
+                }
+            }
+        }
+    }
+};
 
 // A tile of the sorted list: its parts of rows longer than a tile, of which it meets two at most (one that ends
 // in it and one that starts in it).
-template <typename T>
-__global__ __launch_bounds__(kThreads) void tile_sum_kernel(SumArgs a) {
-    constexpr int N = 16 / sizeof(T);
-    const int64_t total = start_of(a, a.rows), k = blockIdx.x;
-    const int64_t from = k * a.tile, to = std::min<int64_t>(from + a.tile, total);
-    if (from >= to) return;
-    const int64_t first = row_at(a, from), last = row_at(a, to - 1);
-    for (int part = 0; part < 2; ++part) {
-        const int64_t row = part ? last : first;
-        if (part && last == first) return;
-        const int64_t s = start_of(a, row), e = start_of(a, row + 1);
-        if (e - s <= a.tile) continue;
-        float* out = a.partial + (2 * k + part) * a.dim;
-        for (int at = (blockIdx.y * kThreads + threadIdx.x) * N; at < a.dim; at += gridDim.y * kThreads * N) {
-            float sum[N] = {};
-            add_rows<T>(a, std::max(s, from), std::min(e, to), at, sum);
+template <typename T, int LANES, int C, bool SHORT>
+__device__ __forceinline__ void sum_tile(const SumArgs& a, int k, int columns) {
+    Group<T, LANES, C, SHORT> g(a, columns);
+    const int total = start_of(a, a.rows);
+    const int from = k * a.tile, to = std::min(from + a.tile, total);
+    int join = -1;
+    if (from < to) {
+        const int ends[2] = {row_at(a, from), row_at(a, to - 1)};
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (at + i < a.dim) out[at + i] = sum[i];
+        for (int part = 0; part < 2; ++part) {
+            const int row = ends[part];
+            if (part && row == ends[0]) break;
+            const int s = start_of(a, row), e = start_of(a, row + 1);
+            if (e - s <= a.tile) continue;
+            if (s >= from) join = row;
+            g.clear();
+            g.add(std::max(s, from), std::min(e, to), to);
+            g.store_partial(2 * static_cast<int64_t>(k) + part);
         }
+    }
+    if (g.lane == 0 && columns == 0) a.joins[k] = join;
+}
+
+// Rows of at most a tile's tokens, `each` adjacent ones: where they start is one load, and so are their tokens.
+template <typename T, int LANES, int C, bool SHORT>
+__device__ __forceinline__ void sum_rows(const SumArgs& a, int row, int columns) {
+    Group<T, LANES, C, SHORT> g(a, columns);
+    const int n = std::min(a.each, a.rows - row);
+    if (n <= 0) return;
+    const int start = start_of(a, row + std::min(g.lane, n));
+    const int end = lane_value<LANES>(start, n);
+    for (int r = 0; r < n; ++r) {
+        const int s = lane_value<LANES>(start, r), e = lane_value<LANES>(start, r + 1);
+        if (e - s > a.tile) continue;
+        g.clear();
+        g.add(s, e, end);
+        g.store(row + r);
     }
 }
 
-// The row longer than a tile that starts in tile k, if there is one: the sum of its tiles' sums. A block takes 64
-// columns, its waves every 16th tile.
+// The first blocks take tiles, which have the longest walks, the others rows.
+template <typename T, int LANES, int C, bool SHORT>
+__global__ __launch_bounds__(kThreads) void sum_kernel(SumArgs first, SumArgs second) {
+    constexpr int kGroups = kThreads / LANES;
+    int block = static_cast<int>(blockIdx.x);
+    const bool other = block >= first.blocks;
+    if (other) block -= first.blocks;
+    const SumArgs& a = other ? second : first;
+    const int columns = static_cast<int>(blockIdx.y) * LANES * C * kPiece<T>;
+    int group = threadIdx.x / LANES;
+    if constexpr (LANES == kWave) group = __builtin_amdgcn_readfirstlane(group);
+    if (block < a.tile_blocks) {
+        const int k = block * kGroups + group;
+        if (k < a.tiles) sum_tile<T, LANES, C, SHORT>(a, k, columns);
+    } else {
+        const int64_t row = (static_cast<int64_t>(block - a.tile_blocks) * kGroups + group) * a.each;
+        if (row < a.rows) sum_rows<T, LANES, C, SHORT>(a, static_cast<int>(row), columns);
+    }
+}
+
+// Rows longer than a tile, those that start in a block's tiles: the sum of their tiles' sums. A block takes 256
+// columns, its waves every eighth tile.
 template <typename T>
-__global__ __launch_bounds__(kSortThreads) void tile_join_kernel(SumArgs a) {
-    __shared__ float sums[kSortWaves][kWave];
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(SumArgs first, SumArgs second, int first_blocks) {
+    constexpr int kWaves = kJoinThreads / kWave, N = 4;
+    __shared__ float sums[kWaves][kWave * N];
+    int block = static_cast<int>(blockIdx.x);
+    const bool other = block >= first_blocks;
+    if (other) block -= first_blocks;
+    const SumArgs& a = other ? second : first;
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const int64_t total = start_of(a, a.rows), k = blockIdx.x;
-    const int64_t from = k * a.tile, to = std::min<int64_t>(from + a.tile, total);
-    if (from >= to) return;
-    const int64_t row = row_at(a, to - 1), s = start_of(a, row), e = start_of(a, row + 1);
-    if (e - s <= a.tile || s < from) return;
-    const int64_t last = (e - 1) / a.tile;
-    for (int first = blockIdx.y * kWave; first < a.dim; first += gridDim.y * kWave) {
-        const int at = first + lane;
-        float sum = 0.0f;
-        if (at < a.dim)
-            for (int64_t t = k + wave; t <= last; t += kSortWaves)
-                sum += a.partial[(2 * t + (t == k && s > from ? 1 : 0)) * a.dim + at];
-        sums[wave][lane] = sum;
-        __syncthreads();
-        if (wave == 0 && at < a.dim) {
-            sum = 0.0f;
+    const int mine = block * kJoinTiles + lane < a.tiles && lane < kJoinTiles ? a.joins[block * kJoinTiles + lane] : -1;
+    for (uint64_t left = __ballot(mine >= 0); left; left &= left - 1) {
+        const int at = __builtin_ctzll(left), k = block * kJoinTiles + at;
+        const int row = __builtin_amdgcn_readlane(mine, at);
+        const int s = start_of(a, row), last = (start_of(a, row + 1) - 1) / a.tile;
+        for (int columns = static_cast<int>(blockIdx.y) * kWave * N; columns < a.dim;
+             columns += static_cast<int>(gridDim.y) * kWave * N) {
+            const int c = columns + lane * N;
+            float sum[N] = {};
+#pragma unroll 4
+            for (int t = k + wave; t <= last; t += kWaves) {
+                // (the row's first tile holds it second where another row ends in it)
+                const int64_t slot = 2 * static_cast<int64_t>(t) + (t == k && s > k * a.tile ? 1 : 0);
+                Pack<float, N> p;
+                load_loose(p, a.partial + slot * a.dim + c, a.dim - c);
 #pragma unroll
-            for (int w = 0; w < kSortWaves; ++w) sum += sums[w][lane];
-            static_cast<T*>(a.grad)[row * a.dim + at] = static_cast<T>(a.scale * sum);
+                for (int e = 0; e < N; ++e) sum[e] += p.v[e];
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e) sums[wave][e * kWave + lane] = sum[e];
+            __syncthreads();
+            if (wave == 0) {
+                Pack<T, N> p;
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    float all = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < kWaves; ++w) all += sums[w][e * kWave + lane];
+                    p.v[e] = static_cast<T>(a.scale * all);
+                }
+                store_loose(static_cast<T*>(a.grad) + static_cast<int64_t>(row) * a.dim + c, p, a.dim - c);
+            }
+            __syncthreads();
         }
-        __syncthreads();
     }
 }
 
 // ---- host -----------------------------------------------------------------------------------
 
-// Threads of a row of `chunks` 16-byte pieces: a power of two, the whole block at most.
-int lanes_of(int64_t chunks) {
-    int lanes = 8;
-    while (lanes < kThreads && lanes < chunks) lanes *= 2;
-    return lanes;
-}
-
-// A tile's tokens: 64, and more where that would make more than 2048 tiles, whose sums are added up.
-int tile_of(int64_t tokens) { return static_cast<int>(std::max<int64_t>(64, ceil_div(tokens, 2048))); }
-// No row is longer than a tile where there are no more tokens.
-int64_t tiles_of(int64_t tokens) { return tokens > tile_of(tokens) ? ceil_div(tokens, tile_of(tokens)) : 0; }
+// A tile's tokens: 16, and more where that would make more than 2048 tiles, whose sums are added up.
+int tile_of(int64_t tokens) { return static_cast<int>(std::max<int64_t>(16, ceil_div(tokens, 2048))); }
 
 constexpr int64_t kMaxTokens = int64_t{1} << 30, kMaxDim = int64_t{1} << 24;
 
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
+// One table's parts of the lists that a lookup leaves and of a backward call's workspace.
 struct Space {
-    size_t starts, partial, bytes;
-    Space(int64_t tokens, int64_t rows, int64_t dim, bool has_keys) {
-        starts = has_keys ? rounded(tokens * sizeof(int)) : 0;
-        partial = starts + (has_keys ? rounded((rows + 1) * sizeof(int)) : 0);
-        bytes = partial + static_cast<size_t>(tiles_of(tokens)) * 2 * dim * sizeof(float);
+    int64_t tiles;
+    size_t starts, lists;         // bytes before the lists' starts, in all
+    size_t partial, workspace;    // bytes before the partial sums, in all
+    Space(int64_t tokens, int64_t rows, int64_t dim, bool keys, int64_t period) {
+        const int tile = tile_of(tokens);
+        // no row is longer than a tile where there are no more tokens; without keys all have one length
+        tiles = tokens > tile && (keys || tokens / period > tile) ? ceil_div(tokens, tile) : 0;
+        starts = keys ? rounded(tokens * sizeof(int)) : 0;
+        lists = starts + (keys ? rounded((rows + 1) * sizeof(int)) : 0);
+        partial = rounded(tiles * sizeof(int));
+        workspace = partial + rounded(static_cast<size_t>(tiles) * 2 * dim * sizeof(float));
     }
 };
 
-bool sizes_fit(int64_t tokens, int64_t rows, int64_t dim) {
-    return tokens >= 0 && tokens <= kMaxTokens && rows >= 0 && rows <= ISA_TRAIN_EMBEDDING_MAX_ROWS && dim >= 1 &&
-           dim <= kMaxDim;
+int check(const isa_train_embedding* e) {
+    if (!e) return fail("embedding is null");
+    if (!known_type(e->type)) return fail("unknown element type %d", e->type);
+    if (e->tokens < 0 || e->tokens > kMaxTokens || e->vocab < 0 || e->vocab > ISA_TRAIN_EMBEDDING_MAX_ROWS ||
+        e->places < 0 || e->places > ISA_TRAIN_EMBEDDING_MAX_ROWS || e->dim < 1 || e->dim > kMaxDim)
+        return fail("sizes out of range: tokens %lld, tables of %lld and %lld rows, dim %lld",
+                    static_cast<long long>(e->tokens), static_cast<long long>(e->vocab),
+                    static_cast<long long>(e->places), static_cast<long long>(e->dim));
+    if (e->tokens && !e->ids) return fail("ids must be set");
+    if (e->tokens && e->places && !e->place_ids && (e->period < 1 || e->tokens % e->period))
+        return fail("period must divide the tokens, got %lld", static_cast<long long>(e->period));
+    return 0;
+}
+
+Space space_of(const isa_train_embedding* e, bool places) {
+    if (!places) return Space(e->tokens, e->vocab, e->dim, true, 1);
+    return Space(e->tokens, e->places, e->dim, e->place_ids != nullptr, e->tokens ? e->period : 1);
+}
+
+// Rows of a group: so many that some 8192 groups of 64 lanes take them all, at most the lanes that know where they
+// start.
+int rows_each(int64_t rows, int lanes, int64_t across) {
+    return static_cast<int>(std::min<int64_t>(lanes - 1, std::max<int64_t>(1, ceil_div(rows * across * lanes, 8192 * kWave))));
+}
+
+struct Jobs {
+    SumArgs sum[2];
+};
+
+template <typename T, int LANES, int C, bool SHORT = false>
+int launch_sums(Jobs& j, hipStream_t s) {
+    constexpr int N = kPiece<T>, kGroups = kThreads / LANES;
+    const int64_t dim = std::max(j.sum[0].dim, j.sum[1].dim), across = ceil_div(dim, LANES * C * N);
+    for (SumArgs& a : j.sum) {
+        if (a.rows == 0) continue;
+        a.each = rows_each(a.rows, LANES, across);
+        a.tile_blocks = static_cast<int>(ceil_div(a.tiles, kGroups));
+        a.blocks = a.tile_blocks + static_cast<int>(ceil_div(ceil_div(a.rows, a.each), kGroups));
+    }
+    // a grid's second dimension ends at 65535: 2^24 columns of fp32 are 16384 times 64 lanes of 4
+    const dim3 grid(static_cast<unsigned>(j.sum[0].blocks + j.sum[1].blocks), static_cast<unsigned>(across));
+    sum_kernel<T, LANES, C, SHORT><<<grid, dim3(kThreads), 0, s>>>(j.sum[0], j.sum[1]);
+    if (int rc = launched("sum_kernel")) return rc;
+    const int64_t blocks[2] = {ceil_div(j.sum[0].tiles, kJoinTiles), ceil_div(j.sum[1].tiles, kJoinTiles)};
+    if (blocks[0] + blocks[1] == 0) return 0;
+    const dim3 joins(static_cast<unsigned>(blocks[0] + blocks[1]),
+                     static_cast<unsigned>(std::min<int64_t>(ceil_div(dim, kWave * 4), 1024)));
+    join_kernel<T><<<joins, dim3(kJoinThreads), 0, s>>>(j.sum[0], j.sum[1], static_cast<int>(blocks[0]));
+    return launched("join_kernel");
+}
+
+// Lanes of a group and chunks of a lane: a row's columns, at most 256 chunks at a time.
+template <typename T>
+int sums(Jobs& j, int64_t dim, hipStream_t s) {
+    const int64_t chunks = ceil_div(dim, static_cast<int64_t>(kPiece<T>));
+    if (dim < kPiece<T>) return launch_sums<T, 8, 1, true>(j, s);
+    if (chunks <= 8) return launch_sums<T, 8, 1>(j, s);
+    if (chunks <= 16) return launch_sums<T, 16, 1>(j, s);
+    if (chunks <= 32) return launch_sums<T, 32, 1>(j, s);
+    if (chunks <= 64) return launch_sums<T, 64, 1>(j, s);
+    if (chunks <= 128) return launch_sums<T, 64, 2>(j, s);
+    if (chunks <= 192) return launch_sums<T, 64, 3>(j, s);
+    return launch_sums<T, 64, 4>(j, s);
+}
+
+// The sorts of a table's tokens into its part of the lists.
+SortArgs sort_of(const isa_train_embedding* e, bool places, int64_t skip, char* lists) {
+    SortArgs o{};
+    const int64_t rows = places ? e->places : e->vocab;
+    o.keys = places ? e->place_ids : e->ids;
+    o.skip = places || skip < 0 || skip >= rows ? ~0u : static_cast<uint32_t>(skip);
+    o.tokens = static_cast<int>(e->tokens);
+    o.rows = static_cast<int>(rows);
+    o.range = static_cast<int>(std::min<int64_t>(ceil_div(rows, kSortBlocks), kSortRange));
+    o.blocks = rows ? static_cast<int>(ceil_div(rows, o.range)) : 0;
+    o.order = reinterpret_cast<int*>(lists);
+    o.starts = reinterpret_cast<int*>(lists + space_of(e, places).starts);
+    return o;
+}
+
+template <typename T, bool PLACES, bool SHORT, int K>
+void launch_lookup(const LookupArgs& a, const SortArgs (&sorts)[2], int lanes, hipStream_t s) {
+    const int others = sorts[0].blocks + sorts[1].blocks, threads = others ? kSortThreads : kThreads;
+    const int64_t blocks = std::min<int64_t>(ceil_div(ceil_div(a.tokens, K), threads / lanes), kMaxBlocks) + others;
+    const dim3 grid(static_cast<unsigned>(blocks)), block(threads);
+    if (others) lookup_kernel<T, PLACES, SHORT, K, kSortThreads><<<grid, block, 0, s>>>(a, lanes, sorts[0], sorts[1]);
+    else lookup_kernel<T, PLACES, SHORT, K, kThreads><<<grid, block, 0, s>>>(a, lanes, sorts[0], sorts[1]);
+}
+
+// Four tokens at a time where that leaves work for every compute unit.
+template <typename T, bool PLACES>
+void launch_lookup(const LookupArgs& a, const SortArgs (&sorts)[2], hipStream_t s) {
+    const int64_t pieces = ceil_div(a.dim, static_cast<int64_t>(kPiece<T>));
+    // a lane has one piece of a row, or as many as the others where a block of 256 has fewer lanes
+    const int lanes = static_cast<int>(ceil_div(pieces, ceil_div(pieces, kThreads)));
+    if (a.dim < kPiece<T>) return launch_lookup<T, PLACES, true, 1>(a, sorts, lanes, s);
+    if (a.tokens * lanes >= 4 * 1024 * kThreads) return launch_lookup<T, PLACES, false, PLACES ? 2 : 4>(a, sorts, lanes, s);
+    launch_lookup<T, PLACES, false, 1>(a, sorts, lanes, s);
 }
 
 template <typename T>
-int sums(const SumArgs& a, hipStream_t s) {
-    const int lanes = lanes_of(ceil_div(a.dim, 16 / sizeof(T)));
-    const int64_t blocks = std::min<int64_t>(ceil_div(a.rows, kThreads / lanes), kMaxBlocks);
-    row_sum_kernel<T><<<dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, s>>>(a, lanes);
-    if (int rc = launched("row_sum_kernel")) return rc;
-    if (!a.tiles) return 0;
-    const auto across = [&](int64_t each) { return static_cast<unsigned>(std::min<int64_t>(ceil_div(a.dim, each), 1024)); };
-    const unsigned tiles = static_cast<unsigned>(a.tiles);
-    tile_sum_kernel<T><<<dim3(tiles, across(kThreads * 16 / sizeof(T))), dim3(kThreads), 0, s>>>(a);
-    if (int rc = launched("tile_sum_kernel")) return rc;
-    tile_join_kernel<T><<<dim3(tiles, across(kWave)), dim3(kSortThreads), 0, s>>>(a);
-    return launched("tile_join_kernel");
+void launch_lookup(const LookupArgs& a, const SortArgs (&sorts)[2], hipStream_t s) {
+    if (a.places) launch_lookup<T, true>(a, sorts, s);
+    else launch_lookup<T, false>(a, sorts, s);
+}
+
+int check_lists(const void* lists, size_t bytes, size_t has) {
+    if (has < bytes) return fail("lists too small: %zu bytes", has);
+    if (bytes && (!lists || !aligned(lists, 256))) return fail("lists must be 256-byte aligned");
+    return 0;
 }
 
 }  // namespace
@@ -325,77 +649,100 @@ using namespace isa_block;
 
 extern "C" int isa_train_abi_version(void) { return ISA_TRAIN_ABI_VERSION; }
 
-extern "C" int isa_train_embedding_forward(const isa_train_embedding* e, void* y, void* stream) {
-    if (!e) return fail("embedding is null");
-    if (!known_type(e->type)) return fail("unknown element type %d", e->type);
-    if (!sizes_fit(e->tokens, e->vocab, e->dim) || e->places < 0 || e->places > ISA_TRAIN_EMBEDDING_MAX_ROWS)
-        return fail("sizes out of range: tokens %lld, tables of %lld and %lld rows, dim %lld",
-                    static_cast<long long>(e->tokens), static_cast<long long>(e->vocab),
-                    static_cast<long long>(e->places), static_cast<long long>(e->dim));
-    if (e->tokens == 0) return 0;
-    if (!e->ids || !y || (e->vocab && !e->weight)) return fail("ids, weight and y must be set");
-    if (e->places && !e->place_weight) return fail("place_weight must be set");
-    if (e->places && !e->place_ids && (e->period < 1 || e->tokens % e->period))
-        return fail("period must divide the tokens, got %lld", static_cast<long long>(e->period));
+extern "C" size_t isa_train_embedding_lists(const isa_train_embedding* e, int weight, int places) {
+    if (check(e)) return 0;
+    return (weight ? space_of(e, false).lists : 0) + (places ? space_of(e, true).lists : 0);
+}
+
+extern "C" int isa_train_embedding_forward(const isa_train_embedding* e, void* y, int weight, int places, int64_t skip,
+                                           void* lists, size_t lists_bytes, void* stream) {
+    if (int rc = check(e)) return rc;
+    if (e->tokens && (!y || (e->vocab && !e->weight))) return fail("weight and y must be set");
+    if (e->tokens && e->places && !e->place_weight) return fail("place_weight must be set");
     const size_t b = type_bytes(e->type);
     if (!aligned(y, b) || !aligned(e->weight, b) || (e->places && !aligned(e->place_weight, b)))
         return fail("y or a table is not aligned to its type");
-    const LookupArgs a{e->ids,           e->place_ids, e->weight, e->place_weight, y, e->tokens, e->vocab, e->weight_stride, e->places,
-                       e->places_stride, e->period,    static_cast<int>(e->dim), e->scale};
-    const int lanes = lanes_of(ceil_div(e->dim, static_cast<int64_t>(16 / b)));
-    const int64_t blocks = std::min<int64_t>(ceil_div(e->tokens, kThreads / lanes), kMaxBlocks);
-    const dim3 grid(static_cast<unsigned>(blocks));
+    if (int rc = check_lists(lists, isa_train_embedding_lists(e, weight, places), lists_bytes)) return rc;
+    SortArgs sorts[2] = {};
+    char* list = static_cast<char*>(lists);
+    if (weight) {
+        sorts[0] = sort_of(e, false, skip, list);
+        list += space_of(e, false).lists;
+    }
+    if (places && e->place_ids) sorts[1] = sort_of(e, true, -1, list);
+    if (e->tokens == 0 && sorts[0].blocks + sorts[1].blocks == 0) return 0;
+    const LookupArgs a{e->ids,
+                       e->place_ids,
+                       e->weight,
+                       e->place_weight,
+                       y,
+                       e->tokens,
+                       e->vocab,
+                       e->weight_stride,
+                       e->places,
+                       e->places_stride,
+                       e->period,
+                       static_cast<int>(e->dim),
+                       e->scale};
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (e->type == ISA_BLOCK_F32) lookup_kernel<float><<<grid, dim3(kThreads), 0, s>>>(a, lanes);
-    else if (e->type == ISA_BLOCK_BF16) lookup_kernel<bf16><<<grid, dim3(kThreads), 0, s>>>(a, lanes);
-    else lookup_kernel<f16><<<grid, dim3(kThreads), 0, s>>>(a, lanes);
+    if (e->type == ISA_BLOCK_F32) launch_lookup<float>(a, sorts, s);
+    else if (e->type == ISA_BLOCK_BF16) launch_lookup<bf16>(a, sorts, s);
+    else launch_lookup<f16>(a, sorts, s);
     return launched("lookup_kernel");
 }
 
-extern "C" size_t isa_train_embedding_backward_workspace(int64_t tokens, int64_t rows, int64_t dim, int has_keys) {
-    return sizes_fit(tokens, rows, dim) ? Space(tokens, rows, dim, has_keys != 0).bytes : 0;
+extern "C" size_t isa_train_embedding_backward_workspace(const isa_train_embedding* e, int weight, int places) {
+    if (check(e)) return 0;
+    return (weight ? space_of(e, false).workspace : 0) + (places ? space_of(e, true).workspace : 0);
 }
 
-extern "C" int isa_train_embedding_backward(int type, int64_t tokens, int64_t rows, int64_t dim, const int64_t* keys,
-                                            int64_t period, int64_t skip, float scale, const void* dy, void* grad,
-                                            void* workspace, size_t workspace_bytes, void* stream) {
-    if (!known_type(type)) return fail("unknown element type %d", type);
-    if (!sizes_fit(tokens, rows, dim))
-        return fail("sizes out of range: tokens %lld, rows %lld, dim %lld", static_cast<long long>(tokens),
-                    static_cast<long long>(rows), static_cast<long long>(dim));
-    if (rows == 0) return 0;
-    if (!grad || (tokens && !dy)) return fail("grad_y and grad must be set");
-    if (!aligned(grad, type_bytes(type)) || !aligned(dy, type_bytes(type)))
-        return fail("grad_y or grad is not aligned to its type");
-    if (tokens && !keys && (period < 1 || tokens % period))
-        return fail("period must divide the tokens, got %lld", static_cast<long long>(period));
-    const bool has_keys = keys && tokens;
-    const Space at(tokens, rows, dim, has_keys);
-    if (workspace_bytes < at.bytes) return fail("workspace too small: %zu bytes", workspace_bytes);
-    if (at.bytes && (!workspace || !aligned(workspace, 256))) return fail("workspace must be 256-byte aligned");
-    const hipStream_t s = static_cast<hipStream_t>(stream);
+extern "C" int isa_train_embedding_backward(const isa_train_embedding* e, const void* lists, size_t lists_bytes,
+                                            const void* dy, void* dweight, void* dplaces, int listed_weight,
+                                            int listed_places, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int rc = check(e)) return rc;
+    if ((dweight && !listed_weight) || (dplaces && !listed_places)) return fail("a gradient's table has no lists");
+    if (int rc = check_lists(lists, isa_train_embedding_lists(e, listed_weight, listed_places), lists_bytes)) return rc;
+    if (e->tokens && (dweight || dplaces) && !dy) return fail("grad_y must be set");
+    const size_t b = type_bytes(e->type);
+    if (!aligned(dy, b) || !aligned(dweight, b) || !aligned(dplaces, b)) return fail("a gradient is not aligned to its type");
+    const size_t bytes = isa_train_embedding_backward_workspace(e, dweight != nullptr, dplaces != nullptr);
+    if (workspace_bytes < bytes) return fail("workspace too small: %zu bytes", workspace_bytes);
+    if (bytes && (!workspace || !aligned(workspace, 256))) return fail("workspace must be 256-byte aligned");
+    if (e->vocab == 0) dweight = nullptr;
+    if (e->places == 0) dplaces = nullptr;
+    if (!dweight && !dplaces) return 0;
+    Jobs j{};
+    const char* list = static_cast<const char*>(lists);
     char* ws = static_cast<char*>(workspace);
-    SumArgs a{};
-    if (has_keys) {
-        SortArgs b{keys, tokens, rows, skip, 0, reinterpret_cast<int*>(ws), reinterpret_cast<int*>(ws + at.starts)};
-        b.range = static_cast<int>(std::min<int64_t>(ceil_div(rows, kSortBlocks), kSortRange));
-        sort_kernel<<<dim3(static_cast<unsigned>(ceil_div(rows, b.range))), dim3(kSortThreads), 0, s>>>(b);
-        if (int rc = launched("sort_kernel")) return rc;
-        a.keys = keys;
-        a.order = b.order;
-        a.starts = b.starts;
+    for (int k = 0; k < 2; ++k) {
+        void* grad = k ? dplaces : dweight;
+        const Space at = space_of(e, k == 1);
+        if (grad) {
+            SumArgs& a = j.sum[k];
+            const int64_t* keys = k ? e->place_ids : e->ids;
+            a.rows = static_cast<int>(k ? e->places : e->vocab);
+            if (at.lists) {
+                a.keys = keys;
+                a.order = reinterpret_cast<const int*>(list);
+                a.starts = reinterpret_cast<const int*>(list + at.starts);
+            } else {
+                a.period = static_cast<int>(e->tokens ? e->period : 1);
+                a.times = static_cast<int>(e->tokens / a.period);
+            }
+            a.dy = dy;
+            a.grad = grad;
+            a.joins = reinterpret_cast<int*>(ws);
+            a.partial = reinterpret_cast<float*>(ws + at.partial);
+            a.tiles = static_cast<int>(at.tiles);
+            a.dim = static_cast<int>(e->dim);
+            a.tile = tile_of(e->tokens);
+            a.scale = k ? 1.0f : e->scale;
+            ws += at.workspace;
+        }
+        if (k ? listed_places : listed_weight) list += at.lists;
     }
-    a.dy = dy;
-    a.grad = grad;
-    a.partial = reinterpret_cast<float*>(ws + at.partial);
-    a.tokens = tokens;
-    a.rows = rows;
-    a.period = has_keys || !tokens ? 1 : period;
-    a.tiles = tiles_of(tokens);
-    a.dim = static_cast<int>(dim);
-    a.tile = tile_of(tokens);
-    a.scale = scale;
-    if (type == ISA_BLOCK_F32) return sums<float>(a, s);
-    if (type == ISA_BLOCK_BF16) return sums<bf16>(a, s);
-    return sums<f16>(a, s);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (e->type == ISA_BLOCK_F32) return sums<float>(j, e->dim, s);
+    if (e->type == ISA_BLOCK_BF16) return sums<bf16>(j, e->dim, s);
+    return sums<f16>(j, e->dim, s);
 }

@@ -50,54 +50,56 @@ struct Lookup {
 
 int64_t period_of(const Tensor& ids) { return ids.dim() ? std::max<int64_t>(ids.size(-1), 1) : 1; }
 
-Tensor lookup(const Tensor& weight, const Tensor& places, const Lookup& how) {
+isa_train_embedding embedding_of(const Lookup& how, int type, int64_t dim, int64_t vocab, int64_t places) {
+    isa_train_embedding e{};
+    e.type = type;
+    e.tokens = how.ids.numel();
+    e.dim = dim;
+    e.vocab = vocab;
+    e.ids = static_cast<const int64_t*>(how.ids.data_ptr());
+    e.scale = static_cast<float>(how.scale);
+    e.places = places;
+    e.place_ids = static_cast<const int64_t*>(pointer(how.place_ids));
+    e.period = period_of(how.ids);
+    return e;
+}
+
+// y and, for a backward call, the lists of the tables that learn.
+std::tuple<Tensor, Tensor> lookup(const Tensor& weight, const Tensor& places, const Lookup& how, bool learns,
+                                  bool places_learn) {
     const c10::DeviceGuard guard(weight.device());
     const Tensor w = rows_of(weight), p = places.defined() ? rows_of(places) : Tensor();
-    isa_train_embedding e{};
-    e.type = type_of(w);
-    e.tokens = how.ids.numel();
-    e.dim = w.size(1);
-    e.vocab = w.size(0);
-    e.weight_stride = w.stride(0);
-    e.ids = static_cast<const int64_t*>(how.ids.data_ptr());
+    isa_train_embedding e = embedding_of(how, type_of(w), w.size(1), w.size(0), p.defined() ? p.size(0) : 0);
     e.weight = w.data_ptr();
-    e.scale = static_cast<float>(how.scale);
+    e.weight_stride = w.stride(0);
     if (p.defined()) {
-        e.places = p.size(0);
-        e.places_stride = p.stride(0);
-        e.place_ids = static_cast<const int64_t*>(pointer(how.place_ids));
-        e.period = period_of(how.ids);
         e.place_weight = p.data_ptr();
+        e.places_stride = p.stride(0);
     }
     std::vector<int64_t> shape = how.ids.sizes().vec();
     shape.push_back(e.dim);
     Tensor y = at::empty(shape, weight.options());
-    check(isa_train_embedding_forward(&e, y.data_ptr(), stream_of(w)), "isa_train_embedding_forward");
-    return y;
-}
-
-// The gradient of a table shaped as `rows` x dy's last dimension.
-Tensor table_gradient(const Tensor& dy, int64_t rows, const Tensor& keys, int64_t period, int64_t skip, double scale) {
-    const int64_t dim = dy.size(-1), tokens = dy.numel() / dim;
-    Tensor grad = at::empty({rows, dim}, dy.options());
-    const Tensor workspace = bytes(isa_train_embedding_backward_workspace(tokens, rows, dim, keys.defined()), dy);
-    check(isa_train_embedding_backward(type_of(dy), tokens, rows, dim, static_cast<const int64_t*>(pointer(keys)), period,
-                                       skip, static_cast<float>(scale), dy.data_ptr(), grad.data_ptr(), pointer(workspace),
-                                       workspace.defined() ? workspace.numel() : 0, stream_of(dy)),
-          "isa_train_embedding_backward");
-    return grad;
+    const Tensor lists = bytes(isa_train_embedding_lists(&e, learns, places_learn), w);
+    check(isa_train_embedding_forward(&e, y.data_ptr(), learns, places_learn, how.padding, pointer(lists),
+                                      lists.defined() ? lists.numel() : 0, stream_of(w)),
+          "isa_train_embedding_forward");
+    return {y, lists};
 }
 
 struct Embedding : torch::autograd::Function<Embedding> {
     static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& ids, const Maybe& places,
                           const Maybe& place_ids, double scale, int64_t padding) {
         const Lookup how{ids, place_ids.value_or(Tensor()), scale, padding};
-        ctx->save_for_backward({ids, how.place_ids});
+        const bool learns = weight.requires_grad(), places_learn = places && places->requires_grad();
+        auto [y, lists] = lookup(weight, places.value_or(Tensor()), how, learns, places_learn);
+        ctx->save_for_backward({ids, how.place_ids, lists});
+        ctx->saved_data["learns"] = learns;
+        ctx->saved_data["places_learn"] = places_learn;
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["padding"] = padding;
         ctx->saved_data["rows"] = weight.size(0);
         ctx->saved_data["places"] = places ? places->size(0) : int64_t{-1};
-        return lookup(weight, places.value_or(Tensor()), how);
+        return y;
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -106,12 +108,19 @@ struct Embedding : torch::autograd::Function<Embedding> {
         const Tensor dy = packed(grads[0]);
         const c10::DeviceGuard guard(dy.device());
         const int64_t places = ctx->saved_data["places"].toInt();
+        const Lookup how{s[0], s[1], ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt()};
+        const isa_train_embedding e =
+            embedding_of(how, type_of(dy), dy.size(-1), ctx->saved_data["rows"].toInt(), std::max<int64_t>(places, 0));
         Tensor dw, dp;
-        if (ctx->needs_input_grad(0))
-            dw = table_gradient(dy, ctx->saved_data["rows"].toInt(), s[0], 1, ctx->saved_data["padding"].toInt(),
-                                ctx->saved_data["scale"].toDouble());
+        if (ctx->needs_input_grad(0)) dw = at::empty({e.vocab, e.dim}, dy.options());
         // counted over the tensors that were there
-        if (places >= 0 && ctx->needs_input_grad(2)) dp = table_gradient(dy, places, s[1], period_of(s[0]), -1, 1.0);
+        if (places >= 0 && ctx->needs_input_grad(2)) dp = at::empty({places, e.dim}, dy.options());
+        const Tensor workspace = bytes(isa_train_embedding_backward_workspace(&e, dw.defined(), dp.defined()), dy);
+        check(isa_train_embedding_backward(&e, pointer(s[2]), s[2].defined() ? s[2].numel() : 0, dy.data_ptr(), pointer(dw),
+                                           pointer(dp), ctx->saved_data["learns"].toBool(),
+                                           ctx->saved_data["places_learn"].toBool(), pointer(workspace),
+                                           workspace.defined() ? workspace.numel() : 0, stream_of(dy)),
+              "isa_train_embedding_backward");
         return {dw, Tensor(), dp, Tensor(), Tensor(), Tensor()};
     }
 };
@@ -148,7 +157,7 @@ Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, const Ma
     if (recorded({&weight, &places}))
         return Embedding::apply(weight, tokens, position_weight, place_ids.defined() ? Maybe(place_ids) : Maybe(), scale,
                                 padding);
-    return lookup(weight, places, {tokens, place_ids, scale, padding});
+    return std::get<0>(lookup(weight, places, {tokens, place_ids, scale, padding}, false, false));
 }
 
 // ---- dropout --------------------------------------------------------------------------------
