@@ -25,7 +25,7 @@ struct alignas(sizeof(T) * N) Pack {
 
 constexpr int kWave = 64;
 
-// N elements as one load or store at any element's address; of `left` < N elements, one by one.
+// N elements as one load or store at any element's address; `left` < N of them one by one.
 template <typename T, int N>
 struct Loose {
     typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));

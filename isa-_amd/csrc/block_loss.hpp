@@ -44,6 +44,7 @@ struct LossArgs {
     float* logp;      // [rows]
     float* row_slope;  // [rows], or null
     double* row_logp;  // [rows], or null: l, 0 in ignored rows
+    bool count_here;   // each block counts the rows that are not ignored, for its gradient
 };
 
 // What a row's loss is of its l.
@@ -69,6 +70,14 @@ __device__ __forceinline__ float block_sum(float x, float* slots) {
 #pragma unroll
     for (int k = 0; k < THREADS / kWave; ++k) x += slots[k];
     return x;
+}
+
+// The rows that are not ignored, by a block (a float: exact to 2^24 rows, which the rows' number is held to).
+template <int THREADS>
+__device__ __forceinline__ float block_count(const int64_t* targets, int64_t rows, int64_t ignore, float* slots) {
+    float n = 0.0f;
+    for (int64_t r = threadIdx.x; r < rows; r += THREADS) n += targets[r] != ignore ? 1.0f : 0.0f;
+    return block_sum<THREADS>(n, slots);
 }
 
 // A row as 16-byte chunks at aligned addresses: chunk c holds elements c N - skip and on. The
@@ -170,11 +179,13 @@ __global__ __launch_bounds__(THREADS) void loss_kernel(LossArgs a) {
     using R = Row<T>;
     constexpr int N = R::N;
     __shared__ float slots[2][THREADS / kWave];
+    [[maybe_unused]] __shared__ float count_slots[OF == Of::kPolicy ? THREADS / kWave : 1];
     const int64_t r = block_row();
     if (r >= a.rows) return;  // (a whole block)
     const R row(static_cast<const T*>(a.logits) + r * a.stride, a.vocab);
     const int chunks = row.chunks();
     const int64_t target = a.targets[r];
+    [[maybe_unused]] float count = 1.0f;
     T* grad = a.grad ? static_cast<T*>(a.grad) + r * a.grad_stride : nullptr;
     if (target == a.ignore) {
         if (threadIdx.x == 0) {
@@ -202,6 +213,8 @@ __global__ __launch_bounds__(THREADS) void loss_kernel(LossArgs a) {
 #pragma unroll
                 for (int e = 0; e < N; ++e) held[i].v[e] = low;
         }
+        if constexpr (OF == Of::kPolicy)  // while the row is on its way
+            if (a.count_here) count = block_count<THREADS>(a.targets, a.rows, a.ignore, count_slots);
 #pragma unroll
         for (int i = 0; i < C; ++i)
 #pragma unroll
@@ -213,6 +226,8 @@ __global__ __launch_bounds__(THREADS) void loss_kernel(LossArgs a) {
             for (int e = 0; e < N; ++e)
                 sum += __builtin_amdgcn_exp2f((static_cast<float>(held[i].v[e]) - top) * kLog2E);
     } else {
+        if constexpr (OF == Of::kPolicy)
+            if (a.count_here) count = block_count<THREADS>(a.targets, a.rows, a.ignore, count_slots);
         for (int c = threadIdx.x; c < chunks; c += THREADS) {
             typename R::Chunk x;
             row.load(x, c, low);
@@ -258,7 +273,7 @@ __global__ __launch_bounds__(THREADS) void loss_kernel(LossArgs a) {
     }
     if (!grad) return;
     float share = inside ? share_of(a, r) : NAN;
-    if constexpr (OF == Of::kPolicy) share *= -slope;
+    if constexpr (OF == Of::kPolicy) share *= -slope / count;
     const float factor = share / sum;
     const int hot = inside ? static_cast<int>(target) : -1;
     if constexpr (C > 0) {
@@ -302,13 +317,10 @@ __global__ __launch_bounds__(THREADS) void loss_backward_kernel(LossArgs a) {
     }
 }
 
-// The rows that count, as a float (exact to 2^24 rows; the rows' number is held to that).
 __global__ __launch_bounds__(kMostThreads) void loss_count_kernel(const int64_t* targets, int64_t rows, int64_t ignore,
                                                               float* count) {
     __shared__ float slots[kMostThreads / kWave];
-    float n = 0.0f;
-    for (int64_t r = threadIdx.x; r < rows; r += kMostThreads) n += targets[r] != ignore ? 1.0f : 0.0f;
-    n = block_sum<kMostThreads>(n, slots);
+    const float n = block_count<kMostThreads>(targets, rows, ignore, slots);
     if (threadIdx.x == 0) count[0] = n;
 }
 
@@ -319,6 +331,17 @@ __global__ __launch_bounds__(kMostThreads) void loss_sum_kernel(const float* row
     for (int64_t r = threadIdx.x; r < rows; r += kMostThreads) s += row_loss[r];
     s = block_sum<kMostThreads>(s, slots);
     if (threadIdx.x == 0) out[0] = count ? s / count[0] : s;
+}
+
+// The mean over the rows that are not ignored, which are counted here.
+__global__ __launch_bounds__(kMostThreads) void loss_mean_kernel(const float* row_loss, const int64_t* targets,
+                                                             int64_t rows, int64_t ignore, float* out) {
+    __shared__ float slots[2][kMostThreads / kWave];
+    float s = 0.0f;
+    for (int64_t r = threadIdx.x; r < rows; r += kMostThreads) s += row_loss[r];
+    const float n = block_count<kMostThreads>(targets, rows, ignore, slots[0]);
+    s = block_sum<kMostThreads>(s, slots[1]);
+    if (threadIdx.x == 0) out[0] = s / n;
 }
 
 template <typename T, int C, int THREADS, Of OF>

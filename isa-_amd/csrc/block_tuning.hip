@@ -10,6 +10,14 @@ namespace {
 
 constexpr int kPairThreads = 256;
 
+// Up to so many rows each row's block counts those that are not ignored: 8 KiB of targets, read beside its logits,
+// instead of a launch before (a call of 1023 x 5003 in bf16: 10.7 us, with the launch 13.8; of 2048 x 5003 17.0 and 16.3).
+constexpr int64_t kCountHere = 1024;
+
+// Up to so many rows one block takes all pairs and their sum (a call of 8192 x 5003 in bf16: 52.2 us, with a block a
+// pair and one for the sum 53.8; of 16384 x 1000 in 32 pairs 45.6 and 40.9).
+constexpr int64_t kPairsHere = 8192;
+
 struct PairArgs {
     const double* row_logp;  // [2 pairs][tokens]
     const float* ref;
@@ -18,50 +26,78 @@ struct PairArgs {
     float beta;
 };
 
-__device__ __forceinline__ double sequence_sum(const double* rows, int64_t n, double* slots) {
-    double s = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += kPairThreads) s += rows[i];
-    slots[threadIdx.x] = s;
-    __syncthreads();
-    for (int half = kPairThreads / 2; half; half /= 2) {
-        if (static_cast<int>(threadIdx.x) < half) slots[threadIdx.x] += slots[threadIdx.x + half];
-        __syncthreads();
-    }
-    return slots[0];
+__device__ __forceinline__ double wave_sum64(double x) {
+#pragma unroll
+    for (int by = 1; by < kWave; by *= 2) x += __shfl_xor(x, by);
+    return x;
 }
 
+// A pair's loss and slopes from the sums of its sequences.
+__device__ __forceinline__ float pair_loss(const PairArgs& a, int64_t p, double chosen, double other) {
+    const double m = a.beta * ((chosen - a.ref[p]) - (other - a.ref[a.pairs + p]));
+    const double slope = -a.beta / (1.0 + exp(m));
+    a.logp[p] = static_cast<float>(chosen);
+    a.logp[a.pairs + p] = static_cast<float>(other);
+    if (a.slope) {
+        a.slope[p] = static_cast<float>(slope);
+        a.slope[a.pairs + p] = static_cast<float>(-slope);
+    }
+    return static_cast<float>((m < 0.0 ? -m : 0.0) + log1p(exp(-fabs(m))));
+}
+
+template <int THREADS>
+__device__ __forceinline__ double block_sum64(double x, double* slots) {
+    x = wave_sum64(x);
+    if (threadIdx.x % kWave == 0) slots[threadIdx.x / kWave] = x;
+    __syncthreads();
+    x = 0.0;
+    for (int k = 0; k < THREADS / kWave; ++k) x += slots[k];
+    return x;
+}
+
+// A block a pair.
 __global__ __launch_bounds__(kPairThreads) void preference_pair_kernel(PairArgs a) {
-    __shared__ double slots[2][kPairThreads];
+    __shared__ double slots[2][kPairThreads / kWave];
     for (int64_t p = blockIdx.x; p < a.pairs; p += gridDim.x) {
-        const double chosen = sequence_sum(a.row_logp + p * a.tokens, a.tokens, slots[0]);
-        const double other = sequence_sum(a.row_logp + (a.pairs + p) * a.tokens, a.tokens, slots[1]);
-        if (threadIdx.x == 0) {
-            const double m = a.beta * ((chosen - a.ref[p]) - (other - a.ref[a.pairs + p]));
-            const double slope = -a.beta / (1.0 + exp(m));
-            a.loss[p] = static_cast<float>((m < 0.0 ? -m : 0.0) + log1p(exp(-fabs(m))));
-            a.logp[p] = static_cast<float>(chosen);
-            a.logp[a.pairs + p] = static_cast<float>(other);
-            if (a.slope) {
-                a.slope[p] = static_cast<float>(slope);
-                a.slope[a.pairs + p] = static_cast<float>(-slope);
-            }
+        double sums[2];
+        for (int k = 0; k < 2; ++k) {
+            const double* rows = a.row_logp + (k * a.pairs + p) * a.tokens;
+            double s = 0.0;
+            for (int64_t i = threadIdx.x; i < a.tokens; i += kPairThreads) s += rows[i];
+            sums[k] = block_sum64<kPairThreads>(s, slots[k]);
         }
+        if (threadIdx.x == 0) a.loss[p] = pair_loss(a, p, sums[0], sums[1]);
         __syncthreads();
     }
+}
+
+// All pairs, a wave each, and the sum or mean of their losses.
+__global__ __launch_bounds__(kMostThreads) void preference_pairs_kernel(PairArgs a, int mean, float* out) {
+    __shared__ double slots[kMostThreads / kWave];
+    const int lane = threadIdx.x % kWave;
+    double all = 0.0;
+    for (int64_t p = threadIdx.x / kWave; p < a.pairs; p += kMostThreads / kWave) {
+        double sums[2];
+        for (int k = 0; k < 2; ++k) {
+            const double* rows = a.row_logp + (k * a.pairs + p) * a.tokens;
+            double s = 0.0;
+#pragma unroll 8
+            for (int64_t i = lane; i < a.tokens; i += kWave) s += rows[i];
+            sums[k] = wave_sum64(s);
+        }
+        if (lane == 0) all += pair_loss(a, p, sums[0], sums[1]);
+    }
+    all = block_sum64<kMostThreads>(all, slots);
+    if (threadIdx.x == 0) out[0] = static_cast<float>(mean ? all / a.pairs : all);
 }
 
 __global__ __launch_bounds__(kPairThreads) void preference_sum_kernel(const float* loss, int64_t pairs, int mean,
                                                                       float* out) {
-    __shared__ double slots[kPairThreads];
+    __shared__ double slots[kPairThreads / kWave];
     double s = 0.0;
     for (int64_t i = threadIdx.x; i < pairs; i += kPairThreads) s += loss[i];
-    slots[threadIdx.x] = s;
-    __syncthreads();
-    for (int half = kPairThreads / 2; half; half /= 2) {
-        if (static_cast<int>(threadIdx.x) < half) slots[threadIdx.x] += slots[threadIdx.x + half];
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) out[0] = static_cast<float>(mean ? slots[0] / pairs : slots[0]);
+    s = block_sum64<kPairThreads>(s, slots);
+    if (threadIdx.x == 0) out[0] = static_cast<float>(mean ? s / pairs : s);
 }
 
 int check(const isa_train_policy* p) {
@@ -113,18 +149,25 @@ int check_workspace(const isa_train_preference* p, const void* workspace, size_t
     return 0;
 }
 
-// l of rows, sequences' sums, losses and slopes of pairs.
-int run_pairs(const isa_train_preference* p, float* stats, float* pair_loss, float* logp, float* slope,
+// l of rows, sequences' sums, losses and slopes of pairs, and unless out is null their losses' sum or mean.
+int run_pairs(const isa_train_preference* p, float* stats, float* losses, float* logp, float* slope, int mean, float* out,
               void* workspace, hipStream_t s) {
     LossArgs a = args_of(&p->loss);
     a.row_logp = static_cast<double*>(workspace);
     a.stats = stats;
     if (p->loss.rows) run_rows<Of::kCrossEntropy>(p->loss.type, a, s);
     if (int rc = launched("loss_kernel")) return rc;
-    const PairArgs b{a.row_logp, p->ref_logp, p->pairs, p->tokens, pair_loss, logp, slope, p->beta};
+    const PairArgs b{a.row_logp, p->ref_logp, p->pairs, p->tokens, losses, logp, slope, p->beta};
+    if (out && p->loss.rows <= kPairsHere && p->pairs <= kPairsHere) {
+        preference_pairs_kernel<<<1, kMostThreads, 0, s>>>(b, mean, out);
+        return launched("preference_pairs_kernel");
+    }
     const int64_t blocks = std::min<int64_t>(p->pairs, 4096);
     if (blocks) preference_pair_kernel<<<dim3(static_cast<unsigned>(blocks)), dim3(kPairThreads), 0, s>>>(b);
-    return launched("preference_pair_kernel");
+    if (int rc = launched("preference_pair_kernel")) return rc;
+    if (!out) return 0;
+    preference_sum_kernel<<<1, kPairThreads, 0, s>>>(losses, p->pairs, mean, out);
+    return launched("preference_sum_kernel");
 }
 
 int run_pairs_backward(const isa_train_preference* p, const float* stats, const float* slope, const float* by, int step,
@@ -213,18 +256,24 @@ extern "C" int isa_train_policy_with_grad(const isa_train_policy* p, float grad_
     if (int rc = check_workspace(l, workspace, workspace_bytes)) return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     float* ws = static_cast<float*>(workspace);
-    loss_count_kernel<<<1, kMostThreads, 0, s>>>(l->targets, l->rows, l->ignore_index, ws);
-    if (int rc = launched("loss_count_kernel")) return rc;
     LossArgs a = args_of(p);
+    a.count_here = l->rows <= kCountHere;
+    if (!a.count_here) {
+        loss_count_kernel<<<1, kMostThreads, 0, s>>>(l->targets, l->rows, l->ignore_index, ws);
+        if (int rc = launched("loss_count_kernel")) return rc;
+        a.count = ws;
+    }
     a.row_loss = ws + 64;
     a.logp = logp;
-    a.count = ws;
     a.scale = grad_scale;
     a.grad = grad;
     a.grad_stride = grad_stride;
     if (l->rows) run_rows<Of::kPolicy>(l->type, a, s);
     if (int rc = launched("loss_kernel")) return rc;
-    loss_sum_kernel<<<1, kMostThreads, 0, s>>>(ws + 64, l->rows, ws, out);
+    if (a.count_here)
+        loss_mean_kernel<<<1, kMostThreads, 0, s>>>(ws + 64, l->targets, l->rows, l->ignore_index, out);
+    else
+        loss_sum_kernel<<<1, kMostThreads, 0, s>>>(ws + 64, l->rows, ws, out);
     return launched("loss_sum_kernel");
 }
 
@@ -243,11 +292,9 @@ extern "C" int isa_train_preference_forward(const isa_train_preference* p, int r
     if (int rc = check_workspace(p, workspace, workspace_bytes)) return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     char* ws = static_cast<char*>(workspace);
-    float* pair_loss = reduction == ISA_BLOCK_NONE ? out : reinterpret_cast<float*>(ws + PreferenceSpace(p).loss);
-    if (int rc = run_pairs(p, stats, pair_loss, logp, slope, ws, s)) return rc;
-    if (reduction == ISA_BLOCK_NONE) return 0;
-    preference_sum_kernel<<<1, kPairThreads, 0, s>>>(pair_loss, p->pairs, reduction == ISA_BLOCK_MEAN, out);
-    return launched("preference_sum_kernel");
+    float* losses = reduction == ISA_BLOCK_NONE ? out : reinterpret_cast<float*>(ws + PreferenceSpace(p).loss);
+    return run_pairs(p, stats, losses, logp, slope, reduction == ISA_BLOCK_MEAN,
+                     reduction == ISA_BLOCK_NONE ? nullptr : out, ws, s);
 }
 
 extern "C" int isa_train_preference_backward(const isa_train_preference* p, int reduction, const float* stats,
@@ -273,11 +320,9 @@ extern "C" int isa_train_preference_with_grad(const isa_train_preference* p, flo
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const PreferenceSpace at(p);
     char* ws = static_cast<char*>(workspace);
-    float *stats = reinterpret_cast<float*>(ws + at.stats), *pair_loss = reinterpret_cast<float*>(ws + at.loss),
+    float *stats = reinterpret_cast<float*>(ws + at.stats), *losses = reinterpret_cast<float*>(ws + at.loss),
           *slope = reinterpret_cast<float*>(ws + at.slope);
-    if (int rc = run_pairs(p, stats, pair_loss, logp, slope, ws, s)) return rc;
-    preference_sum_kernel<<<1, kPairThreads, 0, s>>>(pair_loss, p->pairs, 1, out);
-    if (int rc = launched("preference_sum_kernel")) return rc;
+    if (int rc = run_pairs(p, stats, losses, logp, slope, 1, out, ws, s)) return rc;
     if (p->loss.rows == 0) return 0;
     return run_pairs_backward(p, stats, slope, nullptr, 0, grad_scale / static_cast<float>(p->pairs), grad, grad_stride, s);
 }
