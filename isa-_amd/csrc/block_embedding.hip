@@ -269,7 +269,7 @@ __global__ __launch_bounds__(THREADS, THREADS == kSortThreads ? 8 : 1) void look
 
 // ---- sums -----------------------------------------------------------------------------------
 
-constexpr int kJoinThreads = 512, kJoinTiles = 4;
+constexpr int kJoinThreads = 512, kJoinTiles = 4, kFewThreads = 1024;
 
 struct SumArgs {
     const int64_t* keys;        // null: key_t = t mod period
@@ -313,10 +313,12 @@ struct Group {
     const SumArgs& a;
     int lane, first;  // lane of the group, column of its first piece
     int at[C];        // where its pieces start
-    int base, token;  // the tokens of places base .. base + LANES - 1, one a lane
+    int end;          // of the places that it may add
+    int base, token;  // the tokens of places base .. base + LANES - 1 up to the end, one a lane
     float sum[C][N];
 
-    __device__ Group(const SumArgs& args, int columns) : a(args), lane(threadIdx.x % LANES), base(-LANES - 1), token(0) {
+    __device__ Group(const SumArgs& args, int columns, int places_end)
+        : a(args), lane(threadIdx.x % LANES), end(places_end), base(-LANES - 1), token(0) {
         first = columns + lane * N;
 #pragma unroll
         for (int c = 0; c < C; ++c) at[c] = piece_at<T, SHORT>(first + c * LANES * N, a.dim);
@@ -345,10 +347,10 @@ struct Group {
 #pragma unroll
                 for (int e = 0; e < N; ++e) sum[c][e] += static_cast<float>(p[k][c][e]);
     }
-    __device__ __forceinline__ void add(int from, int to, int end) {
+    __device__ __forceinline__ void add(int from, int to) {
         for (int i = from; i < to; i += kBatch) {
             const int n = std::min(kBatch, to - i);
-            if (i < base || i + n > base + LANES) {  // places up to `end`, which later calls may want
+            if (i < base || i + n > base + LANES) {
                 base = i;
                 token = i + lane < end ? token_at(a, i + lane) : 0;
             }
@@ -399,9 +401,8 @@ struct Group {
 // in it and one that starts in it).
 template <typename T, int LANES, int C, bool SHORT>
 __device__ __forceinline__ void sum_tile(const SumArgs& a, int k, int columns) {
-    Group<T, LANES, C, SHORT> g(a, columns);
-    const int total = start_of(a, a.rows);
-    const int from = k * a.tile, to = std::min(from + a.tile, total);
+    const int from = k * a.tile, to = std::min(from + a.tile, start_of(a, a.rows));
+    Group<T, LANES, C, SHORT> g(a, columns, to);
     int join = -1;
     if (from < to) {
         const int ends[2] = {row_at(a, from), row_at(a, to - 1)};
@@ -413,34 +414,78 @@ __device__ __forceinline__ void sum_tile(const SumArgs& a, int k, int columns) {
             if (e - s <= a.tile) continue;
             if (s >= from) join = row;
             g.clear();
-            g.add(std::max(s, from), std::min(e, to), to);
+            g.add(std::max(s, from), std::min(e, to));
             g.store_partial(2 * static_cast<int64_t>(k) + part);
         }
     }
     if (g.lane == 0 && columns == 0) a.joins[k] = join;
 }
 
-// Rows of at most a tile's tokens, `each` adjacent ones: where they start is one load, and so are their tokens.
+// Rows of at most a tile's tokens, `each` adjacent ones: where they start is one load, and so are their tokens. Returns
+// which of them were longer.
 template <typename T, int LANES, int C, bool SHORT>
-__device__ __forceinline__ void sum_rows(const SumArgs& a, int row, int columns) {
-    Group<T, LANES, C, SHORT> g(a, columns);
-    const int n = std::min(a.each, a.rows - row);
-    if (n <= 0) return;
-    const int start = start_of(a, row + std::min(g.lane, n));
-    const int end = lane_value<LANES>(start, n);
+__device__ __forceinline__ uint64_t sum_rows(const SumArgs& a, int64_t row, int columns) {
+    const int n = static_cast<int>(std::min<int64_t>(a.each, a.rows - row));
+    if (n <= 0) return 0;
+    const int start = start_of(a, static_cast<int>(row) + std::min<int>(threadIdx.x % LANES, n));
+    Group<T, LANES, C, SHORT> g(a, columns, lane_value<LANES>(start, n));
+    uint64_t longer = 0;
     for (int r = 0; r < n; ++r) {
         const int s = lane_value<LANES>(start, r), e = lane_value<LANES>(start, r + 1);
-        if (e - s > a.tile) continue;
+        if (e - s > a.tile) {
+            longer |= uint64_t{1} << r;
+            continue;
+        }
         g.clear();
-        g.add(s, e, end);
-        g.store(row + r);
+        g.add(s, e);
+        g.store(static_cast<int>(row) + r);
+    }
+    return longer;
+}
+
+// The longer rows of a block's groups, by all of its groups: each a part of a row's tokens, added up in LDS.
+template <typename T, int LANES, int C, bool SHORT>
+__device__ __forceinline__ void sum_longer(const SumArgs& a, int64_t first_row, uint64_t longer, int columns) {
+    constexpr int kGroups = kFewThreads / LANES, N = kPiece<T>;
+    __shared__ uint64_t masks[kGroups];
+    __shared__ float sums[kGroups][C * N][LANES];
+    const int group = threadIdx.x / LANES;
+    Group<T, LANES, C, SHORT> g(a, columns, start_of(a, a.rows));
+    if (g.lane == 0) masks[group] = longer;
+    __syncthreads();
+    for (int k = 0; k < kGroups; ++k) {
+        for (uint64_t left = masks[k]; left; left &= left - 1) {
+            const int row = static_cast<int>(first_row) + k * a.each + __builtin_ctzll(left);
+            const int s = start_of(a, row), e = start_of(a, row + 1), part = static_cast<int>(ceil_div(e - s, kGroups));
+            const int from = s + group * part;
+            g.clear();
+            g.add(from, std::min(from + part, e));
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < N; ++i) sums[group][c * N + i][g.lane] = g.sum[c][i];
+            __syncthreads();
+            if (group == 0) {
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        float all = 0.0f;
+                        for (int w = 0; w < kGroups; ++w) all += sums[w][c * N + i][g.lane];
+                        g.sum[c][i] = all;
+                    }
+                g.store(row);
+            }
+            __syncthreads();
+        }
     }
 }
 
-// The first blocks take tiles, which have the longest walks, the others rows.
-template <typename T, int LANES, int C, bool SHORT>
-__global__ __launch_bounds__(kThreads) void sum_kernel(SumArgs first, SumArgs second) {
-    constexpr int kGroups = kThreads / LANES;
+// FEW tokens: rows alone, the longer ones by a whole block, and nothing is left to join. Else the first blocks take
+// tiles, which have the longest walks, the others rows.
+template <typename T, int LANES, int C, bool SHORT, bool FEW>
+__global__ __launch_bounds__(FEW ? kFewThreads : kThreads, FEW ? 4 : 1) void sum_kernel(SumArgs first, SumArgs second) {
+    constexpr int kGroups = (FEW ? kFewThreads : kThreads) / LANES;
     int block = static_cast<int>(blockIdx.x);
     const bool other = block >= first.blocks;
     if (other) block -= first.blocks;
@@ -448,13 +493,14 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(SumArgs first, SumArgs se
     const int columns = static_cast<int>(blockIdx.y) * LANES * C * kPiece<T>;
     int group = threadIdx.x / LANES;
     if constexpr (LANES == kWave) group = __builtin_amdgcn_readfirstlane(group);
-    if (block < a.tile_blocks) {
+    if (!FEW && block < a.tile_blocks) {
         const int k = block * kGroups + group;
         if (k < a.tiles) sum_tile<T, LANES, C, SHORT>(a, k, columns);
-    } else {
-        const int64_t row = (static_cast<int64_t>(block - a.tile_blocks) * kGroups + group) * a.each;
-        if (row < a.rows) sum_rows<T, LANES, C, SHORT>(a, static_cast<int>(row), columns);
+        return;
     }
+    const int64_t row = static_cast<int64_t>(block - a.tile_blocks) * kGroups * a.each;
+    const uint64_t longer = sum_rows<T, LANES, C, SHORT>(a, row + group * a.each, columns);
+    if constexpr (FEW) sum_longer<T, LANES, C, SHORT>(a, row, longer, columns);
 }
 
 // Rows longer than a tile, those that start in a block's tiles: the sum of their tiles' sums. A block takes 256
@@ -510,6 +556,9 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(SumArgs first, SumAr
 // A tile's tokens: 16, and more where that would make more than 2048 tiles, whose sums are added up.
 int tile_of(int64_t tokens) { return static_cast<int>(std::max<int64_t>(16, ceil_div(tokens, 2048))); }
 
+// So many need no tiles: a row of all of them is a walk of 128 tokens for each wave of a block, and a launch less.
+constexpr int64_t kFewTokens = 2048;
+
 constexpr int64_t kMaxTokens = int64_t{1} << 30, kMaxDim = int64_t{1} << 24;
 
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -521,8 +570,8 @@ struct Space {
     size_t partial, workspace;    // bytes before the partial sums, in all
     Space(int64_t tokens, int64_t rows, int64_t dim, bool keys, int64_t period) {
         const int tile = tile_of(tokens);
-        // no row is longer than a tile where there are no more tokens; without keys all have one length
-        tiles = tokens > tile && (keys || tokens / period > tile) ? ceil_div(tokens, tile) : 0;
+        // of few tokens a row's block takes longer ones; without keys all rows have one length
+        tiles = tokens > kFewTokens && (keys || tokens / period > tile) ? ceil_div(tokens, tile) : 0;
         starts = keys ? rounded(tokens * sizeof(int)) : 0;
         lists = starts + (keys ? rounded((rows + 1) * sizeof(int)) : 0);
         partial = rounded(tiles * sizeof(int));
@@ -559,9 +608,9 @@ struct Jobs {
     SumArgs sum[2];
 };
 
-template <typename T, int LANES, int C, bool SHORT = false>
+template <typename T, int LANES, int C, bool FEW, bool SHORT = false>
 int launch_sums(Jobs& j, hipStream_t s) {
-    constexpr int N = kPiece<T>, kGroups = kThreads / LANES;
+    constexpr int N = kPiece<T>, kBlock = FEW ? kFewThreads : kThreads, kGroups = kBlock / LANES;
     const int64_t dim = std::max(j.sum[0].dim, j.sum[1].dim), across = ceil_div(dim, LANES * C * N);
     for (SumArgs& a : j.sum) {
         if (a.rows == 0) continue;
@@ -571,7 +620,7 @@ int launch_sums(Jobs& j, hipStream_t s) {
     }
     // a grid's second dimension ends at 65535: 2^24 columns of fp32 are 16384 times 64 lanes of 4
     const dim3 grid(static_cast<unsigned>(j.sum[0].blocks + j.sum[1].blocks), static_cast<unsigned>(across));
-    sum_kernel<T, LANES, C, SHORT><<<grid, dim3(kThreads), 0, s>>>(j.sum[0], j.sum[1]);
+    sum_kernel<T, LANES, C, SHORT, FEW><<<grid, dim3(kBlock), 0, s>>>(j.sum[0], j.sum[1]);
     if (int rc = launched("sum_kernel")) return rc;
     const int64_t blocks[2] = {ceil_div(j.sum[0].tiles, kJoinTiles), ceil_div(j.sum[1].tiles, kJoinTiles)};
     if (blocks[0] + blocks[1] == 0) return 0;
@@ -581,18 +630,26 @@ int launch_sums(Jobs& j, hipStream_t s) {
     return launched("join_kernel");
 }
 
-// Lanes of a group and chunks of a lane: a row's columns, at most 256 chunks at a time.
+// Lanes of a group and pieces of a lane: a row's columns, at most 256 pieces at a time. Few tokens: one piece a lane, so
+// that a long row's walk is shared by the blocks of its columns, too.
 template <typename T>
-int sums(Jobs& j, int64_t dim, hipStream_t s) {
-    const int64_t chunks = ceil_div(dim, static_cast<int64_t>(kPiece<T>));
-    if (dim < kPiece<T>) return launch_sums<T, 8, 1, true>(j, s);
-    if (chunks <= 8) return launch_sums<T, 8, 1>(j, s);
-    if (chunks <= 16) return launch_sums<T, 16, 1>(j, s);
-    if (chunks <= 32) return launch_sums<T, 32, 1>(j, s);
-    if (chunks <= 64) return launch_sums<T, 64, 1>(j, s);
-    if (chunks <= 128) return launch_sums<T, 64, 2>(j, s);
-    if (chunks <= 192) return launch_sums<T, 64, 3>(j, s);
-    return launch_sums<T, 64, 4>(j, s);
+int sums(Jobs& j, int64_t dim, bool few, hipStream_t s) {
+    const int64_t pieces = ceil_div(dim, static_cast<int64_t>(kPiece<T>));
+    if (few) {
+        if (dim < kPiece<T>) return launch_sums<T, 8, 1, true, true>(j, s);
+        if (pieces <= 8) return launch_sums<T, 8, 1, true>(j, s);
+        if (pieces <= 16) return launch_sums<T, 16, 1, true>(j, s);
+        if (pieces <= 32) return launch_sums<T, 32, 1, true>(j, s);
+        return launch_sums<T, 64, 1, true>(j, s);
+    }
+    if (dim < kPiece<T>) return launch_sums<T, 8, 1, false, true>(j, s);
+    if (pieces <= 8) return launch_sums<T, 8, 1, false>(j, s);
+    if (pieces <= 16) return launch_sums<T, 16, 1, false>(j, s);
+    if (pieces <= 32) return launch_sums<T, 32, 1, false>(j, s);
+    if (pieces <= 64) return launch_sums<T, 64, 1, false>(j, s);
+    if (pieces <= 128) return launch_sums<T, 64, 2, false>(j, s);
+    if (pieces <= 192) return launch_sums<T, 64, 3, false>(j, s);
+    return launch_sums<T, 64, 4, false>(j, s);
 }
 
 // The sorts of a table's tokens into its part of the lists.
@@ -742,7 +799,8 @@ extern "C" int isa_train_embedding_backward(const isa_train_embedding* e, const 
         if (k ? listed_places : listed_weight) list += at.lists;
     }
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (e->type == ISA_BLOCK_F32) return sums<float>(j, e->dim, s);
-    if (e->type == ISA_BLOCK_BF16) return sums<bf16>(j, e->dim, s);
-    return sums<f16>(j, e->dim, s);
+    const bool few = e->tokens <= kFewTokens;
+    if (e->type == ISA_BLOCK_F32) return sums<float>(j, e->dim, few, s);
+    if (e->type == ISA_BLOCK_BF16) return sums<bf16>(j, e->dim, few, s);
+    return sums<f16>(j, e->dim, few, s);
 }

@@ -31,7 +31,7 @@ Tensor indices(const Tensor& t, const char* name, const Tensor& like) {
     if (t.scalar_type() != at::kLong && t.scalar_type() != at::kInt)
         refuse(name, " must be int64 or int32, got ", type_name(t));
     if (t.device() != like.device()) refuse(name, " must be on ", like.device(), ", got ", t.device());
-    return t.to(at::kLong).contiguous();
+    return t.scalar_type() == at::kLong && t.is_contiguous() ? t : t.to(at::kLong).contiguous();
 }
 
 // ---- embedding ------------------------------------------------------------------------------
@@ -148,9 +148,11 @@ Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, const Ma
     if (positions) {
         if (!places.defined()) refuse("positions need position_weight");
         place_ids = indices(*positions, "positions", weight);
-        if (!at::is_expandable_to(place_ids.sizes(), tokens.sizes()))
-            refuse("positions ", place_ids.sizes(), " must broadcast to ids ", tokens.sizes());
-        place_ids = place_ids.expand(tokens.sizes()).contiguous();
+        if (place_ids.sizes() != tokens.sizes()) {
+            if (!at::is_expandable_to(place_ids.sizes(), tokens.sizes()))
+                refuse("positions ", place_ids.sizes(), " must broadcast to ids ", tokens.sizes());
+            place_ids = place_ids.expand(tokens.sizes()).contiguous();
+        }
     }
     no_tangents(std::array{std::cref(weight), std::cref(places)});
     const int64_t padding = padding_index.value_or(-1);
