@@ -14,7 +14,7 @@ void leaves_can_be_captured(std::initializer_list<const Tensor*> tensors) {
         if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
         const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
         const auto stream = node ? node->stream() : std::nullopt;
-        if (stream && *stream == c10::hip::getDefaultHIPStream(t->device().index()).unwrap())
+        if (stream && stream->id() == c10::hip::getDefaultHIPStream(t->device().index()).id())
             refuse("a graph of a leaf lives that was made on the default stream: free it (the results that hold it), or "
                    "make it on another stream, before a step with that leaf is captured");
     }
@@ -31,7 +31,7 @@ Tensor indices(const Tensor& t, const char* name, const Tensor& like) {
     if (t.scalar_type() != at::kLong && t.scalar_type() != at::kInt)
         refuse(name, " must be int64 or int32, got ", type_name(t));
     if (t.device() != like.device()) refuse(name, " must be on ", like.device(), ", got ", t.device());
-    return t.scalar_type() == at::kLong && t.is_contiguous() ? t : t.to(at::kLong).contiguous();
+    return packed(t.scalar_type() == at::kLong ? t : t.to(at::kLong));
 }
 
 // ---- embedding ------------------------------------------------------------------------------
@@ -173,7 +173,7 @@ Tensor seed_of(const Tensor& seed, const Tensor& like) {
     if (seed.scalar_type() != at::kLong || seed.dim() != 1 || seed.size(0) != 2)
         refuse("seed must be int64 [2], got ", type_name(seed), " ", seed.sizes());
     if (seed.device() != like.device()) refuse("seed must be on ", like.device(), ", got ", seed.device());
-    return seed.contiguous();
+    return packed(seed);
 }
 
 isa_train_dropout dropout_of(const Tensor& seed, int64_t site, int64_t threshold) {

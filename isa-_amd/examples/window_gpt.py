@@ -1,7 +1,7 @@
 """A small GPT with physical FFNs, window attention and sinks: trained to repeat what stood some
 tokens before, then asked to go on, a token at a time over its cache.
 
-    python isa-_amd/examples/window_gpt.py [--steps 150]
+    python isa-_amd/examples/window_gpt.py [--steps 150] [--dropout 0.1]
 """
 
 from __future__ import annotations
@@ -23,14 +23,15 @@ from isa.operators.cim import PhysicalFFN
 VOCAB, PERIOD, LENGTH, DIM = 64, 12, 96, 128
 
 
-def make_model(layers: int = 2, heads: int = 4, kv_heads: int = 2, window: int = 32, sinks: int = 4) -> GPT:
+def make_model(layers: int = 2, heads: int = 4, kv_heads: int = 2, window: int = 32, sinks: int = 4,
+               dropout: float = 0.0) -> GPT:
     cfg = make_flash_transistor_ekv_config(default_lut_size=4096)
     blocks = nn.ModuleList(Block(DIM, WindowAttention(DIM, heads, kv_heads=kv_heads, window=window, sinks=sinks),
-                                 PhysicalFFN(DIM, 2 * DIM, cfg)) for _ in range(layers))
+                                 PhysicalFFN(DIM, 2 * DIM, cfg), dropout) for _ in range(layers))
     for block in blocks:  # gains that bring the currents of untrained thresholds to a fraction of a volt
         block.ffn.fc1.set_r_tia(2e6)
         block.ffn.fc2.set_r_tia(2e6)
-    return GPT(VOCAB, 4 * LENGTH, DIM, blocks).cuda()
+    return GPT(VOCAB, 4 * LENGTH, DIM, blocks, dropout).cuda()
 
 
 def batch(n: int, length: int, generator: torch.Generator) -> torch.Tensor:
@@ -75,12 +76,14 @@ def generate(model: GPT, prompt: torch.Tensor, tokens: int):
 def main() -> int:
     parser = argparse.ArgumentParser(description=__doc__)
     parser.add_argument("--steps", type=int, default=150)
+    parser.add_argument("--dropout", type=float, default=0.0)
     args = parser.parse_args()
     torch.manual_seed(0)
     generator = torch.Generator(device="cuda").manual_seed(0)
-    model = make_model()
+    model = make_model(dropout=args.dropout)
     losses = train(model, args.steps, generator)
     print(f"loss: first step {losses[0]:.3f}, last {losses[-1]:.3f}")
+    model.eval()
     whole = batch(4, LENGTH, generator)
     ids, _ = generate(model, whole[:, : 2 * PERIOD], LENGTH - 2 * PERIOD)
     right = (ids[:, 2 * PERIOD:] == whole[:, 2 * PERIOD:]).float().mean()

@@ -1,6 +1,6 @@
 """A transformer block around a physical FFN, on this package's own kernels: pre-norm blocks whose
-norms take the residual add along, and attention over a window of tokens and a few first ones,
-for training and, with a cache, for generation. The reference's models build these parts of a block
+norms take the residual add and its dropout along, attention over a window of tokens and a few first ones,
+and embeddings of tokens and positions in one pass, for training and, with a cache, for generation. The reference's models build these parts of a block
 from torch's operators (`nn.LayerNorm`, scaled-dot-product attention).
 """
 
@@ -11,7 +11,8 @@ from typing import Optional, Tuple
 import torch
 import torch.nn as nn
 
-from isa.kernels.transformer_block import add_layer_norm, layer_norm, window_attention
+from isa.kernels.transformer_block import (add_layer_norm, dropout, dropout_add_layer_norm, embedding, layer_norm,
+                                           window_attention)
 
 
 class LayerNorm(nn.LayerNorm):
@@ -26,6 +27,50 @@ class LayerNorm(nn.LayerNorm):
     def add(self, x: torch.Tensor, residual: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         """(norm of x + residual, x + residual)."""
         return add_layer_norm(x, residual, self.weight, self.bias, self.eps)
+
+    def drop_add(self, x: torch.Tensor, residual: torch.Tensor, p: float, seed: torch.Tensor,
+                 site: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The same of dropout(x, p, seed, site=site)."""
+        return dropout_add_layer_norm(x, residual, self.weight, self.bias, self.eps, p=p, seed=seed, site=site)
+
+
+class Embedding(nn.Embedding):
+    """nn.Embedding (same parameters and state dict) on the HIP kernels: looked up times `scale`, a padding_idx without
+    a gradient. Its other options (max_norm, scale_grad_by_freq, sparse) are refused. An index outside the table makes
+    its row NaN."""
+
+    def __init__(self, num_embeddings: int, embedding_dim: int, padding_idx: Optional[int] = None, scale: float = 1.0,
+                 **options):
+        super().__init__(num_embeddings, embedding_dim, padding_idx, **options)
+        if self.max_norm is not None or self.scale_grad_by_freq or self.sparse:
+            raise ValueError("max_norm, scale_grad_by_freq and sparse are not supported")
+        self.scale = scale
+
+    def forward(self, ids: torch.Tensor, positions: Optional[torch.Tensor] = None,
+                position_weight: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """With a table of positions (a place of its own for each token of a sequence unless `positions` are given)
+        the sum of both."""
+        return embedding(ids, self.weight, scale=self.scale, positions=positions, position_weight=position_weight,
+                         padding_index=self.padding_idx)
+
+
+class DropoutSeed:
+    """The key and offset of a model's dropout, an int64 tensor [2] that moves to the device of the steps.
+
+    A forward pass takes `step`: a copy for its calls, whose sites are 0 .. sites - 1, while the offset moves past them,
+    on the device, so that a HIP graph that recorded a step draws anew in each replay. key: drawn from torch's generator
+    unless given; ranks of one job take a key each. (Not a buffer of the model: those are made alike on all ranks.)"""
+
+    def __init__(self, key: Optional[int] = None):
+        self.state = torch.tensor([int(torch.randint(2 ** 62, ())) if key is None else key, 0])
+
+    @torch.no_grad()
+    def step(self, sites: int, device: torch.device) -> torch.Tensor:
+        if self.state.device != device:
+            self.state = self.state.to(device)
+        seed = self.state.clone()
+        self.state[1:].add_(sites)
+        return seed
 
 
 class WindowCache:
@@ -114,45 +159,83 @@ class WindowAttention(nn.Module):
         return self.proj(a.reshape(b, n, -1).to(x.dtype))
 
 
+def _join(norm: LayerNorm, branch: torch.Tensor, stream: torch.Tensor, p: float, seed: Optional[torch.Tensor], site: int):
+    if seed is None or p == 0.0:
+        return norm.add(branch, stream)
+    return norm.drop_add(branch, stream, p, seed, site)
+
+
 class Block(nn.Module):
     """Norm, attention, norm, FFN. A branch's output joins the residual stream inside the next norm, so
-    a block takes the last one's FFN output and the stream, and returns its own pair."""
+    a block takes the last one's FFN output and the stream, and returns its own pair.
 
-    def __init__(self, dim: int, attention: WindowAttention, ffn: nn.Module):
+    With `dropout` and a seed (`DropoutSeed.step`; none: no dropout, as for evaluation) the branches' outputs are dropped
+    as they join: the last block's under `site`, the own attention's under site + 1."""
+
+    def __init__(self, dim: int, attention: WindowAttention, ffn: nn.Module, dropout: float = 0.0):
         super().__init__()
         self.ln1, self.attention = LayerNorm(dim), attention
         self.ln2, self.ffn = LayerNorm(dim), ffn
+        self.dropout = dropout
 
-    def forward(self, branch: Optional[torch.Tensor], stream: torch.Tensor, cache: Optional[WindowCache] = None):
-        y, stream = (self.ln1(stream), stream) if branch is None else self.ln1.add(branch, stream)
-        y, stream = self.ln2.add(self.attention(y, cache), stream)
+    def forward(self, branch: Optional[torch.Tensor], stream: torch.Tensor, cache: Optional[WindowCache] = None,
+                seed: Optional[torch.Tensor] = None, site: int = 0):
+        y, stream = (self.ln1(stream), stream) if branch is None else _join(self.ln1, branch, stream, self.dropout, seed, site)
+        y, stream = _join(self.ln2, self.attention(y, cache), stream, self.dropout, seed, site + 1)
         return self.ffn(y), stream
 
 
 class GPT(nn.Module):
-    """Token and position embeddings, blocks, a last norm and the tied output projection."""
+    """Token and position embeddings, blocks, a last norm and the tied output projection. `dropout` is that of the
+    embeddings and of the last block's output (the blocks have their own), while the model trains; its numbers follow
+    from `seed`, a DropoutSeed that the model makes when it first drops unless the caller sets one."""
 
-    def __init__(self, vocab: int, positions: int, dim: int, blocks: nn.ModuleList):
+    def __init__(self, vocab: int, positions: int, dim: int, blocks: nn.ModuleList, dropout: float = 0.0):
         super().__init__()
-        self.tokens = nn.Embedding(vocab, dim)
-        self.positions = nn.Embedding(positions, dim)
+        self.tokens = Embedding(vocab, dim)
+        self.positions = Embedding(positions, dim)
         self.blocks = blocks
         self.ln_f = LayerNorm(dim)
+        self.dropout = dropout
+        self.seed = None
         for table in (self.tokens, self.positions):  # logits of untrained weights near zero
             nn.init.normal_(table.weight, std=0.02)
+
+    def _step(self, device: torch.device) -> Optional[torch.Tensor]:
+        """This pass's seed. Sites: the embeddings', two a block, the last block's output."""
+        if not self.training or not (self.dropout or any(getattr(block, "dropout", 0.0) for block in self.blocks)):
+            return None
+        if self.seed is None:
+            self.seed = DropoutSeed()
+        return self.seed.step(2 + 2 * len(self.blocks), device)
+
+    def _embed(self, ids: torch.Tensor, at: Optional[torch.Tensor]) -> torch.Tensor:
+        tokens, positions = self.tokens, self.positions
+        if type(tokens) is type(positions) is Embedding and tokens.weight.dtype == positions.weight.dtype:
+            return tokens(ids, at, positions.weight)
+        if at is None:  # a caller's own modules
+            at = torch.arange(ids.shape[1], device=ids.device)
+        return tokens(ids) + positions(at)
 
     def forward(self, ids: torch.Tensor, caches: Optional[list] = None) -> torch.Tensor:
         """Logits [batch, n, vocab]; with caches (one a block) ids continue their sequences."""
         used, positions = caches[0].longest() or 0 if caches else 0, self.positions.num_embeddings
         if used + ids.shape[1] > positions:
             raise RuntimeError(f"{ids.shape[1]} tokens after {used} do not fit the table of {positions} positions")
-        at = torch.arange(ids.shape[1], device=ids.device)
+        at = None
         if caches is not None:
-            at = caches[0].lengths.long()[:, None] + at
-        branch, stream = None, self.tokens(ids) + self.positions(at)
+            at = caches[0].lengths.long()[:, None] + torch.arange(ids.shape[1], device=ids.device)
+        seed = self._step(ids.device)
+        branch, stream = None, self._embed(ids, at)
+        if seed is not None and self.dropout:
+            stream = dropout(stream, self.dropout, seed)
         for i, block in enumerate(self.blocks):
-            branch, stream = block(branch, stream, None if caches is None else caches[i])
-        y = self.ln_f(stream) if branch is None else self.ln_f.add(branch, stream)[0]
+            rest = {} if seed is None else {"seed": seed, "site": 1 + 2 * i}
+            branch, stream = block(branch, stream, None if caches is None else caches[i], **rest)
+        if branch is None:
+            y = self.ln_f(stream)
+        else:
+            y = _join(self.ln_f, branch, stream, self.dropout, seed, 1 + 2 * len(self.blocks))[0]
         return nn.functional.linear(y, self.tokens.weight)
 
     def caches(self, batch: int, capacity: int, **options) -> list:
