@@ -45,6 +45,7 @@ struct LossArgs {
     float* row_slope;  // [rows], or null
     double* row_logp;  // [rows], or null: l, 0 in ignored rows
     bool count_here;   // each block counts the rows that are not ignored, for its gradient
+    bool past;         // the gradient is written past the caches
 };
 
 // What a row's loss is of its l.
@@ -105,11 +106,18 @@ struct Row {
             for (int e = 0; e < N; ++e) r.v[e] = at + e >= 0 && at + e < vocab ? p[at + e] : fill;
         }
     }
-    __device__ void store(T* out, int c, const Chunk& r) const {
+    __device__ void store(T* out, int c, const Chunk& r, bool past = false) const {
         const int at = c * N - skip;
         // the gradient's rows may be aligned otherwise than the logits'
         if (at >= 0 && at + N <= vocab && reinterpret_cast<uintptr_t>(out + at) % 16 == 0) {
-            *reinterpret_cast<Chunk*>(out + at) = r;
+            if (past) {
+                using V = vec<uint32_t, 4>;
+                asm volatile("");  // two stores of one value to one place become one, of the ordinary kind: not with these between
+                __builtin_nontemporal_store(__builtin_bit_cast(V, r), reinterpret_cast<V*>(out + at));
+                asm volatile("");
+            } else {
+                *reinterpret_cast<Chunk*>(out + at) = r;
+            }
             return;
         }
 #pragma unroll
@@ -198,7 +206,7 @@ __global__ __launch_bounds__(THREADS) void loss_kernel(LossArgs a) {
             if (a.row_logp) a.row_logp[r] = 0.0;
         }
         if (grad)
-            for (int c = threadIdx.x; c < chunks; c += THREADS) row.store(grad, c, typename R::Chunk{});
+            for (int c = threadIdx.x; c < chunks; c += THREADS) row.store(grad, c, typename R::Chunk{}, OF == Of::kPolicy && a.past);
         return;
     }
     const T low = static_cast<T>(-INFINITY);
@@ -280,13 +288,14 @@ __global__ __launch_bounds__(THREADS) void loss_kernel(LossArgs a) {
 #pragma unroll
         for (int i = 0; i < C; ++i) {
             const int c = threadIdx.x + i * THREADS;
-            if (c < chunks) row.store(grad, c, gradient<T, N>(held[i], c * N - row.skip, hot, top, factor, share));
+            if (c < chunks) row.store(grad, c, gradient<T, N>(held[i], c * N - row.skip, hot, top, factor, share),
+                                      OF == Of::kPolicy && a.past);
         }
     } else {
         for (int c = threadIdx.x; c < chunks; c += THREADS) {
             typename R::Chunk x;
             row.load(x, c, low);
-            row.store(grad, c, gradient<T, N>(x, c * N - row.skip, hot, top, factor, share));
+            row.store(grad, c, gradient<T, N>(x, c * N - row.skip, hot, top, factor, share), OF == Of::kPolicy && a.past);
         }
     }
 }
@@ -303,7 +312,7 @@ __global__ __launch_bounds__(THREADS) void loss_backward_kernel(LossArgs a) {
     const int64_t target = a.targets[r];
     T* grad = static_cast<T*>(a.grad) + r * a.grad_stride;
     if (target == a.ignore) {
-        for (int c = threadIdx.x; c < chunks; c += THREADS) row.store(grad, c, typename R::Chunk{});
+        for (int c = threadIdx.x; c < chunks; c += THREADS) row.store(grad, c, typename R::Chunk{}, SLOPED && a.past);
         return;
     }
     const bool inside = target >= 0 && target < a.vocab;
@@ -313,7 +322,7 @@ __global__ __launch_bounds__(THREADS) void loss_backward_kernel(LossArgs a) {
     for (int c = threadIdx.x; c < chunks; c += THREADS) {
         typename R::Chunk x;
         row.load(x, c, static_cast<T>(-INFINITY));
-        row.store(grad, c, gradient<T, N>(x, c * N - row.skip, hot, top, factor, share));
+        row.store(grad, c, gradient<T, N>(x, c * N - row.skip, hot, top, factor, share), SLOPED && a.past);
     }
 }
 

@@ -18,6 +18,9 @@ constexpr int64_t kCountHere = 1024;
 // pair and one for the sum 53.8; of 16384 x 1000 in 32 pairs 45.6 and 40.9).
 constexpr int64_t kPairsHere = 8192;
 
+// Gradients of so many bytes are written past the caches.
+constexpr size_t kGradientPast = size_t{128} << 20;
+
 struct PairArgs {
     const double* row_logp;  // [2 pairs][tokens]
     const float* ref;
@@ -98,6 +101,10 @@ __global__ __launch_bounds__(kPairThreads) void preference_sum_kernel(const floa
     for (int64_t i = threadIdx.x; i < pairs; i += kPairThreads) s += loss[i];
     s = block_sum64<kPairThreads>(s, slots);
     if (threadIdx.x == 0) out[0] = static_cast<float>(mean ? s / pairs : s);
+}
+
+bool past_caches(const isa_block_loss& l) {
+    return static_cast<size_t>(l.rows) * l.vocab * type_bytes(l.type) >= kGradientPast;
 }
 
 int check(const isa_train_policy* p) {
@@ -183,6 +190,7 @@ int run_pairs_backward(const isa_train_preference* p, const float* stats, const 
     a.grad = grad;
     a.grad_stride = grad_stride;
     a.backwards = true;  // those that were read last are in the caches
+    a.past = past_caches(p->loss);
     run_backward<true>(p->loss.type, a, s);
     return launched("loss_backward_kernel");
 }
@@ -240,6 +248,7 @@ extern "C" int isa_train_policy_backward(const isa_block_loss* l, int reduction,
     a.scale_by = grad_out;
     a.scale_step = reduction == ISA_BLOCK_NONE;
     a.scale = 1.0f;
+    a.past = past_caches(*l);
     a.grad = grad;
     a.grad_stride = grad_stride;
     run_backward<true>(l->type, a, static_cast<hipStream_t>(stream));
@@ -265,6 +274,7 @@ extern "C" int isa_train_policy_with_grad(const isa_train_policy* p, float grad_
     }
     a.row_loss = ws + 64;
     a.logp = logp;
+    a.past = past_caches(*l);
     a.scale = grad_scale;
     a.grad = grad;
     a.grad_stride = grad_stride;
