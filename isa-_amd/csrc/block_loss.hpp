@@ -49,7 +49,7 @@ struct LossArgs {
 };
 
 // What a row's loss is of its l.
-enum class Of { kCrossEntropy, kPolicy };
+enum class Of { kCrossEntropy, kPolicy, kStats };  // kStats: l and the statistics alone
 
 template <int THREADS>
 __device__ __forceinline__ float block_max(float x, float* slots) {
@@ -366,9 +366,36 @@ int64_t chunks_of(const LossArgs& a) {
 
 // Blocks of 256 threads where those hold a row in four chunks each, so that several rows share a
 // compute unit (1023 rows of 5003 in bf16: 7.6 us, in blocks of 1024 11.3); larger rows take 1024.
+//
+// The losses of l take blocks of 256 up to 2304 chunks and of 512 up to 4096 (16-bit types, or passes that hold no row): one
+// of 1024, whose rows of few chunks a thread end at its slowest wave, leaves the compute unit to one row. Policy calls
+// of 8192 rows, us of 256 / 512 / 1024 threads: 5003 in fp32 60 / 60 / 74, 8500 101 / 98 / 108, 10000 115 / 114 / 111,
+// 8200 in bf16 57 / 60 / 79, 16384 109 / 117 / 148, 24000 149 / 153 / 179, 28000 228 / 175 / 199; 4096 rows of 33333
+// 240 / 161 / 142. Preference calls of 8192 rows: 5003 in fp32 71 / 74 / 95, 12000 155 / 148 / 156, 50304 729 / 699 / 677.
+template <typename T, Of OF>
+bool launch_smaller_rows(const LossArgs& a, int64_t chunks, hipStream_t s) {
+    const int64_t few = ceil_div(chunks, 256), some = ceil_div(chunks, 512);
+    if (few > 4 && few <= 9) {
+        if (!a.grad) launch<T, 0, 256, OF>(a, s);
+        else if (few <= 5) launch<T, 5, 256, OF>(a, s);
+        else if (few <= 7) launch<T, 7, 256, OF>(a, s);
+        else launch<T, 9, 256, OF>(a, s);
+        return true;
+    }
+    if (few > 9 && some <= 8 && (!a.grad || sizeof(T) == 2)) {
+        if (!a.grad) launch<T, 0, 512, OF>(a, s);
+        else if (some <= 6) launch<T, 6, 512, OF>(a, s);
+        else launch<T, 8, 512, OF>(a, s);
+        return true;
+    }
+    return false;
+}
+
 template <typename T, Of OF>
 void launch_rows(const LossArgs& a, hipStream_t s) {
     const int64_t chunks = chunks_of<T>(a), few = ceil_div(chunks, 256), each = ceil_div(chunks, 1024);
+    if constexpr (OF != Of::kCrossEntropy)
+        if (launch_smaller_rows<T, OF>(a, chunks, s)) return;
     if (!a.grad) return few <= 4 ? launch<T, 0, 256, OF>(a, s) : launch<T, 0, 1024, OF>(a, s);  // nothing is read twice
     if (few <= 1) return launch<T, 1, 256, OF>(a, s);
     if (few <= 2) return launch<T, 2, 256, OF>(a, s);
@@ -386,7 +413,13 @@ void launch_rows(const LossArgs& a, hipStream_t s) {
 template <typename T, bool SLOPED>
 void launch_backward(const LossArgs& a, hipStream_t s) {
     const dim3 grid = grid_of(a.rows);
-    if (chunks_of<T>(a) <= 1024)
+    const int64_t chunks = chunks_of<T>(a);
+    if constexpr (SLOPED)
+        if (chunks > 2304 && chunks <= 4096) {
+            loss_backward_kernel<T, 512, SLOPED><<<grid, 512, 0, s>>>(a);
+            return;
+        }
+    if (chunks <= (SLOPED ? 2304 : 1024))
         loss_backward_kernel<T, 256, SLOPED><<<grid, 256, 0, s>>>(a);
     else
         loss_backward_kernel<T, 1024, SLOPED><<<grid, 1024, 0, s>>>(a);

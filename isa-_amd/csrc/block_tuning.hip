@@ -162,7 +162,7 @@ int run_pairs(const isa_train_preference* p, float* stats, float* losses, float*
     LossArgs a = args_of(&p->loss);
     a.row_logp = static_cast<double*>(workspace);
     a.stats = stats;
-    if (p->loss.rows) run_rows<Of::kCrossEntropy>(p->loss.type, a, s);
+    if (p->loss.rows) run_rows<Of::kStats>(p->loss.type, a, s);
     if (int rc = launched("loss_kernel")) return rc;
     const PairArgs b{a.row_logp, p->ref_logp, p->pairs, p->tokens, losses, logp, slope, p->beta};
     if (out && p->loss.rows <= kPairsHere && p->pairs <= kPairsHere) {

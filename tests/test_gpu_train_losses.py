@@ -20,8 +20,9 @@ pytestmark = pytest.mark.gpu
 
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 V = UNIT[F32]
-SIZES = [(1, 1), (3, 2), (5, 100), (7, 1023), (4, 4096), (9, 5003), (5, 16384), (3, 28672), (3, 50304), (2, 50305), (2, 65536),
-         (2, 150001), (300, 257)]
+# rows of 1 to 16 pieces of 16 bytes for each thread of blocks of 256, 512 and 1024, and more
+SIZES = [(1, 1), (3, 2), (5, 100), (7, 1023), (4, 4096), (9, 5003), (4, 7001), (3, 9000), (5, 16384), (4, 20001), (3, 28672),
+         (4, 36000), (3, 50304), (2, 50305), (2, 65536), (2, 150001), (300, 257)]
 
 
 def make(dev, rows, vocab, dtype, seed=0, low=0.2, high=0.2):
@@ -184,7 +185,7 @@ def pairs(dev, n, tokens, vocab, dtype, seed=0):
     return x, t.masked_fill(~keep, -100), (taken + torch.randn(2 * n, generator=g, device=dev).double() * 3.0).float()
 
 
-PAIRS = [(1, 1, 1), (1, 1, 2), (2, 3, 100), (3, 17, 1023), (2, 300, 257), (1, 5, 5003), (2, 2, 50304), (1, 1, 150001), (33, 4, 40),
+PAIRS = [(1, 1, 1), (1, 1, 2), (2, 3, 100), (3, 17, 1023), (2, 300, 257), (1, 5, 5003), (2, 2, 9000), (1, 3, 20001), (2, 2, 50304), (1, 1, 150001), (33, 4, 40),
          (1, 1500, 33)]
 
 
