@@ -36,6 +36,7 @@ typedef struct isa_train_embedding {
     const void* place_weight;
 } isa_train_embedding;
 #define ISA_TRAIN_EMBEDDING_MAX_ROWS (1 << 24) /* of a table */
+#define ISA_TRAIN_EMBEDDING_MAX_DIM (1 << 20)  /* tokens: at most 2^30 */
 
 /* y [tokens][dim]. For a backward call: lists (256-byte aligned), which the call fills with the tokens of each row of
  * the tables whose gradient will be asked for (weight, places: 0 or 1), without those whose id is `skip` (-1: none) or

@@ -90,7 +90,7 @@ __device__ __forceinline__ void look_up(const LookupArgs& a, int lanes, int bloc
             const int64_t id = a.ids[token];
             inside[k] = id >= 0 && id < a.vocab;
             if constexpr (PLACES) {
-                const int64_t place = a.place_ids ? a.place_ids[token] : token % a.period;
+                const int64_t place = a.place_ids ? a.place_ids[token] : static_cast<uint32_t>(token) % static_cast<uint32_t>(a.period);
                 inside[k] = inside[k] && place >= 0 && place < a.places;
                 p[k] = static_cast<const T*>(a.place_weight) + (inside[k] ? place * a.places_stride : 0);
             }
@@ -573,7 +573,7 @@ constexpr int64_t kFewTokens = 2048;
 // fp32 59 and 61.5. With one set of inputs that the cache holds the latter's gradient takes 34 us past it, 30 in it.
 constexpr size_t kResultPast = size_t{128} << 20, kGradientPast = size_t{64} << 20;
 
-constexpr int64_t kMaxTokens = int64_t{1} << 30, kMaxDim = int64_t{1} << 24;
+constexpr int64_t kMaxTokens = int64_t{1} << 30;
 
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
@@ -597,7 +597,8 @@ int check(const isa_train_embedding* e) {
     if (!e) return fail("embedding is null");
     if (!known_type(e->type)) return fail("unknown element type %d", e->type);
     if (e->tokens < 0 || e->tokens > kMaxTokens || e->vocab < 0 || e->vocab > ISA_TRAIN_EMBEDDING_MAX_ROWS ||
-        e->places < 0 || e->places > ISA_TRAIN_EMBEDDING_MAX_ROWS || e->dim < 1 || e->dim > kMaxDim)
+        e->places < 0 || e->places > ISA_TRAIN_EMBEDDING_MAX_ROWS || e->dim < 1 ||
+        e->dim > ISA_TRAIN_EMBEDDING_MAX_DIM)
         return fail("sizes out of range: tokens %lld, tables of %lld and %lld rows, dim %lld",
                     static_cast<long long>(e->tokens), static_cast<long long>(e->vocab),
                     static_cast<long long>(e->places), static_cast<long long>(e->dim));
@@ -632,7 +633,7 @@ int launch_sums(Jobs& j, hipStream_t s) {
         a.tile_blocks = static_cast<int>(ceil_div(a.tiles, kGroups));
         a.blocks = a.tile_blocks + static_cast<int>(ceil_div(ceil_div(a.rows, a.each), kGroups));
     }
-    // a grid's second dimension ends at 65535: 2^24 columns of fp32 are 16384 times 64 lanes of 4
+    // a grid's second dimension ends at 65535: 2^20 columns of fp32 are 4096 times 64 lanes of 4
     const dim3 grid(static_cast<unsigned>(j.sum[0].blocks + j.sum[1].blocks), static_cast<unsigned>(across));
     sum_kernel<T, LANES, C, SHORT, FEW><<<grid, dim3(kBlock), 0, s>>>(j.sum[0], j.sum[1]);
     if (int rc = launched("sum_kernel")) return rc;

@@ -36,9 +36,11 @@ Tensor indices(const Tensor& t, const char* name, const Tensor& like) {
 
 // ---- embedding ------------------------------------------------------------------------------
 
-void check_table(const Tensor& t, const char* name) {
-    if (t.dim() != 2 || t.size(1) < 1 || t.size(0) > ISA_TRAIN_EMBEDDING_MAX_ROWS)
-        refuse(name, " must be [rows, dim] of at most ", ISA_TRAIN_EMBEDDING_MAX_ROWS, " rows, got ", t.sizes());
+void check_table(const Tensor& t, const char* name, int64_t least_rows) {
+    if (t.dim() != 2 || t.size(1) < 1 || t.size(1) > ISA_TRAIN_EMBEDDING_MAX_DIM || t.size(0) < least_rows ||
+        t.size(0) > ISA_TRAIN_EMBEDDING_MAX_ROWS)
+        refuse(name, " must be [rows, dim] of ", least_rows, " to ", ISA_TRAIN_EMBEDDING_MAX_ROWS, " rows and 1 to ",
+               ISA_TRAIN_EMBEDDING_MAX_DIM, " columns, got ", t.sizes());
 }
 
 // ids and place_ids: contiguous int64; without place_ids a second table's rows are taken in turn along ids' last dimension.
@@ -129,7 +131,7 @@ Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, const Ma
                  const Maybe& position_weight, std::optional<int64_t> padding_index) {
     not_traced();
     require(weight, "weight");
-    check_table(weight, "weight");
+    check_table(weight, "weight", 0);
     if (!std::isfinite(scale)) refuse("scale must be finite, got ", scale);
     if (padding_index && (*padding_index < 0 || *padding_index >= weight.size(0)))
         refuse("padding_index must be None or a row of weight (0 to ", weight.size(0) - 1, "), got ", *padding_index);
@@ -137,7 +139,7 @@ Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, const Ma
     Tensor place_ids;
     if (places.defined()) {
         require(places, "position_weight", weight);
-        check_table(places, "position_weight");
+        check_table(places, "position_weight", 1);
         if (places.scalar_type() != weight.scalar_type() || places.size(1) != weight.size(1))
             refuse("position_weight must be ", type_name(weight), " [rows, ", weight.size(1), "] as weight is, got ",
                    type_name(places), " ", places.sizes());

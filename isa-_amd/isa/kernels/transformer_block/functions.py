@@ -84,7 +84,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, po
     """scale * weight[ids], and with a second table + position_weight[positions], in one pass: [*ids.shape, dim].
 
     ids: int64 or int32 of any shape on weight's device; weight: [vocab, dim], position_weight: [places, dim] of its type
-    (float32, bfloat16 or float16), at most 2^24 rows each. positions broadcast to ids; without them the tokens along
+    (float32, bfloat16 or float16), at most 2^24 rows and 2^20 columns. positions broadcast to ids; without them the tokens along
     ids' last dimension stand at 0, 1, 2, ... The sum is made in fp32 and rounded once.
 
     An id or a position outside its table makes its row NaN and takes no part in that table's gradient, nor does

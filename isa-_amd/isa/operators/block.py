@@ -39,8 +39,8 @@ class Embedding(nn.Embedding):
     a gradient. Its other options (max_norm, scale_grad_by_freq, sparse) are refused. An index outside the table makes
     its row NaN."""
 
-    def __init__(self, num_embeddings: int, embedding_dim: int, padding_idx: Optional[int] = None, scale: float = 1.0,
-                 **options):
+    def __init__(self, num_embeddings: int, embedding_dim: int, padding_idx: Optional[int] = None, *,
+                 scale: float = 1.0, **options):
         super().__init__(num_embeddings, embedding_dim, padding_idx, **options)
         if self.max_norm is not None or self.scale_grad_by_freq or self.sparse:
             raise ValueError("max_norm, scale_grad_by_freq and sparse are not supported")

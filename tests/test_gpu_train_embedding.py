@@ -32,9 +32,12 @@ def within(got, want, bound, what):
 
 
 def depth(tokens):
-    """Additions one after the other: a tile's, then of a wave's tiles, then of 16 waves."""
-    tile = max(64, -(-tokens // 2048))
-    return min(tokens, tile) + -(-tokens // tile // 16) + 17
+    """Additions one after the other. Up to 2048 tokens: those of one of a block's 16 to 128 groups, then of the groups;
+    else a tile's, then of every eighth tile, then of eight waves."""
+    if tokens <= 2048:
+        return -(-tokens // 16) + 128
+    tile = max(16, -(-tokens // 2048))
+    return tile + -(-tokens // tile // 8) + 9
 
 
 def check(dev, ids, weight, scale=1.0, positions=None, position_weight=None, padding=None, seed=0):
@@ -129,7 +132,13 @@ def test_one_token_again_and_again(cuda_device):
     check(cuda_device, torch.arange(5, device=cuda_device).repeat(64) * 2, w)
     check(cuda_device, torch.arange(5, device=cuda_device).repeat_interleave(65) * 2, w)
     p = torch.randn(3, 40, device=cuda_device)
-    check(cuda_device, torch.zeros(5000, 2, dtype=torch.int64, device=cuda_device), w, 1.0, None, p)
+    for times in (200, 5000):  # positions that many tokens share
+        check(cuda_device, torch.zeros(times, 2, dtype=torch.int64, device=cuda_device), w, 1.0, None, p)
+    for dim in (3, 64, 700, 1500):  # long rows of few tokens, by every width of a group
+        w = torch.randn(60, dim, device=cuda_device)
+        for dtype in (F32, BF16):
+            ids = torch.cat([torch.full((900,), 59), torch.arange(60), torch.full((40,), 3), torch.full((17,), 4)]).to(cuda_device)
+            check(cuda_device, ids, w.to(dtype), 0.5)
 
 
 def test_views_and_empty_ones(cuda_device):
@@ -144,6 +153,8 @@ def test_views_and_empty_ones(cuda_device):
     check(cuda_device, ids.t(), whole)
     check(cuda_device, ids[::2, 1::3], whole, 1.0, ids[:1, 1::3], whole)
     check(cuda_device, ids[0, 0], whole, 1.0, None, whole)  # no dimension
+    y, (g,) = check(cuda_device, ids, whole[:0])  # a table without rows
+    assert torch.isnan(y).all() and g.shape == (0, 37)
     for shape in ((0,), (3, 0), (0, 5)):
         print(f"[case] empty {shape}", flush=True)
         none = torch.zeros(shape, dtype=torch.int64, device=cuda_device)

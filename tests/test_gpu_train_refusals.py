@@ -159,6 +159,7 @@ def test_arguments_that_do_not_fit(cuda_device):
     refused("must be int64 or int32", ops.embedding, ids, w, positions=ids.double(), position_weight=w)
     refused("as weight is", ops.embedding, ids, w, position_weight=w.half())
     refused("as weight is", ops.embedding, ids, w, position_weight=w[:, :4])
+    refused(r"must be \[rows, dim\] of 1", ops.embedding, ids, w, positions=ids, position_weight=w[:0])
     refused("do not fit a table of 1 positions", ops.embedding, ids, w, position_weight=w[:1])
     for p in (-0.1, 1.1, float("nan")):
         refused("p must be 0 to 1", ops.dropout, x, p, seed)

@@ -87,7 +87,7 @@ def test_embedding_refusals(lib):
 
     refused(lib, lib.isa_train_embedding_forward(None, FAKE, 0, 0, -1, None, 0, None), "null")
     refused(lib, forward(type=3), "type")
-    for name, bad in (("tokens", -1), ("tokens", (1 << 30) + 1), ("dim", 0), ("dim", (1 << 24) + 1), ("vocab", -1),
+    for name, bad in (("tokens", -1), ("tokens", (1 << 30) + 1), ("dim", 0), ("dim", (1 << 20) + 1), ("vocab", -1),
                       ("vocab", (1 << 24) + 1), ("places", -1), ("places", (1 << 24) + 1)):
         refused(lib, forward(**{name: bad}), "sizes out of range")
     refused(lib, forward(ids=None), "ids must be set")
