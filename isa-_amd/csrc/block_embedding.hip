@@ -304,8 +304,10 @@ __device__ __forceinline__ int token_at(const SumArgs& a, int place) {
     if (a.order) return a.order[place];
     return place % a.times * a.period + place / a.times;
 }
+// (Held to the table: keys that were overwritten since they were sorted give wrong sums, not other memory.)
 __device__ __forceinline__ int row_at(const SumArgs& a, int place) {
-    return a.order ? static_cast<int>(a.keys[a.order[place]]) : place / a.times;
+    if (!a.order) return place / a.times;
+    return static_cast<int>(std::min<uint64_t>(static_cast<uint64_t>(a.keys[a.order[place]]), static_cast<uint64_t>(a.rows - 1)));
 }
 
 // `from`'s value in a group of LANES lanes: uniform in a wave where that is the group.

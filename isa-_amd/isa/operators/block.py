@@ -62,14 +62,16 @@ class DropoutSeed:
     unless given; ranks of one job take a key each. (Not a buffer of the model: those are made alike on all ranks.)"""
 
     def __init__(self, key: Optional[int] = None):
-        self.state = torch.tensor([int(torch.randint(2 ** 62, ())) if key is None else key, 0])
+        with torch.inference_mode(False):  # it changes in place, in any mode
+            self.state = torch.tensor([int(torch.randint(2 ** 62, ())) if key is None else key, 0])
 
     @torch.no_grad()
     def step(self, sites: int, device: torch.device) -> torch.Tensor:
-        if self.state.device != device:
-            self.state = self.state.to(device)
-        seed = self.state.clone()
-        self.state[1:].add_(sites)
+        with torch.inference_mode(False):
+            if self.state.device != device:
+                self.state = self.state.to(device)
+            seed = self.state.clone()
+            self.state[1:].add_(sites)
         return seed
 
 

@@ -269,6 +269,10 @@ def test_a_seeds_steps():
     s = DropoutSeed(key=-4)
     cpu = torch.device("cpu")
     assert s.step(3, cpu).tolist() == [-4, 0] and s.step(5, cpu).tolist() == [-4, 3] and s.state.tolist() == [-4, 8]
+    with torch.inference_mode():
+        made = DropoutSeed(key=1)
+        assert made.step(1, cpu).tolist() == [1, 0]
+    assert made.step(1, cpu).tolist() == [1, 1]
     torch.manual_seed(1)
     a = DropoutSeed().state
     torch.manual_seed(1)
