@@ -300,30 +300,36 @@ __global__ __launch_bounds__(THREADS) void loss_kernel(LossArgs a) {
     }
 }
 
-template <typename T, int THREADS, bool SLOPED>
-__global__ __launch_bounds__(THREADS) void loss_backward_kernel(LossArgs a) {
+// A row's gradient from its statistics, by a block; share(): its factor, asked for where the row counts.
+template <typename T, int THREADS, typename Share>
+__device__ __forceinline__ void row_gradient(const LossArgs& a, int64_t r, bool past, Share share_of_row) {
     using R = Row<T>;
     constexpr int N = R::N;
-    int64_t r = block_row();
-    if (r >= a.rows) return;  // (a whole block)
-    if (SLOPED && a.backwards) r = a.rows - 1 - r;
     const R row(static_cast<const T*>(a.logits) + r * a.stride, a.vocab);
     const int chunks = row.chunks();
     const int64_t target = a.targets[r];
     T* grad = static_cast<T*>(a.grad) + r * a.grad_stride;
     if (target == a.ignore) {
-        for (int c = threadIdx.x; c < chunks; c += THREADS) row.store(grad, c, typename R::Chunk{}, SLOPED && a.past);
+        for (int c = threadIdx.x; c < chunks; c += THREADS) row.store(grad, c, typename R::Chunk{}, past);
         return;
     }
     const bool inside = target >= 0 && target < a.vocab;
-    const float top = a.stats[2 * r], share = !inside ? NAN : SLOPED ? sloped_share_of(a, r) : share_of(a, r);
+    const float top = a.stats[2 * r], share = inside ? share_of_row() : NAN;
     const float factor = share * __builtin_amdgcn_exp2f(-a.stats[2 * r + 1] * kLog2E);
     const int hot = inside ? static_cast<int>(target) : -1;
     for (int c = threadIdx.x; c < chunks; c += THREADS) {
         typename R::Chunk x;
         row.load(x, c, static_cast<T>(-INFINITY));
-        row.store(grad, c, gradient<T, N>(x, c * N - row.skip, hot, top, factor, share), SLOPED && a.past);
+        row.store(grad, c, gradient<T, N>(x, c * N - row.skip, hot, top, factor, share), past);
     }
+}
+
+template <typename T, int THREADS, bool SLOPED>
+__global__ __launch_bounds__(THREADS) void loss_backward_kernel(LossArgs a) {
+    int64_t r = block_row();
+    if (r >= a.rows) return;  // (a whole block)
+    if (SLOPED && a.backwards) r = a.rows - 1 - r;
+    row_gradient<T, THREADS>(a, r, SLOPED && a.past, [&] { return SLOPED ? sloped_share_of(a, r) : share_of(a, r); });
 }
 
 __global__ __launch_bounds__(kMostThreads) void loss_count_kernel(const int64_t* targets, int64_t rows, int64_t ignore,

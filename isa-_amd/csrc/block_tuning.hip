@@ -20,6 +20,12 @@ constexpr int64_t kCountHere = 1024;
 // pair and one for the sum 53.8; of 16384 x 1000 in 32 pairs 45.6 and 40.9).
 constexpr int64_t kPairsHere = 8192;
 
+// Up to so many rows of so many bytes and pairs each row's block of 256 makes its pair's slope from the pair's l, which saves
+// a launch: a call of 2 x 512 x 1000 in bf16 10.2 us, else 15.0; of 6 x 171 x 5003 in fp16 14.8 and 17.8; of 32 x 32 x
+// 5003 in bf16 17.6 and 17.9; of 2 x 1024 x 5003 21.5 and 21.4, of 64 x 32 x 1000 22.5 and 17.3, of 8 x 128 x 50304 in
+// fp32 133 and 101.
+constexpr int64_t kFewRows = 1536, kFewPairs = 16, kFewBytes = 2304 * 16;
+
 // Gradients of so many bytes are written past the caches.
 constexpr size_t kGradientPast = size_t{128} << 20;
 
@@ -37,15 +43,23 @@ __device__ __forceinline__ double wave_sum64(double x) {
     return x;
 }
 
+__device__ __forceinline__ double pair_margin(const PairArgs& a, int64_t p, double chosen, double other) {
+    return a.beta * ((chosen - a.ref[p]) - (other - a.ref[a.pairs + p]));
+}
+
+// The slope of a pair's loss by its chosen sequence's sum; by the other one's it is the negative.
+__device__ __forceinline__ float pair_slope(const PairArgs& a, double margin) {
+    return static_cast<float>(-a.beta / (1.0 + exp(margin)));
+}
+
 // A pair's loss and slopes from the sums of its sequences.
 __device__ __forceinline__ float pair_loss(const PairArgs& a, int64_t p, double chosen, double other) {
-    const double m = a.beta * ((chosen - a.ref[p]) - (other - a.ref[a.pairs + p]));
-    const double slope = -a.beta / (1.0 + exp(m));
+    const double m = pair_margin(a, p, chosen, other);
     a.logp[p] = static_cast<float>(chosen);
     a.logp[a.pairs + p] = static_cast<float>(other);
     if (a.slope) {
-        a.slope[p] = static_cast<float>(slope);
-        a.slope[a.pairs + p] = static_cast<float>(-slope);
+        a.slope[p] = pair_slope(a, m);
+        a.slope[a.pairs + p] = -a.slope[p];
     }
     return static_cast<float>((m < 0.0 ? -m : 0.0) + log1p(exp(-fabs(m))));
 }
@@ -60,28 +74,36 @@ __device__ __forceinline__ double block_sum64(double x, double* slots) {
     return x;
 }
 
+// The sums of pair p's sequences, in all threads of a block. `slots` are free again after the block's next barrier.
+template <int THREADS>
+__device__ __forceinline__ void pair_sums(const PairArgs& a, int64_t p, double (&slots)[2][THREADS / kWave],
+                                          double (&sums)[2]) {
+    double s[2] = {0.0, 0.0};
+    for (int64_t i = threadIdx.x; i < a.tokens; i += THREADS) {
+        s[0] += a.row_logp[p * a.tokens + i];
+        s[1] += a.row_logp[(a.pairs + p) * a.tokens + i];
+    }
+    for (int k = 0; k < 2; ++k) sums[k] = block_sum64<THREADS>(s[k], slots[k]);
+}
+
 // A block a pair.
 __global__ __launch_bounds__(kPairThreads) void preference_pair_kernel(PairArgs a) {
     __shared__ double slots[2][kPairThreads / kWave];
     for (int64_t p = blockIdx.x; p < a.pairs; p += gridDim.x) {
         double sums[2];
-        for (int k = 0; k < 2; ++k) {
-            const double* rows = a.row_logp + (k * a.pairs + p) * a.tokens;
-            double s = 0.0;
-            for (int64_t i = threadIdx.x; i < a.tokens; i += kPairThreads) s += rows[i];
-            sums[k] = block_sum64<kPairThreads>(s, slots[k]);
-        }
+        pair_sums<kPairThreads>(a, p, slots, sums);
         if (threadIdx.x == 0) a.loss[p] = pair_loss(a, p, sums[0], sums[1]);
         __syncthreads();
     }
 }
 
 // All pairs, a wave each, and the sum or mean of their losses.
-__global__ __launch_bounds__(kMostThreads) void preference_pairs_kernel(PairArgs a, int mean, float* out) {
-    __shared__ double slots[kMostThreads / kWave];
+template <int THREADS>
+__device__ __forceinline__ void all_pairs(const PairArgs& a, int mean, float* out) {
+    __shared__ double slots[THREADS / kWave];
     const int lane = threadIdx.x % kWave;
     double all = 0.0;
-    for (int64_t p = threadIdx.x / kWave; p < a.pairs; p += kMostThreads / kWave) {
+    for (int64_t p = threadIdx.x / kWave; p < a.pairs; p += THREADS / kWave) {
         double sums[2];
         for (int k = 0; k < 2; ++k) {
             const double* rows = a.row_logp + (k * a.pairs + p) * a.tokens;
@@ -92,8 +114,27 @@ __global__ __launch_bounds__(kMostThreads) void preference_pairs_kernel(PairArgs
         }
         if (lane == 0) all += pair_loss(a, p, sums[0], sums[1]);
     }
-    all = block_sum64<kMostThreads>(all, slots);
+    all = block_sum64<THREADS>(all, slots);
     if (threadIdx.x == 0) out[0] = static_cast<float>(mean ? all / a.pairs : all);
+}
+
+__global__ __launch_bounds__(kMostThreads) void preference_pairs_kernel(PairArgs a, int mean, float* out) {
+    all_pairs<kMostThreads>(a, mean, out);
+}
+
+// The gradients of few rows, each of whose blocks makes its pair's slope, and by one block more the pairs' losses.
+template <typename T>
+__global__ __launch_bounds__(kPairThreads) void preference_rows_kernel(LossArgs a, PairArgs b, float* out) {
+    __shared__ double slots[2][kPairThreads / kWave];
+    const int64_t r = blockIdx.x;
+    if (r == a.rows) return all_pairs<kPairThreads>(b, 1, out);
+    row_gradient<T, kPairThreads>(a, r, false, [&] {
+        const int64_t sequence = r / b.tokens, p = sequence % b.pairs;
+        double sums[2];
+        pair_sums<kPairThreads>(b, p, slots, sums);
+        const float slope = pair_slope(b, pair_margin(b, p, sums[0], sums[1]));
+        return (sequence < b.pairs ? -slope : slope) * a.scale;
+    });
 }
 
 __global__ __launch_bounds__(kPairThreads) void preference_sum_kernel(const float* loss, int64_t pairs, int mean,
@@ -177,6 +218,25 @@ int run_pairs(const isa_train_preference* p, float* stats, float* losses, float*
     if (!out) return 0;
     preference_sum_kernel<<<1, kPairThreads, 0, s>>>(losses, p->pairs, mean, out);
     return launched("preference_sum_kernel");
+}
+
+// Few rows: l and statistics, then all the rest in one launch.
+int run_few_pairs(const isa_train_preference* p, float scale, float* stats, float* logp, float* out, void* grad,
+                  int64_t grad_stride, void* workspace, hipStream_t s) {
+    LossArgs a = args_of(&p->loss);
+    a.row_logp = static_cast<double*>(workspace);
+    a.stats = stats;
+    run_rows<Of::kStats>(p->loss.type, a, s);
+    if (int rc = launched("loss_kernel")) return rc;
+    a.grad = grad;
+    a.grad_stride = grad_stride;
+    a.scale = scale;
+    const PairArgs b{a.row_logp, p->ref_logp, p->pairs, p->tokens, nullptr, logp, nullptr, p->beta};
+    const dim3 grid(static_cast<unsigned>(a.rows + 1));
+    if (p->loss.type == ISA_BLOCK_F32) preference_rows_kernel<float><<<grid, dim3(kPairThreads), 0, s>>>(a, b, out);
+    else if (p->loss.type == ISA_BLOCK_BF16) preference_rows_kernel<bf16><<<grid, dim3(kPairThreads), 0, s>>>(a, b, out);
+    else preference_rows_kernel<f16><<<grid, dim3(kPairThreads), 0, s>>>(a, b, out);
+    return launched("preference_rows_kernel");
 }
 
 int run_pairs_backward(const isa_train_preference* p, const float* stats, const float* slope, const float* by, int step,
@@ -334,7 +394,11 @@ extern "C" int isa_train_preference_with_grad(const isa_train_preference* p, flo
     char* ws = static_cast<char*>(workspace);
     float *stats = reinterpret_cast<float*>(ws + at.stats), *losses = reinterpret_cast<float*>(ws + at.loss),
           *slope = reinterpret_cast<float*>(ws + at.slope);
+    const float scale = grad_scale / static_cast<float>(p->pairs);
+    const int64_t row_bytes = p->loss.vocab * static_cast<int64_t>(type_bytes(p->loss.type));
+    if (p->loss.rows && p->loss.rows <= kFewRows && p->pairs <= kFewPairs && row_bytes <= kFewBytes)
+        return run_few_pairs(p, scale, stats, logp, out, grad, grad_stride, ws, s);
     if (int rc = run_pairs(p, stats, losses, logp, slope, 1, out, ws, s)) return rc;
     if (p->loss.rows == 0) return 0;
-    return run_pairs_backward(p, stats, slope, nullptr, 0, grad_scale / static_cast<float>(p->pairs), grad, grad_stride, s);
+    return run_pairs_backward(p, stats, slope, nullptr, 0, scale, grad, grad_stride, s);
 }
