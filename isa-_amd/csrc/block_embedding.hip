@@ -85,26 +85,36 @@ __device__ __forceinline__ void look_up(const LookupArgs& a, int lanes, int bloc
     if (group >= per_block) return;
     const int64_t step = static_cast<int64_t>(blocks) * per_block * K;
     for (int64_t t = (static_cast<int64_t>(block) * per_block + group) * K; t < a.tokens; t += step) {
+        int64_t id[K], place[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) id[k] = a.ids[std::min(t + k, a.tokens - 1)];
+        if constexpr (PLACES) {
+            if (a.place_ids)
+#pragma unroll
+                for (int k = 0; k < K; ++k) place[k] = a.place_ids[std::min(t + k, a.tokens - 1)];
+            else
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    place[k] = static_cast<uint32_t>(std::min(t + k, a.tokens - 1)) % static_cast<uint32_t>(a.period);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // all of them before the first is waited for
         const T *w[K], *p[K];
         bool inside[K];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int64_t token = std::min(t + k, a.tokens - 1);
-            const int64_t id = a.ids[token];
-            inside[k] = id >= 0 && id < a.vocab;
+            inside[k] = static_cast<uint64_t>(id[k]) < static_cast<uint64_t>(a.vocab);
             if constexpr (PLACES) {
-                const int64_t place = a.place_ids ? a.place_ids[token] : static_cast<uint32_t>(token) % static_cast<uint32_t>(a.period);
-                inside[k] = inside[k] && place >= 0 && place < a.places;
-                p[k] = static_cast<const T*>(a.place_weight) + (inside[k] ? place * a.places_stride : 0);
+                inside[k] = inside[k] & (static_cast<uint64_t>(place[k]) < static_cast<uint64_t>(a.places));
+                p[k] = static_cast<const T*>(a.place_weight) + (inside[k] ? place[k] : 0) * a.places_stride;
             }
-            w[k] = static_cast<const T*>(a.weight) + (inside[k] ? id * a.weight_stride : 0);
+            w[k] = static_cast<const T*>(a.weight) + (inside[k] ? id[k] : 0) * a.weight_stride;
         }
         for (int column = lane * N; column < a.dim; column += lanes * N) {
             const int at = piece_at<T, SHORT>(column, a.dim);
             vec<T, N> r[K], q[K];
 #pragma unroll
-            for (int k = 0; k < K; ++k) {  // (a table without rows has nothing to read)
-                if (a.vocab) load_piece<T, SHORT>(r[k], w[k] + at, a.dim);
+            for (int k = 0; k < K; ++k) {
+                load_piece<T, SHORT>(r[k], w[k] + at, a.dim);
                 if constexpr (PLACES) load_piece<T, SHORT>(q[k], p[k] + at, a.dim);
             }
 #pragma unroll
@@ -751,14 +761,15 @@ extern "C" int isa_train_embedding_forward(const isa_train_embedding* e, void* y
     }
     if (places && e->place_ids) sorts[1] = sort_of(e, true, -1, list);
     if (e->tokens == 0 && sorts[0].blocks + sorts[1].blocks == 0) return 0;
+    // a table without rows has nothing to read: some memory stands for the row that no id is found in
     const LookupArgs a{e->ids,
                        e->place_ids,
-                       e->weight,
+                       e->vocab ? e->weight : y,
                        e->place_weight,
                        y,
                        e->tokens,
                        e->vocab,
-                       e->weight_stride,
+                       e->vocab ? e->weight_stride : 0,
                        e->places,
                        e->places_stride,
                        e->period,
