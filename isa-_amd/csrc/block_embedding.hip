@@ -580,15 +580,17 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(SumArgs first, SumAr
 // rows and tiles 62 us and the join 7; by 64 65 and 7, by 16 63 and 12).
 int tile_of(int64_t tokens) { return static_cast<int>(std::max<int64_t>(16, ceil_div(tokens, 2048))); }
 
-// So many need no tiles: a row of all of them is a walk of 128 tokens for each wave of a block, and a launch less (a step
-// of 2048 tokens of a 50304 x 768 fp32 table 49 us, by tiles 53; with one token 2048 times 57 and 53).
-constexpr int64_t kFewTokens = 2048;
+// So many need no tiles in tables of so many bytes: a row of all of them is a walk of 128 tokens for each wave of a block, and
+// a launch less (a step of 999 tokens of a 5003 x 390 bf16 table 49 us, by tiles 54). Larger tables' rows are written by
+// waves that take more of a row: the gradient of 131072 x 1024 in bf16 51 us by tiles, else 66.
+constexpr int64_t kFewTokens = 2048, kFewBytes = int64_t{32} << 20;
 
 // Results that are written past the caches: y from half the last cache's size on, which the next operator reads, a
 // gradient from a quarter on, which waits for the optimizer. A step of 65536 tokens of a 50304 x 1024 bf16 table: 110
 // us on inputs that change, 119 through the caches (y alone 114, the gradient alone 117); of 8192 tokens of 50304 x 768 in
 // fp32 59 and 61.5. With one set of inputs that the cache holds the latter's gradient takes 34 us past it, 30 in it.
-constexpr size_t kResultPast = size_t{128} << 20, kGradientPast = size_t{64} << 20;
+// Rows of whole lines alone: parts of one line, of two waves, would each be a write of its own there.
+constexpr size_t kResultPast = size_t{128} << 20, kGradientPast = size_t{64} << 20, kLine = 128;
 
 constexpr int64_t kMaxTokens = int64_t{1} << 30;
 
@@ -599,10 +601,10 @@ struct Space {
     int64_t tiles;
     size_t starts, lists;         // bytes before the lists' starts, in all
     size_t partial, workspace;    // bytes before the partial sums, in all
-    Space(int64_t tokens, int64_t rows, int64_t dim, bool keys, int64_t period) {
+    Space(int64_t tokens, int64_t rows, int64_t dim, bool few, bool keys, int64_t period) {
         const int tile = tile_of(tokens);
         // of few tokens a row's block takes longer ones; without keys all rows have one length
-        tiles = tokens > kFewTokens && (keys || tokens / period > tile) ? ceil_div(tokens, tile) : 0;
+        tiles = !few && tokens > tile && (keys || tokens / period > tile) ? ceil_div(tokens, tile) : 0;
         starts = keys ? rounded(tokens * sizeof(int)) : 0;
         lists = starts + (keys ? rounded((rows + 1) * sizeof(int)) : 0);
         partial = rounded(tiles * sizeof(int));
@@ -625,9 +627,15 @@ int check(const isa_train_embedding* e) {
     return 0;
 }
 
+// Whether no tiles are made: of few tokens, for tables that are not large.
+bool few_of(const isa_train_embedding* e) {
+    return e->tokens <= kFewTokens &&
+           std::max(e->vocab, e->places) * e->dim * static_cast<int64_t>(type_bytes(e->type)) <= kFewBytes;
+}
+
 Space space_of(const isa_train_embedding* e, bool places) {
-    if (!places) return Space(e->tokens, e->vocab, e->dim, true, 1);
-    return Space(e->tokens, e->places, e->dim, e->place_ids != nullptr, e->tokens ? e->period : 1);
+    if (!places) return Space(e->tokens, e->vocab, e->dim, few_of(e), true, 1);
+    return Space(e->tokens, e->places, e->dim, few_of(e), e->place_ids != nullptr, e->tokens ? e->period : 1);
 }
 
 // Rows of a group: so many that some 8192 groups of 64 lanes take them all, at most the lanes that know where they
@@ -775,7 +783,7 @@ extern "C" int isa_train_embedding_forward(const isa_train_embedding* e, void* y
                        e->period,
                        static_cast<int>(e->dim),
                        e->scale,
-                       static_cast<size_t>(e->tokens) * e->dim * b >= kResultPast};
+                       static_cast<size_t>(e->tokens) * e->dim * b >= kResultPast && e->dim * b % kLine == 0};
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (e->type == ISA_BLOCK_F32) launch_lookup<float>(a, sorts, s);
     else if (e->type == ISA_BLOCK_BF16) launch_lookup<bf16>(a, sorts, s);
@@ -829,13 +837,13 @@ extern "C" int isa_train_embedding_backward(const isa_train_embedding* e, const 
             a.dim = static_cast<int>(e->dim);
             a.tile = tile_of(e->tokens);
             a.scale = k ? 1.0f : e->scale;
-            a.past = static_cast<size_t>(a.rows) * a.dim * b >= kGradientPast;
+            a.past = static_cast<size_t>(a.rows) * a.dim * b >= kGradientPast && a.dim * b % kLine == 0;
             ws += at.workspace;
         }
         if (k ? listed_places : listed_weight) list += at.lists;
     }
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    const bool few = e->tokens <= kFewTokens;
+    const bool few = few_of(e);
     if (e->type == ISA_BLOCK_F32) return sums<float>(j, e->dim, few, s);
     if (e->type == ISA_BLOCK_BF16) return sums<bf16>(j, e->dim, few, s);
     return sums<f16>(j, e->dim, few, s);
