@@ -281,7 +281,7 @@ __global__ __launch_bounds__(THREADS) void loss_kernel(LossArgs a) {
     }
     if (!grad) return;
     float share = inside ? share_of(a, r) : NAN;
-    if constexpr (OF == Of::kPolicy) share *= -slope / count;
+    if constexpr (OF == Of::kPolicy) share = share / count * -slope;  // (as where the count is an input)
     const float factor = share / sum;
     const int hot = inside ? static_cast<int>(target) : -1;
     if constexpr (C > 0) {

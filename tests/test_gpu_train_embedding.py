@@ -205,3 +205,26 @@ def test_gradient_against_differences(cuda_device):
                 moved[i][at] += 1.0
                 diff = float(f(*moved)) - float(f(*leaves))
                 assert abs(diff - float(g[at])) <= 400 * V * 8 * max(1.0, float(g.abs().max())), (i, at)
+
+
+@pytest.mark.parametrize("size", [(1500, 50304, 200, F32), (3000, 50304, 512, F32), (70000, 40000, 1024, BF16), (40, 90000, 390, BF16)],
+                         ids=str)
+def test_large_tables_and_results(cuda_device, size):
+    """Tables and results past the sizes from which tiles are made of few tokens and writes go past the caches; the 64-bit
+    sums are made on the GPU."""
+    from isa.kernels.transformer_block import embedding
+
+    tokens, vocab, dim, dtype = size
+    print(f"[case] {size}", flush=True)
+    ids, w = make(cuda_device, (tokens,), vocab, dim, dtype, seed=7)
+    ids[: tokens // 2] = torch.where(torch.rand(tokens // 2, device=cuda_device) < 0.5, vocab - 1, ids[: tokens // 2])
+    g = torch.Generator(device=cuda_device).manual_seed(8)
+    dy = torch.randn(tokens, dim, generator=g, device=cuda_device).to(dtype)
+    w.requires_grad_(True)
+    y = embedding(ids, w)
+    assert torch.equal(y, w.detach()[ids])
+    (dw,) = torch.autograd.grad(y, w, dy)
+    want = torch.zeros(vocab, dim, dtype=torch.float64, device=cuda_device).index_add_(0, ids, dy.double())
+    sizes = torch.zeros_like(want).index_add_(0, ids, dy.double().abs())
+    over = (dw.double() - want).abs() - UNIT[dtype] * want.abs() - V * (depth(tokens) + 2) * sizes
+    assert float(over.max()) <= 0.0

@@ -257,3 +257,29 @@ def test_preference_edges(cuda_device):
     assert math.isnan(float(preference_loss(x[:0], t[:0], ref[:0])[0]))
     assert float(preference_loss(x[:0], t[:0], ref[:0], reduction="sum")[0]) == 0.0
     assert preference_loss(x[:0], t[:0], ref[:0], reduction="none")[0].shape == (0,)
+
+
+@pytest.mark.parametrize("vocab", [25000, 25001], ids=str)
+def test_large_gradients(cuda_device, vocab):
+    """Gradients large enough to be written past the caches are those of a part of the rows, bit by bit."""
+    from isa.kernels.transformer_block import policy_loss, policy_loss_with_grad, preference_loss
+
+    x, t, old, a, _ = make(cuda_device, 3000, vocab, BF16, 4)
+    assert x.numel() * 2 >= 2 ** 27
+    t[400:] = -100
+    many = x.detach().requires_grad_(True)
+    few = x[:400].detach().requires_grad_(True)
+    (dx,) = torch.autograd.grad(policy_loss(many, t, old, a, reduction="sum")[0], many)
+    (part,) = torch.autograd.grad(policy_loss(few, t[:400], old[:400], a[:400], reduction="sum")[0], few)
+    assert torch.equal(dx[:400], part) and part.any() and torch.count_nonzero(dx[400:]) == 0
+    count = float((t[:400] != -100).sum())
+    _, dx, _ = policy_loss_with_grad(x, t, old, a, grad_scale=count)
+    _, part, _ = policy_loss_with_grad(x[:400], t[:400], old[:400], a[:400], grad_scale=count)
+    assert torch.equal(dx[:400], part) and part.any() and torch.count_nonzero(dx[400:]) == 0
+    # one chosen sequence of 1500 tokens, of which 400 count, against the same cut behind them
+    u = t.view(2, 1500)
+    (dx,) = torch.autograd.grad(preference_loss(many.view(2, 1500, vocab), u, old[:2], reduction="sum")[0], many)
+    cut = x.view(2, 1500, vocab)[:, :400].contiguous().requires_grad_(True)
+    (part,) = torch.autograd.grad(preference_loss(cut, u[:, :400].contiguous(), old[:2], reduction="sum")[0], cut)
+    assert torch.equal(dx.view(2, 1500, vocab)[:, :400], part) and part.any()
+    assert torch.count_nonzero(dx.view(2, 1500, vocab)[:, 400:]) == 0
