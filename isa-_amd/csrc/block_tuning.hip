@@ -37,6 +37,17 @@ struct PairArgs {
     float beta;
 };
 
+// The mean over the rows that are not ignored, which are counted here.
+__global__ __launch_bounds__(kMostThreads) void loss_mean_kernel(const float* row_loss, const int64_t* targets,
+                                                             int64_t rows, int64_t ignore, float* out) {
+    __shared__ float slots[2][kMostThreads / kWave];
+    float s = 0.0f;
+    for (int64_t r = threadIdx.x; r < rows; r += kMostThreads) s += row_loss[r];
+    const float n = block_count<kMostThreads>(targets, rows, ignore, slots[0]);
+    s = block_sum<kMostThreads>(s, slots[1]);
+    if (threadIdx.x == 0) out[0] = s / n;
+}
+
 __device__ __forceinline__ double wave_sum64(double x) {
 #pragma unroll
     for (int by = 1; by < kWave; by *= 2) x += __shfl_xor(x, by);
