@@ -32,7 +32,7 @@ typedef struct isa_train_embedding {
     float scale;
     int64_t places, places_stride; /* rows of the second table; 0: none */
     const int64_t* place_ids;      /* [tokens], or null */
-    int64_t period;                /* without place_ids: >= 1, divides tokens */
+    int64_t period;                /* of a second table without place_ids: >= 1, divides tokens */
     const void* place_weight;
 } isa_train_embedding;
 #define ISA_TRAIN_EMBEDDING_MAX_ROWS (1 << 24) /* of a table */

@@ -598,9 +598,10 @@ size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // One table's parts of the lists that a lookup leaves and of a backward call's workspace.
 struct Space {
-    int64_t tiles;
-    size_t starts, lists;         // bytes before the lists' starts, in all
-    size_t partial, workspace;    // bytes before the partial sums, in all
+    int64_t tiles = 0;
+    size_t starts = 0, lists = 0;       // bytes before the lists' starts, in all
+    size_t partial = 0, workspace = 0;  // bytes before the partial sums, in all
+    Space() = default;                  // of a table that is not there
     Space(int64_t tokens, int64_t rows, int64_t dim, bool few, bool keys, int64_t period) {
         const int tile = tile_of(tokens);
         // of few tokens a row's block takes longer ones; without keys all rows have one length
@@ -635,6 +636,7 @@ bool few_of(const isa_train_embedding* e) {
 
 Space space_of(const isa_train_embedding* e, bool places) {
     if (!places) return Space(e->tokens, e->vocab, e->dim, few_of(e), true, 1);
+    if (e->places == 0) return Space();  // whose period may be anything
     return Space(e->tokens, e->places, e->dim, few_of(e), e->place_ids != nullptr, e->tokens ? e->period : 1);
 }
 
