@@ -281,7 +281,7 @@ extern "C" int isa_train_policy_forward(const isa_train_policy* p, int reduction
     if (reduction < ISA_BLOCK_MEAN || reduction > ISA_BLOCK_NONE) return fail("unknown reduction %d", reduction);
     if (reduction == ISA_BLOCK_NONE && l->rows == 0) return 0;
     if (!out || (l->rows && !logp)) return fail("out and logp must be set");
-    if ((stats == nullptr) != (slope == nullptr) || (stats == nullptr) != (count == nullptr))
+    if (l->rows && ((stats == nullptr) != (slope == nullptr) || (stats == nullptr) != (count == nullptr)))
         return fail("stats, slope and count go together");
     if (int rc = check_workspace(l, workspace, workspace_bytes)) return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);
