@@ -10,6 +10,7 @@ from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
+from torch.nn.modules.module import _has_any_global_hook
 
 from isa.kernels.transformer_block import (add_layer_norm, dropout, dropout_add_layer_norm, embedding, layer_norm,
                                            window_attention)
@@ -52,6 +53,12 @@ class Embedding(nn.Embedding):
         the sum of both."""
         return embedding(ids, self.weight, scale=self.scale, positions=positions, position_weight=position_weight,
                          padding_index=self.padding_idx)
+
+
+def _operator_alone(table: nn.Module) -> bool:
+    """Whether a call of this table is `embedding` of its weight and nothing else: no hooks, no forward of a caller's."""
+    return (type(table) is Embedding and "forward" not in vars(table) and not _has_any_global_hook()
+            and not (table._forward_hooks or table._forward_pre_hooks or table._backward_hooks or table._backward_pre_hooks))
 
 
 class DropoutSeed:
@@ -213,9 +220,10 @@ class GPT(nn.Module):
 
     def _embed(self, ids: torch.Tensor, at: Optional[torch.Tensor]) -> torch.Tensor:
         tokens, positions = self.tokens, self.positions
-        if type(tokens) is type(positions) is Embedding and tokens.weight.dtype == positions.weight.dtype:
+        if (_operator_alone(tokens) and _operator_alone(positions) and positions.scale == 1.0
+                and positions.padding_idx is None and tokens.weight.dtype == positions.weight.dtype):
             return tokens(ids, at, positions.weight)
-        if at is None:  # a caller's own modules
+        if at is None:  # a caller's own modules, or tables that do more than one call of the operator does
             at = torch.arange(ids.shape[1], device=ids.device)
         return tokens(ids) + positions(at)
 
