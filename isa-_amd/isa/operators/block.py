@@ -178,8 +178,8 @@ class Block(nn.Module):
     """Norm, attention, norm, FFN. A branch's output joins the residual stream inside the next norm, so
     a block takes the last one's FFN output and the stream, and returns its own pair.
 
-    With `dropout` and a seed (`DropoutSeed.step`; none: no dropout, as for evaluation) the branches' outputs are dropped
-    as they join: the last block's under `site`, the own attention's under site + 1."""
+    With `dropout` and a seed (`DropoutSeed.step`; none: no dropout) a block that trains (its own flag says so) drops the
+    branches' outputs as they join: the last block's under `site`, the own attention's under site + 1."""
 
     def __init__(self, dim: int, attention: WindowAttention, ffn: nn.Module, dropout: float = 0.0):
         super().__init__()
@@ -189,6 +189,8 @@ class Block(nn.Module):
 
     def forward(self, branch: Optional[torch.Tensor], stream: torch.Tensor, cache: Optional[WindowCache] = None,
                 seed: Optional[torch.Tensor] = None, site: int = 0):
+        if not self.training:
+            seed = None
         y, stream = (self.ln1(stream), stream) if branch is None else _join(self.ln1, branch, stream, self.dropout, seed, site)
         y, stream = _join(self.ln2, self.attention(y, cache), stream, self.dropout, seed, site + 1)
         return self.ffn(y), stream
@@ -196,8 +198,9 @@ class Block(nn.Module):
 
 class GPT(nn.Module):
     """Token and position embeddings, blocks, a last norm and the tied output projection. `dropout` is that of the
-    embeddings and of the last block's output (the blocks have their own), while the model trains; its numbers follow
-    from `seed`, a DropoutSeed that the model makes when it first drops unless the caller sets one."""
+    embeddings and of the last block's output (the blocks have their own), while the model trains (its own flag, and the
+    blocks' for theirs); its numbers follow from `seed`, a DropoutSeed that the model makes when it first drops unless the
+    caller sets one."""
 
     def __init__(self, vocab: int, positions: int, dim: int, blocks: nn.ModuleList, dropout: float = 0.0):
         super().__init__()
@@ -211,8 +214,8 @@ class GPT(nn.Module):
             nn.init.normal_(table.weight, std=0.02)
 
     def _step(self, device: torch.device) -> Optional[torch.Tensor]:
-        """This pass's seed. Sites: the embeddings', two a block, the last block's output."""
-        if not self.training or not (self.dropout or any(getattr(block, "dropout", 0.0) for block in self.blocks)):
+        """This pass's seed, if any part drops. Sites: the embeddings', two a block, the last block's output."""
+        if not any(part.training and getattr(part, "dropout", 0.0) for part in (self, *self.blocks)):
             return None
         if self.seed is None:
             self.seed = DropoutSeed()
@@ -237,15 +240,16 @@ class GPT(nn.Module):
             at = caches[0].lengths.long()[:, None] + torch.arange(ids.shape[1], device=ids.device)
         seed = self._step(ids.device)
         branch, stream = None, self._embed(ids, at)
-        if seed is not None and self.dropout:
-            stream = dropout(stream, self.dropout, seed)
+        p = self.dropout if self.training else 0.0
+        if seed is not None and p:
+            stream = dropout(stream, p, seed)
         for i, block in enumerate(self.blocks):
             rest = {} if seed is None else {"seed": seed, "site": 1 + 2 * i}
             branch, stream = block(branch, stream, None if caches is None else caches[i], **rest)
         if branch is None:
             y = self.ln_f(stream)
         else:
-            y = _join(self.ln_f, branch, stream, self.dropout, seed, 1 + 2 * len(self.blocks))[0]
+            y = _join(self.ln_f, branch, stream, p, seed, 1 + 2 * len(self.blocks))[0]
         return nn.functional.linear(y, self.tokens.weight)
 
     def caches(self, batch: int, capacity: int, **options) -> list:
