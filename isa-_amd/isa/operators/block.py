@@ -6,6 +6,8 @@ from torch's operators (`nn.LayerNorm`, scaled-dot-product attention).
 
 from __future__ import annotations
 
+import inspect
+from numbers import Real
 from typing import Optional, Tuple
 
 import torch
@@ -196,11 +198,23 @@ class Block(nn.Module):
         return self.ffn(y), stream
 
 
+def _drops(part: nn.Module) -> bool:
+    p = getattr(part, "dropout", 0.0)  # of a caller's block: perhaps a module
+    return part.training and isinstance(p, Real) and p != 0.0
+
+
+def _takes_seed(block: nn.Module) -> bool:
+    if type(block) is Block:
+        return True
+    parameters = inspect.signature(block.forward).parameters.values()
+    return any(p.name == "seed" or p.kind is p.VAR_KEYWORD for p in parameters)
+
+
 class GPT(nn.Module):
     """Token and position embeddings, blocks, a last norm and the tied output projection. `dropout` is that of the
     embeddings and of the last block's output (the blocks have their own), while the model trains (its own flag, and the
     blocks' for theirs); its numbers follow from `seed`, a DropoutSeed that the model makes when it first drops unless the
-    caller sets one."""
+    caller sets one. Blocks of a caller's own whose forward has no `seed` get none."""
 
     def __init__(self, vocab: int, positions: int, dim: int, blocks: nn.ModuleList, dropout: float = 0.0):
         super().__init__()
@@ -215,7 +229,7 @@ class GPT(nn.Module):
 
     def _step(self, device: torch.device) -> Optional[torch.Tensor]:
         """This pass's seed, if any part drops. Sites: the embeddings', two a block, the last block's output."""
-        if not any(part.training and getattr(part, "dropout", 0.0) for part in (self, *self.blocks)):
+        if not (_drops(self) or any(_drops(block) and _takes_seed(block) for block in self.blocks)):
             return None
         if self.seed is None:
             self.seed = DropoutSeed()
@@ -244,7 +258,7 @@ class GPT(nn.Module):
         if seed is not None and p:
             stream = dropout(stream, p, seed)
         for i, block in enumerate(self.blocks):
-            rest = {} if seed is None else {"seed": seed, "site": 1 + 2 * i}
+            rest = {"seed": seed, "site": 1 + 2 * i} if seed is not None and _takes_seed(block) else {}
             branch, stream = block(branch, stream, None if caches is None else caches[i], **rest)
         if branch is None:
             y = self.ln_f(stream)
