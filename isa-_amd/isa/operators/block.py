@@ -67,8 +67,9 @@ class DropoutSeed:
     """The key and offset of a model's dropout, an int64 tensor [2] that moves to the device of the steps.
 
     A forward pass takes `step`: a copy for its calls, whose sites are 0 .. sites - 1, while the offset moves past them,
-    on the device, so that a HIP graph that recorded a step draws anew in each replay. key: drawn from torch's generator
-    unless given; ranks of one job take a key each. (Not a buffer of the model: those are made alike on all ranks.)"""
+    on the device, so that a HIP graph that recorded a step draws anew in each replay; the first step on a device, which
+    moves the state there, comes before any that is captured. key: drawn from torch's generator unless given; ranks of one
+    job take a key each. (Not a buffer of the model: those are made alike on all ranks.)"""
 
     def __init__(self, key: Optional[int] = None):
         with torch.inference_mode(False):  # it changes in place, in any mode
@@ -76,8 +77,14 @@ class DropoutSeed:
 
     @torch.no_grad()
     def step(self, sites: int, device: torch.device) -> torch.Tensor:
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
         with torch.inference_mode(False):
             if self.state.device != device:
+                # a recorded copy would read memory that is free by then, and set the offset back, in each replay
+                if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError(f"a dropout seed on {self.state.device} cannot move to {device} in a capture: take "
+                                       "a step there before one is captured")
                 self.state = self.state.to(device)
             seed = self.state.clone()
             self.state[1:].add_(sites)
