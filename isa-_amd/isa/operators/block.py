@@ -7,6 +7,7 @@ from torch's operators (`nn.LayerNorm`, scaled-dot-product attention).
 from __future__ import annotations
 
 import inspect
+import threading
 from numbers import Real
 from typing import Optional, Tuple
 
@@ -63,31 +64,58 @@ def _operator_alone(table: nn.Module) -> bool:
             and not (table._forward_hooks or table._forward_pre_hooks or table._backward_hooks or table._backward_pre_hooks))
 
 
+_ONE_STEP = threading.Lock()  # (of all seeds: one of its own could not be copied or pickled with a model)
+
+
 class DropoutSeed:
     """The key and offset of a model's dropout, an int64 tensor [2] that moves to the device of the steps.
 
     A forward pass takes `step`: a copy for its calls, whose sites are 0 .. sites - 1, while the offset moves past them,
     on the device, so that a HIP graph that recorded a step draws anew in each replay; the first step on a device, which
-    moves the state there, comes before any that is captured. key: drawn from torch's generator unless given; ranks of one
-    job take a key each. (Not a buffer of the model: those are made alike on all ranks.)"""
+    moves the state there, comes before any that is captured. Steps of several threads or streams come one after the
+    other; a graph's replays are ordered by who replays it.
+
+    key: drawn from torch's generator unless given; ranks of one job take a key each. (Not a buffer of the model: those
+    are made alike on all ranks, so no state dict has it. A run that is to go on where it stopped keeps `state` with its
+    checkpoint and copies it back; one that starts again under the same torch.manual_seed repeats its first masks.)"""
+
+    _stream = _done = None  # of the last eager step on a GPU, and its end
 
     def __init__(self, key: Optional[int] = None):
         with torch.inference_mode(False):  # it changes in place, in any mode
             self.state = torch.tensor([int(torch.randint(2 ** 62, ())) if key is None else key, 0])
 
+    def __getstate__(self) -> dict:
+        return {k: v for k, v in vars(self).items() if k not in ("_stream", "_done")}
+
+    def _wait(self) -> None:
+        if self._done is not None and self.state.is_cuda:
+            stream = torch.cuda.current_stream(self.state.device)
+            if stream != self._stream:
+                stream.wait_event(self._done)
+
     @torch.no_grad()
     def step(self, sites: int, device: torch.device) -> torch.Tensor:
         if device.type == "cuda" and device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
-        with torch.inference_mode(False):
+        recorded = device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+        with _ONE_STEP, torch.inference_mode(False):
+            if not recorded:
+                self._wait()
             if self.state.device != device:
                 # a recorded copy would read memory that is free by then, and set the offset back, in each replay
-                if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                if recorded:
                     raise RuntimeError(f"a dropout seed on {self.state.device} cannot move to {device} in a capture: take "
                                        "a step there before one is captured")
                 self.state = self.state.to(device)
             seed = self.state.clone()
             self.state[1:].add_(sites)
+            if device.type == "cuda" and not recorded:
+                stream = torch.cuda.current_stream(device)
+                if self._done is None or self._stream.device != stream.device:
+                    self._done = torch.cuda.Event()
+                self._done.record(stream)
+                self._stream = stream
         return seed
 
 
