@@ -8,22 +8,28 @@ namespace {
 // Autograd keeps a leaf's accumulator, with the stream it was made on, as long as a graph of that leaf lives. One of
 // the default stream would take part in a capture, which the runtime answers with an error in autograd's threads,
 // where it ends the process.
-void leaves_can_be_captured(std::initializer_list<const Tensor*> tensors) {
-    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-    for (const Tensor* t : tensors) {
-        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-        const auto stream = node ? node->stream() : std::nullopt;
-        if (stream && stream->id() == c10::hip::getDefaultHIPStream(t->device().index()).id())
-            refuse("a graph of a leaf lives that was made on the default stream: free it (the results that hold it), or "
-                   "make it on another stream, before a step with that leaf is captured");
-    }
+bool captured() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
+
+void leaf_can_be_captured(const Tensor& t) {
+    if (!t.defined() || !t.requires_grad() || !t.is_leaf()) return;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    const auto stream = node ? node->stream() : std::nullopt;
+    if (stream && stream->id() == c10::hip::getDefaultHIPStream(t.device().index()).id())
+        refuse("a graph of a leaf lives that was made on the default stream: free it (the results that hold it), or "
+               "make it on another stream, before a step with that leaf is captured");
 }
 
 bool recorded(std::initializer_list<const Tensor*> tensors) {
     if (!tracked(tensors)) return false;
-    leaves_can_be_captured(tensors);
+    if (captured())
+        for (const Tensor* t : tensors) leaf_can_be_captured(*t);
     return true;
+}
+
+// For a model that calls the operators unchecked: called in its backward pass, before that reaches a leaf.
+void leaves_can_be_captured(const std::vector<Tensor>& leaves) {
+    if (captured())
+        for (const Tensor& t : leaves) leaf_can_be_captured(t);
 }
 
 // Integer indices as contiguous int64.
@@ -127,8 +133,9 @@ struct Embedding : torch::autograd::Function<Embedding> {
     }
 };
 
+// unchecked: the caller answers for a backward pass that is captured (leaves_can_be_captured).
 Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, const Maybe& positions,
-                 const Maybe& position_weight, std::optional<int64_t> padding_index) {
+                 const Maybe& position_weight, std::optional<int64_t> padding_index, bool unchecked) {
     not_traced();
     require(weight, "weight");
     check_table(weight, "weight", 0);
@@ -158,7 +165,7 @@ Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, const Ma
     }
     no_tangents(std::array{std::cref(weight), std::cref(places)});
     const int64_t padding = padding_index.value_or(-1);
-    if (recorded({&weight, &places}))
+    if (unchecked ? tracked({&weight, &places}) : recorded({&weight, &places}))
         return Embedding::apply(weight, tokens, position_weight, place_ids.defined() ? Maybe(place_ids) : Maybe(), scale,
                                 padding);
     return std::get<0>(lookup(weight, places, {tokens, place_ids, scale, padding}, false, false));
@@ -556,6 +563,7 @@ void bind_training(pybind11::module_& m) {
     m.def("train_abi_version", &isa_train_abi_version);
     m.attr("TRAIN_ABI_VERSION") = ISA_TRAIN_ABI_VERSION;
     m.def("embedding", &embedding, Free());
+    m.def("leaves_can_be_captured", &leaves_can_be_captured, Free());
     m.def("dropout", &dropout, Free());
     m.def("dropout_add_layer_norm", &dropout_add_layer_norm, Free());
     m.def("policy_loss", &policy_loss, Free());

@@ -2,7 +2,7 @@
 
 from __future__ import annotations
 
-from typing import Optional, Tuple, Union
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -90,7 +90,19 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, po
     An id or a position outside its table makes its row NaN and takes no part in that table's gradient, nor does
     padding_index in weight's. The gradients (dense, shaped as the tables) are fp32 sums over the tokens sorted by row,
     rounded once, without atomics: the same call gives the same bits."""
-    return _binding.embedding(ids, weight, scale, positions, position_weight, padding_index)
+    return _binding.embedding(ids, weight, scale, positions, position_weight, padding_index, False)
+
+
+def unchecked_embedding(ids, weight, *, scale=1.0, positions=None, position_weight=None, padding_index=None) -> torch.Tensor:
+    """embedding for a model that calls leaves_can_be_captured in its backward pass: so a forward pass alone can be
+    captured whatever graphs of the tables live."""
+    return _binding.embedding(ids, weight, scale, positions, position_weight, padding_index, True)
+
+
+def leaves_can_be_captured(leaves: Sequence[torch.Tensor]) -> None:
+    """While a HIP graph is recorded: refuses leaves of which a graph made on the default stream still lives. A backward
+    pass that reached one would end the process."""
+    _binding.leaves_can_be_captured(list(leaves))
 
 
 def dropout(x: torch.Tensor, p: float, seed: torch.Tensor, *, site: int = 0) -> torch.Tensor:

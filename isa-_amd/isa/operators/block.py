@@ -17,6 +17,7 @@ from torch.nn.modules.module import _has_any_global_hook
 
 from isa.kernels.transformer_block import (add_layer_norm, dropout, dropout_add_layer_norm, embedding, layer_norm,
                                            window_attention)
+from isa.kernels.transformer_block.functions import leaves_can_be_captured, unchecked_embedding
 
 
 class LayerNorm(nn.LayerNorm):
@@ -51,17 +52,21 @@ class Embedding(nn.Embedding):
         self.scale = scale
 
     def forward(self, ids: torch.Tensor, positions: Optional[torch.Tensor] = None,
-                position_weight: Optional[torch.Tensor] = None) -> torch.Tensor:
+                position_weight: Optional[torch.Tensor] = None, *, operator=None) -> torch.Tensor:
         """With a table of positions (a place of its own for each token of a sequence unless `positions` are given)
-        the sum of both."""
-        return embedding(ids, self.weight, scale=self.scale, positions=positions, position_weight=position_weight,
-                         padding_index=self.padding_idx)
+        the sum of both. operator: `embedding` unless given."""
+        return (operator or embedding)(ids, self.weight, scale=self.scale, positions=positions,
+                                       position_weight=position_weight, padding_index=self.padding_idx)
+
+
+def _is_ours(table: nn.Module) -> bool:
+    return type(table) is Embedding and "forward" not in vars(table)
 
 
 def _operator_alone(table: nn.Module) -> bool:
     """Whether a call of this table is `embedding` of its weight and nothing else: no hooks, no forward of a caller's."""
-    return (type(table) is Embedding and "forward" not in vars(table) and not _has_any_global_hook()
-            and not (table._forward_hooks or table._forward_pre_hooks or table._backward_hooks or table._backward_pre_hooks))
+    return (_is_ours(table) and not _has_any_global_hook() and not (
+        table._forward_hooks or table._forward_pre_hooks or table._backward_hooks or table._backward_pre_hooks))
 
 
 _ONE_STEP = threading.Lock()  # (of all seeds: one of its own could not be copied or pickled with a model)
@@ -270,14 +275,15 @@ class GPT(nn.Module):
             self.seed = DropoutSeed()
         return self.seed.step(2 + 2 * len(self.blocks), device)
 
-    def _embed(self, ids: torch.Tensor, at: Optional[torch.Tensor]) -> torch.Tensor:
+    def _embed(self, ids: torch.Tensor, at: Optional[torch.Tensor], captured: bool = False) -> torch.Tensor:
         tokens, positions = self.tokens, self.positions
+        how = [{"operator": unchecked_embedding} if captured and _is_ours(table) else {} for table in (tokens, positions)]
         if (_operator_alone(tokens) and _operator_alone(positions) and positions.scale == 1.0
                 and positions.padding_idx is None and tokens.weight.dtype == positions.weight.dtype):
-            return tokens(ids, at, positions.weight)
+            return tokens(ids, at, positions.weight, **how[0])
         if at is None:  # a caller's own modules, or tables that do more than one call of the operator does
             at = torch.arange(ids.shape[1], device=ids.device)
-        return tokens(ids) + positions(at)
+        return tokens(ids, **how[0]) + positions(at, **how[1])
 
     def forward(self, ids: torch.Tensor, caches: Optional[list] = None) -> torch.Tensor:
         """Logits [batch, n, vocab]; with caches (one a block) ids continue their sequences."""
@@ -288,7 +294,8 @@ class GPT(nn.Module):
         if caches is not None:
             at = caches[0].lengths.long()[:, None] + torch.arange(ids.shape[1], device=ids.device)
         seed = self._step(ids.device)
-        branch, stream = None, self._embed(ids, at)
+        captured = ids.is_cuda and torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing()
+        branch, stream = None, self._embed(ids, at, captured)
         p = self.dropout if self.training else 0.0
         if seed is not None and p:
             stream = dropout(stream, p, seed)
@@ -299,7 +306,10 @@ class GPT(nn.Module):
             y = self.ln_f(stream)
         else:
             y = _join(self.ln_f, branch, stream, p, seed, 1 + 2 * len(self.blocks))[0]
-        return nn.functional.linear(y, self.tokens.weight)
+        logits = nn.functional.linear(y, self.tokens.weight)
+        if captured and logits.requires_grad:  # a forward pass may be captured beside any graph; a backward may not
+            logits.register_hook(lambda _: leaves_can_be_captured(self.parameters()))
+        return logits
 
     def caches(self, batch: int, capacity: int, **options) -> list:
         """Empty caches for generation."""
