@@ -157,8 +157,9 @@ __device__ __forceinline__ float sloped_share_of(const LossArgs& a, int64_t r) {
 
 // The policy loss of a row and its slope by l.
 __device__ __forceinline__ float policy(const LossArgs& a, int64_t r, float l, float& slope) {
-    const float ratio = expf(l - a.old_logp[r]), by = a.advantages[r];
-    const float free = ratio * by, held = fminf(fmaxf(ratio, a.low), a.high) * by;
+    const float moved = l - a.old_logp[r], ratio = expf(moved), by = a.advantages[r];
+    // (without an advantage 0, also of a ratio past fp32's largest number)
+    const float free = by == 0.0f && fabsf(moved) < INFINITY ? 0.0f : ratio * by, held = fminf(fmaxf(ratio, a.low), a.high) * by;
     float loss = -fminf(free, held);
     slope = free <= held ? -free : 0.0f;
     if (free != free) loss = slope = free;  // (the minimum of NaN and a number is the number)
