@@ -43,7 +43,7 @@ struct LossArgs {
     float low, high, kl;
     float* logp;      // [rows]
     float* row_slope;  // [rows], or null
-    double* row_logp;  // [rows], or null: l, 0 in ignored rows
+    double* row_logp;  // [rows], statistics alone: l, 0 in ignored rows
     bool count_here;   // each block counts the rows that are not ignored, for its gradient
     bool past;         // the gradient is written past the caches
 };
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(THREADS) void loss_kernel(LossArgs a) {
                 a.logp[r] = 0.0f;
                 if (a.row_slope) a.row_slope[r] = 0.0f;
             }
-            if (a.row_logp) a.row_logp[r] = 0.0;
+            if constexpr (OF == Of::kStats) a.row_logp[r] = 0.0;
         }
         if (grad)
             for (int c = threadIdx.x; c < chunks; c += THREADS) row.store(grad, c, typename R::Chunk{}, OF == Of::kPolicy && a.past);
@@ -271,8 +271,9 @@ __global__ __launch_bounds__(THREADS) void loss_kernel(LossArgs a) {
         const float log_sum = logf(sum);
         if (OF == Of::kCrossEntropy && a.row_loss)
             a.row_loss[r] = inside ? log_sum + (top - static_cast<float>(row.p[target])) : NAN;
-        // sums of it over a long sequence need more than its own rounding leaves
-        if (a.row_logp)
+        // sums of it over a long sequence need more than its own rounding leaves (for the statistics alone: a logarithm of
+        // 64 bits takes registers, and 16 more than 64 leave a compute unit to one row of the others)
+        if constexpr (OF == Of::kStats)
             a.row_logp[r] = inside ? static_cast<double>(static_cast<float>(row.p[target])) - top - log(static_cast<double>(sum))
                                    : NAN;
         if (a.stats) {
