@@ -139,7 +139,7 @@ Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, const Ma
     not_traced();
     require(weight, "weight");
     check_table(weight, "weight", 0);
-    if (!std::isfinite(scale)) refuse("scale must be finite, got ", scale);
+    if (!std::isfinite(static_cast<float>(scale))) refuse("scale must be finite in float32, got ", scale);
     if (padding_index && (*padding_index < 0 || *padding_index >= weight.size(0)))
         refuse("padding_index must be None or a row of weight (0 to ", weight.size(0) - 1, "), got ", *padding_index);
     const Tensor places = position_weight.value_or(Tensor());
