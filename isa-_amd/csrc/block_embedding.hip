@@ -11,7 +11,7 @@
 // A row with many tokens would be one wave's long walk: lists longer than a tile are summed by tiles of
 // the sorted list, in the rows' launch, and a third launch adds up their sums. Both tables share the launches.
 //
-// 65536 tokens of a 50304 x 1024 bf16 table: lookup with its sort 33 us (162 MB), rows and tiles 37 (237 MB, 6.4 TB/s),
+// 65536 tokens of a 50304 x 1024 bf16 table: lookup with its sort 31 us (162 MB), rows and tiles 37 (237 MB, 6.4 TB/s),
 // join 7; 8192 tokens of 50304 x 768 and 1024 x 768 in fp32: 13, 34 (207 MB) and 4.
 #include "block_common.hpp"
 

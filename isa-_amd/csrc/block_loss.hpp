@@ -7,7 +7,8 @@
 //
 // Bound by HBM: a row of logits is read once and its gradient written once. One block takes a
 // row and holds it in registers, as the 16-byte chunks that were loaded, between the maximum,
-// the sum and the gradient; rows too long for that are read again from the caches.
+// the sum and the gradient. Rows too long for that, of more than 16 chunks a thread (65500 elements of fp32, 131000 of
+// 16 bits), are read again, in part from the last cache: 4096 x 128256 in fp32 1012 us, 6.2 TB/s of three transfers.
 #pragma once
 
 #include "block_common.hpp"
